@@ -20,6 +20,7 @@
 #include "../../include/etxb200.h"
 #include "etxb_kernel.cuh"
 #include "etxb_gemv_nb.cuh"
+#include "etxb_host.h"
 
 static_assert(sizeof(etxb_gemv_args) == 160 && offsetof(etxb_gemv_args, grid) == 144, "GEMV block layout (etx/ops/gemv.py:80-94)");
 static_assert(sizeof(etxb_topk_args) == 64 && offsetof(etxb_topk_args, grid) == 48, "top-k block layout (etx/ops/topk.py:16-23)");
@@ -36,6 +37,10 @@ static_assert(ETXB_NBR_OFF + 2 * ETXB_NB_ROWS * ETXB_NBC * 4 <= ETXB_GEN_BYTES &
 
 static thread_local std::string g_err;
 static int32_t fail(int32_t code, const std::string& msg) { g_err = msg; return code; }
+int32_t etxb_host_fail(int32_t code, const char* msg) noexcept {
+  try { g_err = msg; } catch (...) { g_err.clear(); }
+  return code;
+}
 #define CU(call)                                                                                         \
   do {                                                                                                   \
     cudaError_t e_ = (call);                                                                             \

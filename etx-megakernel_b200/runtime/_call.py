@@ -1,0 +1,37 @@
+"""What the operators beside the step share: checks of tensors, and the stream of a call."""
+from __future__ import annotations
+
+import torch
+
+
+def cuda_tensor(name: str, t, dtypes, shape=None, inner: bool = True):
+    """`t` as a CUDA tensor of one of `dtypes`; `shape` with None for sizes that are free; inner: the last dimension's elements adjoin."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor, got {getattr(t, 'device', type(t).__name__)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: dtype {t.dtype} is none of {', '.join(str(d) for d in dtypes)}")
+    if shape is not None and (t.dim() != len(shape) or any(w is not None and w != s for w, s in zip(shape, t.shape))):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple('any' if w is None else w for w in shape)}")
+    if inner and t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the elements of the last dimension adjoin (stride {t.stride(-1)})")
+    return t
+
+
+def same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the call runs on {device}")
+
+
+def stream_handle(device, stream, tensors) -> int:
+    """The raw handle of the call's stream: the current one of `device`, or `stream` (a raw handle or a torch stream), which the tensors' memory is then
+    kept for until it has passed the call."""
+    if stream is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    handle = int(getattr(stream, "cuda_stream", stream))
+    if handle != torch.cuda.current_stream(device).cuda_stream:
+        s = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+        for t in tensors:
+            if t is not None:
+                t.record_stream(s)
+    return handle

@@ -14,8 +14,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parents[1]
 CSRC = PKG / "csrc"
 LIB_PATH = PKG / "libetxb200.so"
-SOURCES = ["etxb.cu"]
-HEADERS = ["etxb_abi.h", "etxb_prims.cuh", "etxb_gemv.cuh", "etxb_gemv_nb.cuh", "etxb_attn.cuh", "etxb_attn_fused.cuh", "etxb_attn_gq.cuh", "etxb_batch.cuh", "etxb_tc.cuh", "etxb_mla.cuh", "etxb_kernel.cuh"]
+SOURCES = ["etxb.cu", "etxb_sample.cu"]
+HEADERS = ["etxb_abi.h", "etxb_prims.cuh", "etxb_gemv.cuh", "etxb_gemv_nb.cuh", "etxb_attn.cuh", "etxb_attn_fused.cuh", "etxb_attn_gq.cuh", "etxb_batch.cuh", "etxb_tc.cuh", "etxb_mla.cuh", "etxb_kernel.cuh", "etxb_host.h", "../../include/etxb200.h"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-fmad=false",
               "-shared", "-Xcompiler", "-fPIC"]
 
@@ -28,7 +28,8 @@ BODY = {"nop": 0, "prologue": 1, "argmax": 2, "gemv": 3, "moe_up": 4, "moe_down"
 SYMBOLS = ["etxb_version", "etxb_last_error", "etxb_device_info", "etxb_create", "etxb_bind", "etxb_set_step", "etxb_set_option",
            "etxb_launch", "etxb_launch_unfused", "etxb_wait", "etxb_step", "etxb_status", "etxb_trace", "etxb_exec_counts", "etxb_destroy",
            "etxb_decode_host", "etxb_op_launch", "etxb_attn_fused_static", "etxb_exchange_alloc", "etxb_exchange_free", "etxb_exchange_open",
-           "etxb_exchange_close", "etxb_set_exchange"]
+           "etxb_exchange_close", "etxb_set_exchange", "etxb_sample"]
+DTYPES = {"bf16": 0, "f16": 1, "f32": 2}
 IPC_HANDLE_BYTES = 64
 
 
@@ -55,6 +56,12 @@ class DeviceInfo(C.Structure):
                 ("cc_minor", C.c_int32), ("workers", C.c_int32), ("threads", C.c_int32), ("smem_bytes", C.c_int32), ("hbm_bytes", C.c_uint64)]
 
 
+class SampleArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "u", "temperature", "top_k", "top_p", "min_p", "tokens", "next", "logprobs", "kept")] + \
+               [("row_stride", C.c_int64), ("rows", C.c_int32), ("V", C.c_int32), ("dtype", C.c_int32), ("top_k_all", C.c_int32),
+                ("temperature_all", C.c_float), ("top_p_all", C.c_float), ("min_p_all", C.c_float), ("reserved", C.c_int32)]
+
+
 def needs_build() -> bool:
     if not LIB_PATH.exists():
         return True
@@ -67,12 +74,30 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not needs_build():
         return LIB_PATH
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
-    cmd = [nvcc, *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-o", str(LIB_PATH), *[str(CSRC / s) for s in SOURCES]]
+    (PKG / "build").mkdir(exist_ok=True)
+    flags = [*NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else [])]
+    objects = [PKG / "build" / (Path(s).stem + ".o") for s in SOURCES]
+    newest = max((CSRC / f).stat().st_mtime for f in HEADERS)
+    jobs = []                                                     # one nvcc per stale source, side by side
+    for s, o in zip(SOURCES, objects):
+        if force or not o.exists() or o.stat().st_mtime < max(newest, (CSRC / s).stat().st_mtime):
+            cmd = [nvcc, *[f for f in flags if f != "-shared"], "-c", "-o", str(o), str(CSRC / s)]
+            jobs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    log = ""
+    failed = None
+    for cmd, p in jobs:
+        out = p.communicate()[0]
+        log += out
+        if p.returncode != 0:
+            failed = failed or (cmd, out)
+    if failed:
+        raise RuntimeError("nvcc failed:\n" + " ".join(failed[0]) + "\n" + failed[1])
+    cmd = [nvcc, *NVCC_FLAGS, "-o", str(LIB_PATH), *map(str, objects)]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
     if verbose:
-        print(r.stderr)
+        print(log)
     return LIB_PATH
 
 
@@ -104,6 +129,7 @@ def load():
         "etxb_exchange_alloc": [C.c_int, sz, C.POINTER(vp), vp], "etxb_exchange_free": [C.c_int, vp],
         "etxb_exchange_open": [C.c_int, vp, C.POINTER(vp)], "etxb_exchange_close": [C.c_int, vp],
         "etxb_set_exchange": [vp, i32, i32, vp, sz, C.POINTER(vp)],
+        "etxb_sample": [C.c_int, C.POINTER(SampleArgs), sz, vp],
     }
     for name, args in proto.items():
         fn = getattr(lib, name)

@@ -1,0 +1,79 @@
+"""Drawing tokens from logits on the device (etxb_sample): temperature, top-k, top-p and min-p, with given random numbers.
+
+No counterpart in the reference, whose host loop is greedy (examples/vllm_llm/vl_tiles.hip:47-89)."""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from typing import NamedTuple
+
+import torch
+
+from . import lib as L
+from ._call import cuda_tensor, same_device, stream_handle
+
+_DT = {torch.bfloat16: L.DTYPES["bf16"], torch.float16: L.DTYPES["f16"], torch.float32: L.DTYPES["f32"]}
+MAX_V = 524288
+
+
+class Sampled(NamedTuple):
+    tokens: torch.Tensor       # int32 [rows]; -1 where no token of a row is allowed
+    logprobs: torch.Tensor     # float32 [rows]: of the token among the kept ones
+    kept: torch.Tensor         # int32 [rows]: how many tokens the cuts left
+
+
+@dataclass(frozen=True)
+class Sampling:
+    """How a program draws its tokens: the settings of `sample` (numbers, or tensors of one value per sequence) and the seed of the random numbers."""
+    temperature: object = 1.0
+    top_k: object = 0
+    top_p: object = 1.0
+    min_p: object = 0.0
+    seed: int = 0
+
+    def numbers(self, steps: int, rows: int, device) -> torch.Tensor:
+        """The random numbers of a run: [steps][rows] in [0, 1)."""
+        return torch.rand((steps, rows), device=device, generator=torch.Generator(device=device).manual_seed(self.seed))
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=None, next_tokens=None, stream=None) -> Sampled:
+    """One token per row of `logits` [rows][V] (bf16, fp16 or fp32; rows may lie further apart), drawn with u [rows] in [0, 1).
+
+    A row's allowed tokens (neither -inf nor NaN) stand in the order "larger logit first, equal ones by index" with the weights
+    exp((logit - largest) / temperature).  top_k keeps the first so many (0: all); top_p of those the ones with less than its share of their sum before
+    them (1: all); min_p the ones of at least that share of the largest weight (0: all); one is always kept.  The token is the first whose sum up to and
+    with itself exceeds u times the sum of the kept ones.  temperature 0: the largest logit.  Equal inputs give equal tokens, whatever else runs.
+
+    temperature, top_k, top_p, min_p: numbers, or tensors [rows] (float32; top_k int32).  tokens / next_tokens: int32 tensors [rows] that take the tokens
+    (the second one them once more: the next step's input).  stream: a raw handle or torch stream; None is the current one."""
+    cuda_tensor("logits", logits, tuple(_DT), (None, None))
+    rows, V = logits.shape
+    if not 1 <= V <= MAX_V:
+        raise ValueError(f"logits: {V} tokens outside 1..{MAX_V}")
+    if rows > 1 and logits.stride(0) < V:
+        raise ValueError(f"logits: rows overlap (stride {logits.stride(0)} below {V})")
+    dev = logits.device
+    cuda_tensor("u", u, (torch.float32,), (rows,))
+    a = L.SampleArgs(logits=logits.data_ptr(), u=u.data_ptr(), row_stride=max(logits.stride(0), V) if rows > 1 else V, rows=rows, V=V, dtype=_DT[logits.dtype])
+    keep = [logits, u]
+    for name, v, dt, cast in (("temperature", temperature, torch.float32, float), ("top_k", top_k, torch.int32, int), ("top_p", top_p, torch.float32, float),
+                              ("min_p", min_p, torch.float32, float)):
+        if isinstance(v, torch.Tensor):
+            cuda_tensor(name, v, (dt,), (rows,))
+            setattr(a, name, v.data_ptr())
+            keep.append(v)
+        else:
+            setattr(a, name + "_all", min(cast(v), MAX_V) if cast is int else cast(v))
+    same_device(dev, u=u, **{f"setting {i}": t for i, t in enumerate(keep[2:])})
+    for name, t in (("tokens", tokens), ("next_tokens", next_tokens)):
+        if t is not None:
+            cuda_tensor(name, t, (torch.int32,), (rows,))
+            same_device(dev, **{name: t})
+    if tokens is None:
+        tokens = torch.empty(rows, dtype=torch.int32, device=dev)
+    logprobs, kept = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.int32, device=dev)
+    a.tokens, a.logprobs, a.kept = tokens.data_ptr(), logprobs.data_ptr(), kept.data_ptr()
+    a.next = next_tokens.data_ptr() if next_tokens is not None else None
+    handle = stream_handle(dev, stream, keep + [tokens, next_tokens, logprobs, kept])
+    L.check(L.load().etxb_sample(dev.index, C.byref(a), C.sizeof(a), C.c_void_p(handle)))
+    return Sampled(tokens, logprobs, kept)

@@ -203,6 +203,38 @@ int32_t etxb_op_launch(int device, int32_t body, const void* argblock, size_t by
  * stream capture.  All calls share the array; calls that overlap on the GPU race on it.  Asynchronous on the stream. */
 int32_t etxb_attn_fused_static(int device, const void* argblock, size_t bytes, void* cuda_stream);
 
+/* ---- several answers to one prompt --------------------------------------------------------------------------------
+ * Three operators beside the step: tokens drawn from its logits, pages of its KV cache shared by several sequences, and decode attention that reads
+ * what they share once.  They own nothing and keep nothing between calls: all memory is the caller's, a call is asynchronous on its stream (0: the
+ * default stream), may be captured into a graph, and runs on `device` whatever device is current.  `bytes` = sizeof of the argument structure. */
+enum { ETXB_BF16 = 0, ETXB_F16 = 1, ETXB_F32 = 2 };
+
+/* One token per row of logits.  The live tokens of a row (neither -inf nor NaN) in the order "larger logit first, equal ones by index", token r
+ * weighted w_r = exp((l_r - l_0) / temperature): top-k keeps the first k (k < 1: all), top-p of those the ones with less than p times their sum before
+ * them (p not below 1: all), min-p the ones with w_r >= min_p (not above 0: all); at least one is kept.  Drawn is the first token whose inclusive
+ * sum exceeds u times the sum of the kept ones.  temperature not above 0: the first of the order.  u is taken as within [0, 1 - 2^-24].  A row without a
+ * live token: token -1, log-probability -inf, kept 0.
+ * Weights are summed as integers in steps of 2^-43 of the largest or finer: the outcome depends on no order of execution. */
+#define ETXB_SAMPLE_MAX_V 524288
+typedef struct etxb_sample_args {
+  const void* logits;          /* [rows][V], row_stride elements apart */
+  const float* u;              /* [rows] */
+  const float* temperature;    /* [rows], or null: temperature_all for every row; the same for the next three */
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int32_t* tokens;             /* [rows] */
+  int32_t* next;               /* [rows], the tokens once more (the next step's input), may be null */
+  float* logprobs;             /* [rows] log-probability of the token among the kept ones, may be null */
+  int32_t* kept;               /* [rows] number of tokens kept, may be null */
+  int64_t row_stride;
+  int32_t rows, V, dtype;      /* dtype: ETXB_BF16, ETXB_F16, ETXB_F32 */
+  int32_t top_k_all;
+  float temperature_all, top_p_all, min_p_all;
+  int32_t reserved;            /* 0 */
+} etxb_sample_args;
+int32_t etxb_sample(int device, const etxb_sample_args* args, size_t bytes, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

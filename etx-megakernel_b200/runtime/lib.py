@@ -14,7 +14,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parents[1]
 CSRC = PKG / "csrc"
 LIB_PATH = PKG / "libetxb200.so"
-SOURCES = ["etxb.cu", "etxb_sample.cu"]
+SOURCES = ["etxb.cu", "etxb_sample.cu", "etxb_pages.cu", "etxb_attn_shared.cu"]
 HEADERS = ["etxb_abi.h", "etxb_prims.cuh", "etxb_gemv.cuh", "etxb_gemv_nb.cuh", "etxb_attn.cuh", "etxb_attn_fused.cuh", "etxb_attn_gq.cuh", "etxb_batch.cuh", "etxb_tc.cuh", "etxb_mla.cuh", "etxb_kernel.cuh", "etxb_host.h", "../../include/etxb200.h"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-fmad=false",
               "-shared", "-Xcompiler", "-fPIC"]
@@ -28,7 +28,8 @@ BODY = {"nop": 0, "prologue": 1, "argmax": 2, "gemv": 3, "moe_up": 4, "moe_down"
 SYMBOLS = ["etxb_version", "etxb_last_error", "etxb_device_info", "etxb_create", "etxb_bind", "etxb_set_step", "etxb_set_option",
            "etxb_launch", "etxb_launch_unfused", "etxb_wait", "etxb_step", "etxb_status", "etxb_trace", "etxb_exec_counts", "etxb_destroy",
            "etxb_decode_host", "etxb_op_launch", "etxb_attn_fused_static", "etxb_exchange_alloc", "etxb_exchange_free", "etxb_exchange_open",
-           "etxb_exchange_close", "etxb_set_exchange", "etxb_sample"]
+           "etxb_exchange_close", "etxb_set_exchange", "etxb_sample", "etxb_pages_update",
+           "etxb_attn_shared", "etxb_attn_shared_work"]
 DTYPES = {"bf16": 0, "f16": 1, "f32": 2}
 IPC_HANDLE_BYTES = 64
 
@@ -60,6 +61,23 @@ class SampleArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("logits", "u", "temperature", "top_k", "top_p", "min_p", "tokens", "next", "logprobs", "kept")] + \
                [("row_stride", C.c_int64), ("rows", C.c_int32), ("V", C.c_int32), ("dtype", C.c_int32), ("top_k_all", C.c_int32),
                 ("temperature_all", C.c_float), ("top_p_all", C.c_float), ("min_p_all", C.c_float), ("reserved", C.c_int32)]
+
+
+class PageTensor(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p)] + [(n, C.c_int64) for n in ("src_layer", "src_page", "dst_layer", "dst_page", "page_bytes")]
+
+
+class PagesArgs(C.Structure):
+    _fields_ = [("t", PageTensor * 4), ("n_tensors", C.c_int32), ("layers", C.c_int32), ("src_pages", C.c_int32), ("dst_pages", C.c_int32),
+                ("src_ids", C.c_void_p), ("dst_ids", C.c_void_p), ("tables", C.c_void_p), ("table_stride", C.c_int64)] + \
+               [(n, C.c_void_p) for n in ("set_rows", "set_cols", "set_pages", "share_rows", "remap_rows", "remap_entries")] + \
+               [(n, C.c_int32) for n in ("n_copy", "table_rows", "table_width", "n_set", "n_share", "share_from", "shared", "n_remap")]
+
+
+class AttnSharedArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out", "kc", "vc", "tables", "lens", "prefix_tables", "prefix_lens", "group_first", "status", "work")] + \
+               [("work_bytes", C.c_size_t)] + [(n, C.c_int64) for n in ("q_stride", "out_stride", "k_stride", "v_stride", "table_stride", "prefix_stride")] + \
+               [(n, C.c_int32) for n in ("seqs", "groups", "NH", "NKV", "HD", "pages", "table_width", "prefix_width")] + [("scale", C.c_float), ("reserved", C.c_int32)]
 
 
 def needs_build() -> bool:
@@ -129,7 +147,8 @@ def load():
         "etxb_exchange_alloc": [C.c_int, sz, C.POINTER(vp), vp], "etxb_exchange_free": [C.c_int, vp],
         "etxb_exchange_open": [C.c_int, vp, C.POINTER(vp)], "etxb_exchange_close": [C.c_int, vp],
         "etxb_set_exchange": [vp, i32, i32, vp, sz, C.POINTER(vp)],
-        "etxb_sample": [C.c_int, C.POINTER(SampleArgs), sz, vp],
+        "etxb_sample": [C.c_int, C.POINTER(SampleArgs), sz, vp], "etxb_pages_update": [C.c_int, C.POINTER(PagesArgs), sz, vp],
+        "etxb_attn_shared": [C.c_int, C.POINTER(AttnSharedArgs), sz, vp], "etxb_attn_shared_work": [C.c_int, C.POINTER(AttnSharedArgs), sz, C.POINTER(sz)],
     }
     for name, args in proto.items():
         fn = getattr(lib, name)

@@ -235,6 +235,56 @@ typedef struct etxb_sample_args {
 } etxb_sample_args;
 int32_t etxb_sample(int device, const etxb_sample_args* args, size_t bytes, void* cuda_stream);
 
+/* Pages of a paged KV cache.  One call copies pages (of all layers and tensors: keys, values) and brings block tables up to date; the lists are host
+ * memory, are checked (ETXB_E_ARG) and copied before the call returns, and the device needs none of its own.
+ *   copies    page dst_ids[i] := page src_ids[i] of every tensor and layer.  Within one pool no page is both read and written; no page is written twice.
+ *   set       tables[set_rows[i]][set_cols[i]] := set_pages[i]
+ *   share     the first `shared` entries of each of share_rows := those of row share_from
+ *   remap     in the first remap_entries[i] entries of row remap_rows[i], a page that is a source of the copies gets the number it was copied to (a call
+ *             without set and share) */
+#define ETXB_PAGES_MAX_TENSORS 4
+typedef struct etxb_page_tensor {
+  const void* src; void* dst;                             /* the pools: page p of layer l lies at base + l * layer + p * page (bytes, multiples of 16) */
+  int64_t src_layer, src_page, dst_layer, dst_page;
+  int64_t page_bytes;
+} etxb_page_tensor;
+typedef struct etxb_pages_args {
+  etxb_page_tensor t[ETXB_PAGES_MAX_TENSORS];
+  int32_t n_tensors, layers, src_pages, dst_pages;
+  const int32_t* src_ids; const int32_t* dst_ids;         /* [n_copy] */
+  int32_t* tables; int64_t table_stride;                  /* device memory: [table_rows][table_width], rows table_stride entries apart */
+  const int32_t* set_rows; const int32_t* set_cols; const int32_t* set_pages;   /* [n_set] */
+  const int32_t* share_rows;                              /* [n_share] */
+  const int32_t* remap_rows; const int32_t* remap_entries;/* [n_remap] */
+  int32_t n_copy, table_rows, table_width, n_set, n_share, share_from, shared, n_remap;
+} etxb_pages_args;
+int32_t etxb_pages_update(int device, const etxb_pages_args* args, size_t bytes, void* cuda_stream);
+
+/* Decode attention of one layer for sequences that share prefixes: group g has a block table and a length of the positions its sequences have in
+ * common, each sequence a table and a length of its own ones behind them (the new position's key and value are in the cache already, and counted).
+ * Caches as in the step: keys [pages][NKV][HD / 8][16][8], values [pages][NKV][HD][16], bf16.  The keys and values of a prefix are read once for all
+ * sequences of its group.  A sequence without a position has the output 0.
+ * A page outside the cache or a length outside its table makes the outputs of the sequences it concerns NaN and sets a bit of *status (which no call
+ * clears); nothing outside the buffers is read. */
+#define ETXB_SHARED_MAX_SEQS 1024
+enum { ETXB_SHARED_BAD_PAGE = 1, ETXB_SHARED_BAD_LENGTH = 2 };
+typedef struct etxb_attn_shared_args {
+  const void* q; void* out;                               /* bf16 [seqs][NH][HD], q_stride / out_stride elements between sequences */
+  const void* kc; const void* vc;                         /* k_stride / v_stride elements between pages */
+  const int32_t* tables; const int32_t* lens;             /* device: [seqs][table_width] (rows table_stride apart), [seqs] */
+  const int32_t* prefix_tables; const int32_t* prefix_lens;   /* device: [groups][prefix_width] (rows prefix_stride apart), [groups] */
+  const int32_t* group_first;                             /* host: [groups + 1], the sequences of group g are group_first[g] .. group_first[g + 1] - 1 */
+  int32_t* status;                                        /* device, may be null */
+  void* work; size_t work_bytes;                          /* device memory of the call alone, as much as etxb_attn_shared_work says */
+  int64_t q_stride, out_stride, k_stride, v_stride, table_stride, prefix_stride;
+  int32_t seqs, groups, NH, NKV, HD, pages, table_width, prefix_width;
+  float scale;
+  int32_t reserved;
+} etxb_attn_shared_args;
+int32_t etxb_attn_shared(int device, const etxb_attn_shared_args* args, size_t bytes, void* cuda_stream);
+/* The bytes of `work` a call with these sizes needs (pointers are not looked at). */
+int32_t etxb_attn_shared_work(int device, const etxb_attn_shared_args* args, size_t bytes, size_t* work_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,7 +12,7 @@ from . import lib as L
 from ._call import cuda_tensor, same_device, stream_handle
 
 MAX_SEQS = 1024
-_BAD = {1: "a table names a page outside the cache", 2: "a length lies outside its table"}
+_BAD = {1: "a table names a page outside the cache", 2: "a length lies outside its table", 4: "a wait inside the kernel ran past two seconds"}
 
 
 def attn_shared(q, kc, vc, tables, lens, prefix_tables, prefix_lens, groups=None, scale=None, out=None, status=None, stream=None):
@@ -80,4 +80,4 @@ def attn_shared_check(status) -> None:
     """Raises what `status` has recorded (waits for its device)."""
     v = int(status.item())
     if v:
-        raise L.EtxbError(1, "attn_shared: " + "; ".join(text for bit, text in _BAD.items() if v & bit))
+        raise L.EtxbError(5 if v & 4 else 1, "attn_shared: " + "; ".join(text for bit, text in _BAD.items() if v & bit))

@@ -267,7 +267,7 @@ int32_t etxb_pages_update(int device, const etxb_pages_args* args, size_t bytes,
  * A page outside the cache or a length outside its table makes the outputs of the sequences it concerns NaN and sets a bit of *status (which no call
  * clears); nothing outside the buffers is read. */
 #define ETXB_SHARED_MAX_SEQS 1024
-enum { ETXB_SHARED_BAD_PAGE = 1, ETXB_SHARED_BAD_LENGTH = 2 };
+enum { ETXB_SHARED_BAD_PAGE = 1, ETXB_SHARED_BAD_LENGTH = 2, ETXB_SHARED_GAVE_UP = 4 };   /* 4: a wait inside the kernel ran past two seconds */
 typedef struct etxb_attn_shared_args {
   const void* q; void* out;                               /* bf16 [seqs][NH][HD], q_stride / out_stride elements between sequences */
   const void* kc; const void* vc;                         /* k_stride / v_stride elements between pages */

@@ -74,6 +74,7 @@ class Case:
 
     def check(self, out=None, **kw):
         out = self.run(**kw) if out is None else out
+        assert out.shape[0] == len(self.lens_)
         want, vmax = self.want(kw.get("scale"))
         err = (out.double().view(want.shape) - want).abs()
         bound = want.abs() * 2.0 ** -8 + vmax * 2.0 ** -12
@@ -101,6 +102,15 @@ def test_lengths_of_the_prefix(plen):
 @pytest.mark.parametrize("own", [0, 1, 16, 100, 3000])
 def test_nothing_shared(own):
     Case(8, 4, 64, [3], [0], [own, own // 2, own], seed=own).check()
+
+
+@pytest.mark.parametrize("NH,NKV,HD,plen,own", [(8, 8, 64, 60001, [59, 422]), (16, 1, 128, 300011, [1, 40, 7]), (8, 2, 256, 30003, [5, 33]), (32, 8, 128, 9000, [4001, 5, 17, 3000, 900])])
+def test_shares_of_many_tiles(NH, NKV, HD, plen, own):
+    """Shares of tens of tiles that end inside a page and go on with short contexts."""
+    c = Case(NH, NKV, HD, [len(own)], [plen], own, seed=plen)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    c.check(status=status)
+    attn_shared_check(status)
 
 
 def test_groups_of_all_sizes():

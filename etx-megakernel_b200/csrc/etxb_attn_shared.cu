@@ -32,8 +32,8 @@
 
 namespace etxb_shared {
 
-constexpr int BS = 16, ROWS = 128, SLOTS = 4, SLOT_BYTES = 32768;
-constexpr int W_COPY = 4, W_MMA = 5, W_Q = 6, THREADS = 256;     // (softmax: 0 .. 3; the last one clears)
+constexpr int BS = 16, ROWS = 128, SLOT_BYTES = 32768, OWN_ROWS = 16;
+constexpr int SM_WARPS = 8, W_COPY = 8, W_QK = 9, W_PV = 10, W_Q = 11, THREADS = 384;
 constexpr unsigned long long WAIT_NS = 2000000000ull;
 
 struct Groups { int32_t first[ETXB_SHARED_MAX_SEQS + 1]; };
@@ -44,10 +44,12 @@ struct Layout {
   int tp;                     // positions of a tile
   int workers;
   int prows;                  // rows of a slot of a prefix
+  int punits;                 // units of prefixes, counted generously (see prefix_unit); a unit's parts lie in the slots unit + worker
   long long pslots, oslots;   // slots of prefixes / of own positions
   float* pO; float* pml; float* oO; float* oml;      // [slot][HD / 4][rows][4], [slot][rows][2] (m in units of log2, l)
   int32_t* hdr;               // [pslots + oslots]: status bits of a segment
-  int32_t* state;             // [workers]: not 0 where a worker gave up
+  int32_t* gave_up;           // [workers]: not 0 where one did
+  int32_t* of;                // [units][2]: first and last worker that has tiles of a unit
 };
 
 struct Params {
@@ -74,17 +76,19 @@ __device__ __forceinline__ unsigned long long now_ns() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-// Waits for phase `n` (0, 1, ..) of a barrier; false, for everyone from then on, when it takes two seconds.
+// Waits for phase `n` (0, 1, ..) of a barrier; false, for everyone from then on, when it takes two seconds.  (The clock is looked at once in 256 tries:
+// reading it takes longer than most waits.)
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t n, volatile int* stop) {
-  if (bar_try(b, n & 1)) return true;
-  const unsigned long long t0 = now_ns();
-  for (uint32_t i = 1;; ++i) {
-    if (bar_try(b, n & 1)) return true;
-    if ((i & 15) == 0) {
+  unsigned long long t0 = 0;
+  for (uint32_t i = 1; !bar_try(b, n & 1); ++i) {
+    if ((i & 255) == 0) {
+      const unsigned long long t = now_ns();
+      if (t0 == 0) t0 = t;
       if (*stop) return false;
-      if (now_ns() - t0 > WAIT_NS) { *stop = 1; return false; }
+      if (t - t0 > WAIT_NS) { *stop = 1; return false; }
     }
   }
+  return true;
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
@@ -103,6 +107,13 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accum) : "memory");
+}
+// The same, adding to what is in d.
+__device__ __forceinline__ void mma_ss_add(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+}
+__device__ __forceinline__ void mma_ts_add(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc) : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -141,24 +152,32 @@ __device__ __forceinline__ float ex2(float x) {
 // ------------------------------------------------------------------------------------------------ shares
 // Tiles before group g / sequence b in the order of all tiles: the prefixes' units (group, kv head, rows), then the sequences' (sequence, kv head).
 struct Cum {
-  int32_t p[ETXB_SHARED_MAX_SEQS + 1], s[ETXB_SHARED_MAX_SEQS + 1];
+  int32_t* p;                 // [groups + 1]
+  int32_t* s;                 // [seqs + 1]
+  int32_t* len;               // [groups], [seqs]
 };
 __device__ __forceinline__ bool bad_length(int len, int width) { return len < 0 || len > width * BS; }
 __device__ __forceinline__ int tiles_of(int len, int width, int tp) { return bad_length(len, width) ? 0 : (len + tp - 1) / tp; }
 __device__ __forceinline__ int units_of(const Params& P, int g) { return (P.groups.first[g + 1] - P.groups.first[g] + P.y.spt - 1) / P.y.spt; }
 
-// Fills c (threads 0 .. 63 of the block; the caller's barrier follows).
-__device__ void cumulate(const Params& P, Cum& c) {
+// Fills c (warps 0 and 1; the caller's barrier follows).
+__device__ __forceinline__ void cumulate(const Params& P, const Cum& c) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp > 1) return;
   const etxb_attn_shared_args& a = P.a;
-  const int n = warp == 0 ? a.groups : a.seqs;
+  const int n = warp == 0 ? a.groups : a.seqs, width = warp == 0 ? a.prefix_width : a.table_width;
+  const int32_t* lens = warp == 0 ? a.prefix_lens : a.lens;
   int32_t* out = warp == 0 ? c.p : c.s;
+  int32_t* len = warp == 0 ? c.len : c.len + a.groups;
   int base = 0;
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int i = i0 + lane;
     int v = 0;
-    if (i < n) v = warp == 0 ? tiles_of(a.prefix_lens[i], a.prefix_width, P.y.tp) * units_of(P, i) * a.NKV : tiles_of(a.lens[i], a.table_width, P.y.tp) * a.NKV;
+    if (i < n) {
+      len[i] = lens[i];
+      v = tiles_of(len[i], width, P.y.tp) * a.NKV;
+      if (warp == 0) v *= units_of(P, i);
+    }
     int s = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(~0u, s, o); if (lane >= o) s += x; }
@@ -175,85 +194,98 @@ __device__ __forceinline__ int find(const int32_t* c, int n, int t) {      // th
   }
   return lo;
 }
-__device__ __forceinline__ int share(long long total, int w, int workers) { return (int)(total * w / workers); }
+// The first tile of worker w: floor(total * w / workers), without 64-bit arithmetic (workers <= 256).
+__device__ __forceinline__ int share(int total, int w, int workers) {
+  const int q = total / workers, r = total - q * workers;
+  return q * w + r * w / workers;
+}
+
+// The first unit of group g's prefix: no more units lie before it than sequences / spt + groups, for each kv head.
+__device__ __forceinline__ int prefix_unit(const Params& P, int g) { return (P.groups.first[g] / P.y.spt + g) * P.a.NKV; }
 
 struct Segment {
-  bool own;
-  int who, h;                 // group or sequence; kv head
+  int n;                      // tiles of the unit from tile0 on
+  int own;                    // a sequence's own positions, not a prefix's
+  int h;                      // kv head
   int seq0, rows;             // first sequence and number of rows
-  int tile0, n;               // tiles [tile0, tile0 + n) of the unit
+  int tile0, ends;            // the unit's last tile is in it
   int len;                    // positions of the unit
-  long long slot;             // of its partial results, prefixes' first
+  int unit;                   // of all units, prefixes' first; its parts lie in the slots unit + worker
+  int pad;
   const int32_t* table;
 };
-__device__ __forceinline__ Segment segment_at(const Params& P, const Cum& c, int t, int end, int worker) {
+__device__ __forceinline__ void segment_at(const Params& P, const Cum& c, int t, int end, Segment& s) {
   const etxb_attn_shared_args& a = P.a;
-  Segment s;
   const int tp_all = c.p[a.groups];
+  int per;
   s.own = t >= tp_all;
   if (!s.own) {
-    const int g = s.who = find(c.p, a.groups, t), mt = units_of(P, g), size = P.groups.first[g + 1] - P.groups.first[g];
-    const int per = (c.p[g + 1] - c.p[g]) / (mt * a.NKV), rel = t - c.p[g], unit = rel / per;
+    const int g = find(c.p, a.groups, t), mt = units_of(P, g), first = P.groups.first[g];
+    per = (c.p[g + 1] - c.p[g]) / (mt * a.NKV);
+    const int rel = t - c.p[g], unit = rel / per;
     s.h = unit / mt;
     const int m = unit - s.h * mt;
-    s.seq0 = P.groups.first[g] + m * P.y.spt;
-    s.rows = min(P.y.spt, size - m * P.y.spt) * P.y.G;
+    s.seq0 = first + m * P.y.spt;
+    s.rows = min(P.y.spt, P.groups.first[g + 1] - s.seq0) * P.y.G;
     s.tile0 = rel - unit * per;
-    s.n = min(per - s.tile0, end - t);
-    s.len = a.prefix_lens[g];
+    s.len = c.len[g];
     s.table = a.prefix_tables + g * a.prefix_stride;
-    s.slot = (long long)(P.groups.first[g] / P.y.spt + g) * a.NKV + unit + worker;
+    s.unit = prefix_unit(P, g) + unit;
   } else {
-    const int r = t - tp_all, b = s.who = find(c.s, a.seqs, r);
-    const int per = (c.s[b + 1] - c.s[b]) / a.NKV, rel = r - c.s[b];
+    const int r = t - tp_all, b = find(c.s, a.seqs, r);
+    per = (c.s[b + 1] - c.s[b]) / a.NKV;
+    const int rel = r - c.s[b];
     s.h = rel / per;
     s.seq0 = b; s.rows = P.y.G;
     s.tile0 = rel - s.h * per;
-    s.n = min(per - s.tile0, end - t);
-    s.len = a.lens[b];
+    s.len = c.len[a.groups + b];
     s.table = a.tables + b * a.table_stride;
-    s.slot = P.y.pslots + (long long)b * a.NKV + s.h + worker;
+    s.unit = P.y.punits + b * a.NKV + s.h;
   }
-  return s;
+  s.n = min(per - s.tile0, end - t);
+  s.ends = s.tile0 + s.n == per;
 }
 
 // ------------------------------------------------------------------------------------------------ the tiles
+constexpr int SEGS = 8;                       // segments known ahead
+template <int SLOTS>
 struct Shared {
-  Cum cum;
   uint64_t full[SLOTS], empty[SLOTS];         // ring of key / value tiles: K0 K1 V0 K2 V1 .. (V of tile n: use 2 n + 2)
-  uint64_t v_ready[4];                        // tile n's values are there and those behind the last position cleared, at n % 4 (the ring holds fewer tiles)
-  uint64_t s_full[2], p_full[2], pv_done, o_full[2], o_free[2], q_full[2], q_free[2];
+  uint64_t s_full[2], p_full[2], pv_done[2], o_full[2], o_free[2], q_full[4], q_free[4], seg_full[SEGS], seg_free[SEGS], pair[4];
+  Segment seg[SEGS];
+  float part[2][2][ROWS];                     // what the two warps of a row tell each other: by turn, by half
   uint32_t tmem;
   int stop;
 };
 
-template <int TP>
+// Shared memory: SLOTS tiles of keys or values, Q, the tiles before each group and sequence and their lengths.
+// SLOTS is even: values always lie in the even slots, so that whoever looks at values alone sees every use of its slots (but the first of slot 0).
+constexpr int fixed_bytes(int hd, int slots) { return 256 + slots * SLOT_BYTES + ROWS * hd * 2; }
+template <int TP, int SLOTS>
 __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant__ Params P) {
-  extern __shared__ __align__(1024) unsigned char dyn[];
-  __shared__ Shared sh;
+  extern __shared__ __align__(256) unsigned char dyn[];
+  __shared__ Shared<SLOTS> sh;
   constexpr int PAGES = TP / BS, HALF = TP / 2;                     // pages of a tile; columns of S that one half of the pages' positions take
-  constexpr int NO = TP == 128 ? 2 : 1, NQ = NO;                    // accumulators of O and buffers of Q: two where they fit
+  constexpr int NO = TP == 128 ? 2 : 1;                             // accumulators of O: two where they fit
   const etxb_attn_shared_args& a = P.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, HD = a.HD, worker = blockIdx.x;
   const uint32_t page_bytes = (uint32_t)HD * BS * 2, q_bytes = ROWS * (uint32_t)HD * 2;
-  unsigned char* const base = (unsigned char*)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023);
+  unsigned char* const base = (unsigned char*)(((uintptr_t)dyn + 255) & ~(uintptr_t)255);
   unsigned char* const qbuf = base + SLOTS * SLOT_BYTES;
+  const Cum cum = {(int32_t*)(qbuf + q_bytes), (int32_t*)(qbuf + q_bytes) + a.groups + 1, (int32_t*)(qbuf + q_bytes) + a.groups + a.seqs + 2};
   volatile int* const stop = &sh.stop;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (what follows on the device waits for this grid before it reads)
-  if (tid == 0) {
+  cumulate(P, cum);
+  if (tid == W_Q * 32) {
     for (int i = 0; i < SLOTS; ++i) { bar_init(&sh.full[i], 1); bar_init(&sh.empty[i], 1); }
-    bar_init(&sh.pv_done, 1);
-    for (int i = 0; i < 4; ++i) bar_init(&sh.v_ready[i], 32);
-    for (int i = 0; i < 2; ++i) {
-      bar_init(&sh.s_full[i], 1); bar_init(&sh.p_full[i], 4); bar_init(&sh.o_full[i], 1); bar_init(&sh.o_free[i], 4);
-      bar_init(&sh.q_full[i], 32); bar_init(&sh.q_free[i], 1);
-    }
+    for (int i = 0; i < 2; ++i) { bar_init(&sh.s_full[i], 1); bar_init(&sh.pv_done[i], 1); bar_init(&sh.p_full[i], SM_WARPS); bar_init(&sh.o_full[i], 1); bar_init(&sh.o_free[i], SM_WARPS); }
+    for (int i = 0; i < 4; ++i) { bar_init(&sh.q_full[i], 32); bar_init(&sh.q_free[i], 1); bar_init(&sh.pair[i], 2); }
+    for (int i = 0; i < SEGS; ++i) { bar_init(&sh.seg_full[i], 1); bar_init(&sh.seg_free[i], SM_WARPS + 3); }
     sh.stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  cumulate(P, sh.cum);
-  if (warp == W_MMA) {
+  if (warp == W_QK) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     fence_before();
@@ -262,17 +294,37 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
-  const Cum& cum = sh.cum;
-  const long long total = (long long)cum.p[a.groups] + cum.s[a.seqs];
-  const int t0 = share(total, worker, P.y.workers), t1 = share(total, worker + 1, P.y.workers);
+  const int total = cum.p[a.groups] + cum.s[a.seqs], workers = min(P.y.workers, total);        // (no worker without a tile among those that share)
+  const int t0 = worker < workers ? share(total, worker, workers) : 0, t1 = worker < workers ? share(total, worker + 1, workers) : 0;
+  // A role's next segment (false: a wait ran out), and the end of its use.
+  auto next_segment = [&](uint32_t k, Segment& s) {
+    if (!bar_wait(&sh.seg_full[k % SEGS], k / SEGS, stop)) return false;
+    s = sh.seg[k % SEGS];
+    return true;
+  };
 
-  if (warp < 4) {
-    // ---- softmax: row = thread
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const float sl = a.scale * 1.4426950408889634f;                 // scores in units of log2
-    uint32_t n = 0, seg = 0;
+  if (warp < SM_WARPS) {
+    // ---- softmax: a row belongs to a lane of two warps, each of which has half of a tile's positions: blocks of 16 columns of S in both halves
+    constexpr int MINE = TP / 2;                                    // positions of a warp
+    const int quarter = warp & 3, hf = warp >> 2, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    // scores in units of log2 (a scale of 0 as the least there is: a masked score stays minus infinity)
+    const float sl = fmaxf(a.scale * 1.4426950408889634f, 1e-37f);
+    uint32_t n = 0, seg = 0, turn = 0;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
+    // tells the other warp of the row x and gets its value
+    auto exchange = [&](float x) {
+      float* mine = &sh.part[turn & 1][hf][row];
+      *mine = x;
+      __syncwarp();
+      if (lane == 0) bar_arrive(&sh.pair[quarter]);
+      ok = ok && bar_wait(&sh.pair[quarter], turn, stop);
+      ok = __all_sync(~0u, ok);
+      const float y = sh.part[turn & 1][hf ^ 1][row];
+      ++turn;
+      return y;
+    };
     // Results of the segment before, written while the present one's first products run.
     Segment prev = {};
     float prev_m = 0.f, prev_l = 0.f;
@@ -281,19 +333,19 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
       ok = ok && bar_wait(&sh.o_full[ob], sg / NO, stop);
       ok = __all_sync(~0u, ok);
       fence_after();
-      if (ok && warp * 32 < prev.rows) {
+      if (ok && quarter * 32 < prev.rows) {
         const int stride = prev.own ? P.y.G : P.y.prows;
-        const long long slot = prev.own ? prev.slot - P.y.pslots : prev.slot;
-        float* O = (prev.own ? P.y.oO : P.y.pO) + slot * stride * HD + (size_t)tid * 4;
-        if (tid < prev.rows) {
-          float* ml = (prev.own ? P.y.oml : P.y.pml) + (slot * stride + tid) * 2;
-          ml[0] = prev_m; ml[1] = prev_l;
-        }
-        for (int c = 0; c < HD; c += 16) {
+        const long long slot = (long long)(prev.own ? prev.unit - P.y.punits : prev.unit) + worker;
+        float* O = (prev.own ? P.y.oO : P.y.pO) + slot * stride * HD + (size_t)row * 4;
+        const float l2 = exchange(prev_l);
+        if (hf == 0 && row < prev.rows) *(float2*)((prev.own ? P.y.oml : P.y.pml) + (slot * stride + row) * 2) = make_float2(prev_m, prev_l + l2);
+        const int mid = (HD / 16 + 1) / 2 * 16;
+#pragma unroll 1
+        for (int c = hf ? mid : 0; c < (hf ? HD : mid); c += 16) {
           uint32_t r[16];
           tmem_ld16(tmem + lanes + 2 * TP + ob * HD + c, r);
           tmem_wait_ld();
-          if (tid < prev.rows) {
+          if (row < prev.rows) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) *(uint4*)(O + (size_t)(c / 4 + k) * stride * 4) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
           }
@@ -303,41 +355,50 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
       __syncwarp();
       if (lane == 0) bar_arrive(&sh.o_free[ob]);
     };
-    for (int t = t0; t < t1 && ok;) {
-      const Segment s = segment_at(P, cum, t, t1, worker);
-      const bool busy = warp * 32 < s.rows;                         // (a warp without rows only keeps the others' time)
+    for (int t = t0; t < t1 && ok; ++seg) {
+      Segment s;
+      ok = __all_sync(~0u, next_segment(seg, s));
+      if (!ok) break;
+      const bool busy = quarter * 32 < s.rows;                      // (a warp without rows only keeps the others' time)
       for (int i = 0; i < s.n && ok; ++i, ++n) {
-        const uint32_t sb = n & 1, scol = tmem + lanes + sb * TP;
+        const uint32_t sb = n & 1, scol = tmem + lanes + sb * TP + hf * (MINE / 2);
         ok = bar_wait(&sh.s_full[sb], n >> 1, stop);
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         fence_after();
         if (busy) {
-          uint32_t r[TP];
-#pragma unroll
-          for (int c = 0; c < TP; c += 32) tmem_ld32(scol + c, r + c);
+          // r: position p of the warp's is at p / 8 % 2 * (MINE / 2) + p / 16 * 8 + p % 8
+          uint32_t r[MINE];
+          if (MINE == 64) { tmem_ld32(scol, r); tmem_ld32(scol + HALF, r + MINE / 2); }
+          else { tmem_ld16(scol, r); tmem_ld16(scol + HALF, r + MINE / 2); }
           tmem_wait_ld();
-          const int valid = s.len - (s.tile0 + i) * TP;
-          // column c holds position (c % HALF) / 8 * 16 + c / HALF * 8 + c % 8 of the tile
-          if (valid < TP) {
+          const int valid = s.len - (s.tile0 + i) * TP - hf * MINE;
+          if (valid < MINE) {
 #pragma unroll
-            for (int c = 0; c < TP; ++c) if ((c % HALF) / 8 * 16 + c / HALF * 8 + c % 8 >= valid) r[c] = 0xff800000u;
+            for (int c = 0; c < MINE; ++c) if (c % (MINE / 2) / 8 * 16 + c / (MINE / 2) * 8 + c % 8 >= valid) r[c] = 0xff800000u;
           }
-          float mt = -INFINITY;
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < TP; c += 2) mt = fmaxf(mt, fmaxf(__uint_as_float(r[c]), __uint_as_float(r[c + 1])));
+          for (int c = 0; c < MINE; c += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1])));
+          float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          mt = fmaxf(mt, exchange(mt));
+          if (!ok) break;
           if (i == 0) { m = mt; l = 0.f; }
           else {
             // the maximum moves only when the new one is above it by a factor of 2^8 or more: till then probabilities of up to 2^8 do no harm
-            const bool up = m != -INFINITY && (mt - m) * sl > 8.f;
+            const bool up = row < s.rows && m != -INFINITY && (mt - m) * sl > 8.f;
             if (__any_sync(~0u, up)) {
               const float f = up ? ex2((m - mt) * sl) : 1.f;
-              ok = bar_wait(&sh.pv_done, n - 1, stop);
+              ok = bar_wait(&sh.pv_done[(n - 1) & 1], (n - 1) >> 1, stop);
               ok = __all_sync(~0u, ok);
               if (!ok) break;
               fence_after();
               const uint32_t ocol = tmem + lanes + 2 * TP + (seg % NO) * HD;
-              for (int c = 0; c < HD; c += 16) {
+              const int mid = (HD / 16 + 1) / 2 * 16;
+#pragma unroll 1
+              for (int c = hf ? mid : 0; c < (hf ? HD : mid); c += 16) {
                 uint32_t o[16];
                 tmem_ld16(ocol + c, o);
                 tmem_wait_ld();
@@ -349,34 +410,34 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
             }
             if (up || m == -INFINITY) m = mt;
           }
-          const float ms = m == -INFINITY ? 0.f : m * sl;
-          const int left = min(valid, TP);
+          if (valid > 0) {                                          // (nothing multiplies the pages behind the last)
+            const float ms = m == -INFINITY ? 0.f : m * sl;
+            float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < TP / 32; ++j) {                       // 32 positions (two pages) at a time: 16 columns of hi, 16 of lo
-            uint32_t hi[16], lo[16];
+            for (int j = 0; j < MINE / 32; ++j) {                   // two pages at a time: 16 columns of hi, 16 of lo
+              uint32_t hi[16], lo[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float x[2], y[2];
+              for (int k = 0; k < 16; ++k) {
+                float p[2], y[2];
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int pos = 32 * j + 2 * k + e, c = (pos / 8 & 1) * HALF + pos / 16 * 8 + pos % 8;
-                const float v = __uint_as_float(r[c]);
-                float p = ex2(__fmaf_rn(v, sl, -ms));
-                if (valid < TP && pos >= left) p = 0.f;
-                l += p;
-                // hi: the upper 16 bits; lo: what is left, never 0 where p is not (0 x inf would spoil an infinite value's sum)
-                const uint32_t u = p == 0.f ? 0u : __float_as_uint(p) | 1u;
-                x[e] = __uint_as_float(u & 0xffff0000u);
-                y[e] = __uint_as_float(u) - x[e];
+                for (int e = 0; e < 2; ++e) {
+                  const int pos = 32 * j + 2 * k + e;
+                  p[e] = ex2(__fmaf_rn(__uint_as_float(r[pos / 8 % 2 * (MINE / 2) + pos / 16 * 8 + pos % 8]), sl, -ms));
+                  ls[k & 3] += p[e];
+                  // hi: the upper 16 bits; lo: what is left and 2^-22 of p more, so that it is never 0 where p is not (0 x inf would spoil the sum of
+                  // an infinite value) nor negative
+                  y[e] = __fmaf_rn(p[e], 1.0f + 0x1p-22f, -__uint_as_float(__float_as_uint(p[e]) & 0xffff0000u));
+                }
+                hi[k] = __byte_perm(__float_as_uint(p[0]), __float_as_uint(p[1]), 0x7632);
+                const __nv_bfloat162 b2 = __floats2bfloat162_rn(y[0], y[1]);
+                lo[k] = *(const uint32_t*)&b2;
               }
-              hi[k] = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x7632);
-              const __nv_bfloat162 b2 = __floats2bfloat162_rn(y[0], y[1]);
-              lo[k] = *(const uint32_t*)&b2;
+              tmem_st16(scol + 16 * j, hi);
+              tmem_st16(scol + HALF + 16 * j, lo);
             }
-            tmem_st16(scol + 16 * j, hi);
-            tmem_st16(scol + TP / 2 + 16 * j, lo);
+            l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+            tmem_wait_st();
           }
-          tmem_wait_st();
         }
         fence_before();
         __syncwarp();
@@ -384,16 +445,16 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
         if (i == 0 && seg > 0) write_out(seg - 1);
       }
       prev = s; prev_m = m == -INFINITY ? m : m * sl; prev_l = l;
-      ++seg;
+      __syncwarp();
+      if (lane == 0) bar_arrive(&sh.seg_free[seg % SEGS]);
       t += s.n;
     }
     if (ok && seg > 0) write_out(seg - 1);
   } else if (warp == W_COPY) {
     // ---- copies: a lane per page
-    uint32_t use = 0, filled[SLOTS] = {};                           // running number of ring slots taken; how often each was
-    bool ok = true;
-    Segment s;
-    int t = t0, i = 0;
+    uint32_t use = 0, filled[SLOTS] = {}, seg = 0;                  // running number of ring slots taken; how often each was
+    bool ok = true, have = false;
+    int vp = 0, vn = 0, vh = 0;                                     // the tile whose values follow
     auto put = [&](int n_pages, int page, int h, bool values) {
       const uint32_t sl = use % SLOTS, round = use / SLOTS;
       if (round > 0) ok = ok && bar_wait(&sh.empty[sl], round - 1, stop);
@@ -410,22 +471,35 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
       }
       ++use;
     };
-    int bad = 0, vp = 0, vn = 0, vh = 0;                            // the tile whose values follow
-    bool have = false;
-    while (t < t1 && ok) {
-      if (i == 0) s = segment_at(P, cum, t, t1, worker);
-      const int pg0 = (s.tile0 + i) * PAGES, np = min(PAGES, (s.len + BS - 1) / BS - pg0);
-      int page = lane < np ? s.table[pg0 + lane] : 0;
-      const bool off = page < 0 || page >= a.pages;
-      if (__any_sync(~0u, off)) { bad = ETXB_SHARED_BAD_PAGE; if (off) page = 0; }
-      put(np, page, s.h, false);
-      if (have) put(vn, vp, vh, true);
-      have = true; vp = page; vn = np; vh = s.h;
-      if (++i == s.n) {
-        if (lane == 0) P.y.hdr[s.slot] = bad;
-        if (bad && lane == 0 && a.status) atomicOr(a.status, bad);
-        bad = 0; i = 0; t += s.n;
+    for (int t = t0; t < t1 && ok; ++seg) {
+      Segment s;
+      ok = __all_sync(~0u, next_segment(seg, s));
+      if (!ok) break;
+      const int first = s.tile0 * PAGES, pages = min(s.n * PAGES, (s.len + BS - 1) / BS - first);
+      int bad = 0;
+      // the numbers of 32 pages at a time, the next ones on their way
+      int ids = lane < pages ? s.table[first + lane] : 0, more = 0;
+      for (int p0 = 0; p0 < pages && ok; p0 += PAGES) {
+        if (p0 % 32 == 0) {
+          if (p0 > 0) ids = more;
+          if (p0 + 32 + lane < pages) more = s.table[first + p0 + 32 + lane];
+          const bool off = p0 + lane < pages && (ids < 0 || ids >= a.pages);
+          if (off) ids = 0;
+          if (__any_sync(~0u, off)) bad = ETXB_SHARED_BAD_PAGE;
+        }
+        const int np = min(PAGES, pages - p0), page = __shfl_sync(~0u, ids, (p0 + lane) & 31);
+        put(np, page, s.h, false);
+        if (have) put(vn, vp, vh, true);
+        have = true; vp = page; vn = np; vh = s.h;
       }
+      if (lane == 0) {
+        P.y.hdr[(s.own ? P.y.pslots - P.y.punits : 0) + s.unit + worker] = bad;
+        if (s.tile0 == 0) P.y.of[2 * s.unit] = worker;
+        if (s.ends) P.y.of[2 * s.unit + 1] = worker;
+        if (bad && a.status) atomicOr(a.status, bad);
+        bar_arrive(&sh.seg_free[seg % SEGS]);
+      }
+      t += s.n;
     }
     ++use;
     if (have && ok) put(vn, vp, vh, true);
@@ -435,101 +509,70 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
       const unsigned long long w0 = now_ns();
       while (filled[i] && !bar_try(&sh.full[i], (filled[i] - 1) & 1) && now_ns() - w0 < WAIT_NS) {}
     }
-  } else if (warp == W_MMA) {
-    // ---- products
-    const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(ROWS >> 4) << 24);
-    const uint32_t idesc_pv = idesc | ((uint32_t)(HD >> 3) << 17);
-    uint32_t use = 0, n = 0, seg = 0;
-    bool ok = true;
-    int t = t0, i = 0;
-    Segment s;
-    struct { int np; bool first, last; uint32_t seg; } v = {0, false, false, 0};   // the tile whose PV follows
-    bool have = false;
-    auto pv = [&]() {
-      const uint32_t sl = use % SLOTS, m = n - 1, ob = v.seg % NO;
-      ok = ok && bar_wait(&sh.full[sl], use / SLOTS, stop);
-      ok = ok && bar_wait(&sh.v_ready[m & 3], m >> 2, stop);
-      if (v.first && v.seg >= NO) ok = ok && bar_wait(&sh.o_free[ob], v.seg / NO - 1, stop);
-      ok = ok && bar_wait(&sh.p_full[m & 1], m >> 1, stop);
-      if (!ok) return;
-      fence_after();
-      if (elect()) {
-        const uint32_t d = tmem + 2 * TP + ob * HD, pc = tmem + (m & 1) * TP;
-        uint64_t b = desc(smem_u32(base + sl * SLOT_BYTES), 16, 256, 6);
-        for (int k = 0; k < v.np; ++k, b += page_bytes >> 4) {
-          mma_ts(d, pc + 8 * k, b, idesc_pv, (!v.first || k > 0) ? 1u : 0u);
-          mma_ts(d, pc + TP / 2 + 8 * k, b, idesc_pv, 1u);
+  } else if (warp == W_QK) {
+    // ---- S = Q K^T: one thread, and another one for O += P V, so that neither waits behind what the other waits for
+    if (elect()) {
+      const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(ROWS >> 4) << 24);
+      uint32_t n = 0, seg = 0;
+      bool ok = true;
+      for (int t = t0; t < t1 && ok; ++seg) {
+        Segment s;
+        ok = next_segment(seg, s);
+        ok = ok && bar_wait(&sh.q_full[seg & 3], seg >> 2, stop);
+        // (a sequence's own rows lie close together: what the other rows of the instruction read there reaches accumulator rows that nobody reads)
+        const uint32_t qrows = s.own ? OWN_ROWS : ROWS;
+        const uint64_t ad = desc(smem_u32(qbuf + (s.own ? (seg & 3) * (OWN_ROWS * (uint32_t)HD * 2) : 0u)), qrows * 16, 128, 0), astep = 2 * qrows;
+        for (int i = 0; i < s.n && ok; ++i, ++n) {
+          const int np = min(PAGES, (s.len + BS - 1) / BS - (s.tile0 + i) * PAGES);
+          const uint32_t use = n == 0 ? 0 : 2 * n - 1, sl = use % SLOTS;
+          if (n >= 2) ok = bar_wait(&sh.pv_done[n & 1], (n >> 1) - 1, stop);         // (P of tile n - 2 lies where S of this one goes)
+          ok = ok && bar_wait(&sh.full[sl], use / SLOTS, stop);
+          if (!ok) break;
+          fence_after();
+          const uint32_t id = idesc | ((uint32_t)((np + 1) & ~1) << 17);             // N = 8 positions of each page, a multiple of 16
+          const uint32_t d = tmem + (n & 1) * TP;
+          const uint64_t b0 = desc(smem_u32(base + sl * SLOT_BYTES), 256, page_bytes, 0);
+          mma_ss(d, ad, b0, id, 0u);
+          mma_ss(d + HALF, ad, b0 + (128 >> 4), id, 0u);
+          if (TP == 128 && HD == 128) {
+#pragma unroll
+            for (int k = 1; k < 8; ++k) {
+              mma_ss_add(d, ad + k * astep, b0 + k * (512 >> 4), id);
+              mma_ss_add(d + HALF, ad + k * astep, b0 + k * (512 >> 4) + (128 >> 4), id);
+            }
+          } else {
+#pragma unroll 1
+            for (int k = 1; k < HD / 16; ++k) {
+              mma_ss_add(d, ad + k * astep, b0 + k * (512 >> 4), id);
+              mma_ss_add(d + HALF, ad + k * astep, b0 + k * (512 >> 4) + (128 >> 4), id);
+            }
+          }
+          mma_commit(&sh.s_full[n & 1]);
+          mma_commit(&sh.empty[sl]);
+          if (i == s.n - 1) mma_commit(&sh.q_free[seg & 3]);
         }
-        mma_commit(&sh.empty[sl]);
-        mma_commit(&sh.pv_done);
-        if (v.last) mma_commit(&sh.o_full[ob]);
+        bar_arrive(&sh.seg_free[seg % SEGS]);
+        t += s.n;
       }
-      __syncwarp();
-      ++use;
-    };
-    while (t < t1 && ok) {
-      if (i == 0) {
-        s = segment_at(P, cum, t, t1, worker);
-        ok = bar_wait(&sh.q_full[seg % NQ], seg / NQ, stop);
-      }
-      const int np = min(PAGES, (s.len + BS - 1) / BS - (s.tile0 + i) * PAGES);
-      const uint32_t sl = use % SLOTS;
-      ok = ok && bar_wait(&sh.full[sl], use / SLOTS, stop);
-      if (!ok) break;
-      fence_after();
-      if (elect()) {
-        const uint32_t id = idesc | ((uint32_t)((np + 1) & ~1) << 17);               // N = 8 positions of each page, a multiple of 16
-        const uint32_t qa = smem_u32(qbuf + (seg % NQ) * q_bytes), ka = smem_u32(base + sl * SLOT_BYTES);
-        uint64_t ad = desc(qa, ROWS * 16, 128, 0), b0 = desc(ka, 256, page_bytes, 0);
-        for (int k = 0; k < HD / 16; ++k, ad += (2 * ROWS * 16) >> 4, b0 += 512 >> 4) {
-          mma_ss(tmem + (n & 1) * TP, ad, b0, id, k > 0 ? 1u : 0u);
-          mma_ss(tmem + (n & 1) * TP + HALF, ad, b0 + (128 >> 4), id, k > 0 ? 1u : 0u);
-        }
-        mma_commit(&sh.empty[sl]);
-        mma_commit(&sh.s_full[n & 1]);
-        if (i == s.n - 1) mma_commit(&sh.q_free[seg % NQ]);
-      }
-      __syncwarp();
-      ++use;
-      if (have) pv();
-      have = true;
-      v = {np, i == 0, i == s.n - 1, seg};
-      ++n;
-      if (++i == s.n) { i = 0; t += s.n; ++seg; }
     }
-    ++use;
-    if (have && ok) pv();
-  } else if (warp == W_Q) {
-    // ---- Q: the rows of a segment as [HD / 8][128 rows][8]
-    uint32_t seg = 0;
-    for (int t = t0; t < t1; ++seg) {
-      const Segment s = segment_at(P, cum, t, t1, worker);
-      const uint32_t qb = seg % NQ;
-      if (seg >= NQ && !bar_wait(&sh.q_free[qb], seg / NQ - 1, stop)) break;
-      const uint32_t dst = smem_u32(qbuf + qb * q_bytes);
-      const int ch = HD / 8;
-      for (int x = lane; x < s.rows * ch; x += 32) {
-        const int row = x / ch, c = x - row * ch, sq = row / P.y.G, j = row - sq * P.y.G;
-        const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + (s.seq0 + sq) * a.q_stride + (long long)(s.h * P.y.G + j) * HD + c * 8;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * (ROWS * 16) + row * 16), "l"(src) : "memory");
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_async();
-      bar_arrive(&sh.q_full[qb]);
-      t += s.n;
-    }
-  } else {
-    // ---- values behind the last position of a unit become 0
-    // It looks at every tile of values, in order: a wait that skipped some would take an earlier phase of the slot's barrier for the one it means.
-    // Ring order K0 K1 V0 K2 V1 .. (behind the last K a use is left out): V of tile n is use 2 n + 2.
+    __syncwarp();
+  } else if (warp == W_PV) {
+    // ---- O += P V, behind the clearing of the values behind the unit's last position
+    const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+    const uint64_t step = page_bytes >> 4;
+    uint32_t n = 0, seg = 0;
     bool ok = true;
-    uint32_t n = 0;
-    if (t0 < t1) ok = bar_wait(&sh.full[0], 0, stop);                 // (K0: the one use of slot 0 that is not V's)
-    for (int t = t0; t < t1 && ok;) {
-      const Segment s = segment_at(P, cum, t, t1, worker);
+    if (t0 < t1) ok = bar_wait(&sh.full[0], 0, stop);                 // (K0: the one use of slot 0 that is not V's; a wait for V1 would take it for its own)
+    for (int t = t0; t < t1 && ok; ++seg) {
+      Segment s;
+      ok = next_segment(seg, s);
+      const uint32_t ob = seg % NO, d = tmem + 2 * TP + ob * HD;
+      if (seg >= NO) ok = ok && bar_wait(&sh.o_free[ob], seg / NO - 1, stop);
+      ok = __all_sync(~0u, ok);
       for (int i = 0; i < s.n && ok; ++i, ++n) {
-        const uint32_t u = 2 * n + 2, sl = u % SLOTS;
-        ok = bar_wait(&sh.full[sl], u / SLOTS, stop);
+        const int np = min(PAGES, (s.len + BS - 1) / BS - (s.tile0 + i) * PAGES);
+        const uint32_t use = 2 * n + 2, sl = use % SLOTS, pc = tmem + (n & 1) * TP;
+        ok = bar_wait(&sh.full[sl], use / SLOTS, stop);
         const int rem = s.len % BS, page = (s.len - 1) / BS - (s.tile0 + i) * PAGES;
         if (ok && rem && page < PAGES) {
           unsigned char* v = base + sl * SLOT_BYTES + page * page_bytes;
@@ -548,93 +591,159 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
           }
           fence_async();
         }
-        bar_arrive(&sh.v_ready[n & 3]);
+        ok = ok && bar_wait(&sh.p_full[n & 1], n >> 1, stop);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        fence_after();
+        if (elect()) {
+          const uint64_t b = desc(smem_u32(base + sl * SLOT_BYTES), 16, 256, 6);
+          mma_ts(d, pc, b, idesc, i == 0 ? 0u : 1u);
+          mma_ts_add(d, pc + TP / 2, b, idesc);
+          if (np == PAGES) {
+#pragma unroll
+            for (int k = 1; k < PAGES; ++k) {
+              mma_ts_add(d, pc + 8 * k, b + k * step, idesc);
+              mma_ts_add(d, pc + TP / 2 + 8 * k, b + k * step, idesc);
+            }
+          } else {
+#pragma unroll 1
+            for (int k = 1; k < np; ++k) {
+              mma_ts_add(d, pc + 8 * k, b + k * step, idesc);
+              mma_ts_add(d, pc + TP / 2 + 8 * k, b + k * step, idesc);
+            }
+          }
+          mma_commit(&sh.pv_done[n & 1]);
+          mma_commit(&sh.empty[sl]);
+          if (i == s.n - 1) mma_commit(&sh.o_full[ob]);
+        }
+        __syncwarp();
       }
+      if (lane == 0) bar_arrive(&sh.seg_free[seg % SEGS]);
+      t += s.n;
+    }
+  } else if (warp == W_Q) {
+    // ---- the segments, and Q: their rows as [HD / 8][rows][8]: 128 rows of a prefix in all of the buffer, a sequence's 16 in one of four places of it
+    uint32_t seg = 0, waited = 0;                                   // segments whose rows the products are known to be done with
+    const int ch = HD / 8, qn = 32 / ch, qr = lane / ch < qn ? lane / ch : ROWS, qc = lane % ch;
+    bool ok = true;
+    int own = 0;
+    for (int t = t0; t < t1 && ok; ++seg) {
+      Segment s;
+      segment_at(P, cum, t, t1, s);
+      if (seg >= SEGS) ok = __all_sync(~0u, bar_wait(&sh.seg_free[seg % SEGS], seg / SEGS - 1, stop));
+      if (lane == 0 && ok) { sh.seg[seg % SEGS] = s; bar_arrive(&sh.seg_full[seg % SEGS]); }
+      const uint32_t until = s.own && own ? (seg < 3 ? 0 : seg - 3) : seg;
+      for (; waited < until && ok; ++waited) ok = bar_wait(&sh.q_free[waited & 3], waited >> 2, stop);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      own = s.own;
+      const int qrows = s.own ? OWN_ROWS : ROWS;
+      const uint32_t dst = smem_u32(qbuf + (s.own ? (seg & 3) * (OWN_ROWS * (uint32_t)HD * 2) : 0u));
+      int sq = qr / P.y.G, j = qr - sq * P.y.G;                       // a lane has piece qc of every qn-th row
+      for (int row = qr; row < s.rows; row += qn) {
+        const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + (s.seq0 + sq) * a.q_stride + (long long)(s.h * P.y.G + j) * HD + qc * 8;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + qc * (qrows * 16) + row * 16), "l"(src) : "memory");
+        for (j += qn; j >= P.y.G; j -= P.y.G) ++sq;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_async();
+      bar_arrive(&sh.q_full[seg & 3]);
       t += s.n;
     }
   }
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  if (warp == W_QK) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   if (tid == 0) {
-    P.y.state[worker] = sh.stop;
+    P.y.gave_up[worker] = sh.stop;
     if (sh.stop && a.status) atomicOr(a.status, ETXB_SHARED_GAVE_UP);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ joining the segments
-// A thread has four output elements of one row: it adds the parts of the prefix's unit and of the sequence's own one, each weighted with 2^(m - M).
-constexpr int JOIN_THREADS = 256;
+// A block has the G rows of one sequence and kv head: it adds the parts of the prefix's unit and of the sequence's own one, each weighted with 2^(m - M).
+constexpr int JOIN_THREADS = 128, MAX_WORKERS = 256;
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ Params P) {
-  __shared__ Cum cum;
+  __shared__ float f[2 * MAX_WORKERS][16], sum[16];                 // weight of a part in a row
+  __shared__ int s_bad;
   const etxb_attn_shared_args& a = P.a;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  cumulate(P, cum);
-  __syncthreads();
-  const int HD = a.HD, G = P.y.G, W = P.y.workers;
-  const long long idx = (long long)blockIdx.x * JOIN_THREADS + threadIdx.x;
-  if (idx >= (long long)a.seqs * a.NH * (HD / 4)) return;
-  const int j = (int)(idx % G);
-  const long long r1 = idx / G;
-  const int c = (int)(r1 % (HD / 4));
-  const long long r2 = r1 / (HD / 4);
-  const int h = (int)(r2 % a.NKV), b = (int)(r2 / a.NKV);
+  const int tid = threadIdx.x, HD = a.HD, G = P.y.G, W = P.y.workers, h = blockIdx.x, b = blockIdx.y;
   int lo = 0, hi = a.groups - 1;                                    // the group of b: the last that begins at or before it
   while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (P.groups.first[mid] <= b) lo = mid; else hi = mid - 1; }
   const int g = lo, first = P.groups.first[g], mt = units_of(P, g), um = (b - first) / P.y.spt;
-  const long long total = (long long)cum.p[a.groups] + cum.s[a.seqs];
   int bad = 0;
   if (bad_length(a.prefix_lens[g], a.prefix_width) || bad_length(a.lens[b], a.table_width)) bad = ETXB_SHARED_BAD_LENGTH;
-  // the two units: tiles [ta, tb) of all, the slot of worker 0, the rows of a slot and this row
-  int ta[2], tb[2], stride[2], row[2];
-  long long slot[2];
-  {
-    const int per = (cum.p[g + 1] - cum.p[g]) / (mt * a.NKV), unit = h * mt + um;
-    ta[0] = cum.p[g] + unit * per; tb[0] = ta[0] + per;
-    slot[0] = (long long)(first / P.y.spt + g) * a.NKV + unit;
-    stride[0] = P.y.prows; row[0] = (b - first - um * P.y.spt) * G + j;
-    const int po = (cum.s[b + 1] - cum.s[b]) / a.NKV;
-    ta[1] = cum.p[a.groups] + cum.s[b] + h * po; tb[1] = ta[1] + po;
-    slot[1] = (long long)b * a.NKV + h;
-    stride[1] = G; row[1] = j;
-  }
-  float M = -INFINITY;
-  for (int k = 0; k < 2; ++k) {
-    if (ta[k] >= tb[k]) continue;
-    int w = (int)((long long)ta[k] * W / total);                    // a worker at or before the first; the shares are rounded down
-    while (share(total, w + 1, W) <= ta[k]) ++w;
-    for (; w < W && share(total, w, W) < tb[k]; ++w) {
-      if (share(total, w, W) == share(total, w + 1, W)) continue;   // (more workers than tiles: an empty share)
-      const float* ml = (k ? P.y.oml : P.y.pml) + ((slot[k] + w) * stride[k] + row[k]) * 2;
-      M = fmaxf(M, __ldcg(ml));
-      bad |= P.y.hdr[(k ? P.y.pslots : 0) + slot[k] + w] | (P.y.state[w] ? ETXB_SHARED_GAVE_UP : 0);
-    }
-  }
-  float L = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < 2; ++k) {
-    if (ta[k] >= tb[k]) continue;
-    int w = (int)((long long)ta[k] * W / total);
-    while (share(total, w + 1, W) <= ta[k]) ++w;
-    for (; w < W && share(total, w, W) < tb[k]; ++w) {
-      if (share(total, w, W) == share(total, w + 1, W)) continue;
-      const float* ml = (k ? P.y.oml : P.y.pml) + ((slot[k] + w) * stride[k] + row[k]) * 2;
-      const float m = __ldcg(ml), l = __ldcg(ml + 1);
-      if (l == 0.f) continue;                                       // (nothing but scores of minus infinity; NaN goes on)
-      const float f = m == M ? 1.f : ex2(m - M);
-      const float4 o = __ldcg((const float4*)((k ? P.y.oO : P.y.pO) + (slot[k] + w) * stride[k] * HD + ((size_t)c * stride[k] + row[k]) * 4));
-      L = __fmaf_rn(l, f, L);
-      y[0] = __fmaf_rn(o.x, f, y[0]); y[1] = __fmaf_rn(o.y, f, y[1]); y[2] = __fmaf_rn(o.z, f, y[2]); y[3] = __fmaf_rn(o.w, f, y[3]);
-    }
-  }
-  if (bad && a.status && c == 0 && j == 0) atomicOr(a.status, bad);
-  __nv_bfloat162 out[2];
+  if (tid == 0) s_bad = 0;
+  const int unit[2] = {prefix_unit(P, g) + h * mt + um, P.y.punits + b * a.NKV + h};
+  const long long slot[2] = {unit[0], (long long)b * a.NKV + h};      // of worker 0
+  const int stride[2] = {P.y.prows, G}, row[2] = {(b - first - um * P.y.spt) * G, 0};
+  const bool has[2] = {!bad && a.prefix_lens[g] > 0, !bad && a.lens[b] > 0};
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int w0[2], n[2], lost = 0;
+  for (int w = tid; w < W; w += JOIN_THREADS) lost |= __ldcg(P.y.gave_up + w);
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const float z0 = bad ? NAN : L == 0.f ? 0.f : y[2 * e] / L, z1 = bad ? NAN : L == 0.f ? 0.f : y[2 * e + 1] / L;
-    out[e] = __floats2bfloat162_rn(z0, z1);
+  for (int k = 0; k < 2; ++k) {
+    const int2 of = has[k] ? __ldcg((const int2*)P.y.of + unit[k]) : make_int2(0, -1);
+    w0[k] = of.x; n[k] = of.y - of.x + 1;
   }
-  *(uint2*)((__nv_bfloat16*)a.out + b * a.out_stride + (long long)(h * G + j) * HD + 4 * c) = *(const uint2*)out;
+  if (__syncthreads_or(lost)) { bad |= ETXB_SHARED_GAVE_UP; n[0] = n[1] = 0; }     // (a worker that gave up left something unwritten: nothing is looked at)
+  const int parts = n[0] + n[1];
+  for (int i = tid; i < parts; i += JOIN_THREADS) {
+    const int k = i >= n[0], w = w0[k] + i - (k ? n[0] : 0);
+    bad |= __ldcg(P.y.hdr + (k ? P.y.pslots : 0) + slot[k] + w);
+  }
+  if (bad) atomicOr(&s_bad, bad);
+  for (int j = tid >> 5; j < G; j += JOIN_THREADS / 32) {           // a warp has a row
+    const int lane = tid & 31;
+    float M = -INFINITY, L = 0.f;
+    for (int pass = 0; pass < 2; ++pass) {
+      for (int i = lane; i < parts; i += 32) {
+        const int k = i >= n[0], w = w0[k] + i - (k ? n[0] : 0);
+        const float2 ml = __ldcg((const float2*)(k ? P.y.oml : P.y.pml) + (slot[k] + w) * stride[k] + row[k] + j);
+        if (pass == 0) M = fmaxf(M, ml.x);
+        else {
+          // (a part with nothing but scores of minus infinity has no weight; one that is NaN goes on)
+          const float x = ml.y == 0.f ? 0.f : ml.x == M ? 1.f : ex2(ml.x - M);
+          f[i][j] = x;
+          if (ml.y != 0.f) L = __fmaf_rn(ml.y, x, L);
+        }
+      }
+      if (pass == 0)
+        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
+    }
+    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
+    if (lane == 0) sum[j] = L;
+  }
+  __syncthreads();
+  bad = s_bad;
+  if (bad && a.status && tid == 0) atomicOr(a.status, bad);
+  for (int x = tid; x < G * HD / 4; x += JOIN_THREADS) {            // four output elements of a row
+    const int j = x % G, c = x / G;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float4* O = (const float4*)(k ? P.y.oO : P.y.pO) + (slot[k] + w0[k]) * stride[k] * (HD / 4) + (size_t)c * stride[k] + row[k] + j;
+      const size_t step = (size_t)stride[k] * (HD / 4);
+      const int at = k ? n[0] : 0;
+      for (int i0 = 0; i0 < n[k]; i0 += 8) {                        // (eight loads in flight)
+        float4 o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = __ldcg(O + min(i0 + i, n[k] - 1) * step);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float w = i0 + i < n[k] ? f[at + i0 + i][j] : 0.f;
+          if (w != 0.f) { y.x = __fmaf_rn(o[i].x, w, y.x); y.y = __fmaf_rn(o[i].y, w, y.y); y.z = __fmaf_rn(o[i].z, w, y.z); y.w = __fmaf_rn(o[i].w, w, y.w); }
+        }
+      }
+    }
+    const float L = sum[j];
+    const float z[4] = {y.x / L, y.y / L, y.z / L, y.w / L};
+    __nv_bfloat162 out[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) out[e] = __floats2bfloat162_rn(bad ? NAN : L == 0.f ? 0.f : z[2 * e], bad ? NAN : L == 0.f ? 0.f : z[2 * e + 1]);
+    *(uint2*)((__nv_bfloat16*)a.out + b * a.out_stride + (long long)(h * G + j) * HD + 4 * c) = *(const uint2*)out;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -683,7 +792,8 @@ static bool lay_out(const etxb_attn_shared_args& a, int workers, unsigned char* 
   const long long tiles = (units * ((a.prefix_width * (long long)BS + y.tp - 1) / y.tp) + a.seqs * ((a.table_width * (long long)BS + y.tp - 1) / y.tp)) * a.NKV;
   if (tiles >= (1ll << 31)) return false;
   y.prows = (most < y.spt ? most : y.spt) * y.G;
-  y.pslots = ((long long)a.seqs / y.spt + a.groups) * a.NKV + workers;      // (see segment_at: each group's units begin at (first / spt + g) * NKV)
+  y.punits = (a.seqs / y.spt + a.groups) * a.NKV;
+  y.pslots = (long long)y.punits + workers;
   y.oslots = (long long)a.seqs * a.NKV + workers;
   size_t at = 0;
   auto take = [&](size_t n) { unsigned char* p = work + at; at += up256(n); return p; };
@@ -692,7 +802,8 @@ static bool lay_out(const etxb_attn_shared_args& a, int workers, unsigned char* 
   y.pml = (float*)take((size_t)y.pslots * y.prows * 8);
   y.oml = (float*)take((size_t)y.oslots * y.G * 8);
   y.hdr = (int32_t*)take((size_t)(y.pslots + y.oslots) * 4);
-  y.state = (int32_t*)take((size_t)workers * 4);
+  y.gave_up = (int32_t*)take((size_t)workers * 4);
+  y.of = (int32_t*)take(((size_t)y.punits + (size_t)a.seqs * a.NKV) * 8);
   bytes = at;
   return true;
 }
@@ -705,6 +816,7 @@ static int32_t sizes(int device, const etxb_attn_shared_args& a, unsigned char* 
   using namespace etxb_shared;
   int sms = 0;
   ETXB_HOST_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  if (sms > MAX_WORKERS) sms = MAX_WORKERS;
   if (!lay_out(a, sms, work, y, bytes)) return refuse(ETXB_E_UNSUPPORTED, "the tables' widths allow 2^31 tiles");
   return ETXB_OK;
 }
@@ -754,16 +866,19 @@ extern "C" int32_t etxb_attn_shared(int device, const etxb_attn_shared_args* arg
   const CUresult r = encode(&P.vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)a.vc, dim, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return refuse(ETXB_E_CUDA, "cuTensorMapEncodeTiled failed for the values");
-  const void* k = a.HD <= 128 ? (const void*)tiles_kernel<128> : (const void*)tiles_kernel<64>;
-  const int smem = 1024 + SLOTS * SLOT_BYTES + (a.HD <= 128 ? 2 : 1) * ROWS * a.HD * 2;
+  // six tiles in the ring where they fit beside the counts of up to 300 groups and sequences, else four.  (Four where six would do: prefixes of 32500
+  // positions for 64 sequences, @@; the ring is then empty when a product's operands are asked for.)
+  const int count = (a.groups + a.seqs + 1) * 8, limit = 232448 - 3328;
+  const bool six = a.HD <= 128 && fixed_bytes(a.HD, 6) + count <= limit;
+  const void* k = a.HD > 128 ? (const void*)tiles_kernel<64, 4> : six ? (const void*)tiles_kernel<128, 6> : (const void*)tiles_kernel<128, 4>;
+  const int smem = fixed_bytes(a.HD, six ? 6 : 4) + count;
   ETXB_HOST_CU(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = dim3((unsigned)P.y.workers); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = (size_t)smem; cfg.stream = (cudaStream_t)cuda_stream;
   void* kargs[] = {(void*)&P};
   ETXB_HOST_CU(cudaLaunchKernelExC(&cfg, k, kargs));
-  const long long threads = (long long)a.seqs * a.NH * (a.HD / 4);
-  cfg.gridDim = dim3((unsigned)((threads + JOIN_THREADS - 1) / JOIN_THREADS)); cfg.blockDim = dim3(JOIN_THREADS); cfg.dynamicSmemBytes = 0;
+  cfg.gridDim = dim3((unsigned)a.NKV, (unsigned)a.seqs); cfg.blockDim = dim3(JOIN_THREADS); cfg.dynamicSmemBytes = 0;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;

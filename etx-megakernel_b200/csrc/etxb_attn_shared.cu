@@ -16,7 +16,7 @@
 //   softmax     a thread has a row: it reads its scores from tensor memory, keeps the running maximum and sum, and writes P over S.
 //   O += P V    A from tensor memory; a page of values, [HD][16 positions], is 32-byte rows with the positions inside: a TMA tensor copy with SWIZZLE_32B makes it
 //               the K-major operand of one k16 step.
-// P goes in as two bf16 numbers, P = hi + lo with hi cut off and lo rounded: 16 bits or more.  One would round every probability by 2^-9, which contexts
+// P goes in as two bf16 numbers, P = hi + lo, both cut off: 16 bits.  One would round every probability by 2^-9, which contexts
 // of few positions show in the output; the second product is 512 clocks of tensor pipe a tile, beside the 2900 clocks that a tile's bytes take from HBM.
 //
 // Roles: four warps of softmax; a warp that copies keys and values into a ring of tiles; a thread that issues the products; a warp that fetches the rows of
@@ -77,10 +77,13 @@ __device__ __forceinline__ unsigned long long now_ns() {
   return t;
 }
 // Waits for phase `n` (0, 1, ..) of a barrier; false, for everyone from then on, when it takes two seconds.  (The clock is looked at once in 256 tries:
-// reading it takes longer than most waits.)
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t n, volatile int* stop) {
+// reading it takes longer than most waits.  The loop is not inlined: some twenty waits, and the roles together have to fit the code that an SM keeps.)
+__device__ __noinline__ bool bar_wait_on(uint32_t bar, uint32_t parity, volatile int* stop) {
   unsigned long long t0 = 0;
-  for (uint32_t i = 1; !bar_try(b, n & 1); ++i) {
+  for (uint32_t i = 1;; ++i) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
     if ((i & 255) == 0) {
       const unsigned long long t = now_ns();
       if (t0 == 0) t0 = t;
@@ -88,8 +91,8 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t n, volatile int* 
       if (t - t0 > WAIT_NS) { *stop = 1; return false; }
     }
   }
-  return true;
 }
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t n, volatile int* stop) { return bar_try(b, n & 1) || bar_wait_on(smem_u32(b), n & 1, stop); }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
@@ -107,13 +110,6 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accum) : "memory");
-}
-// The same, adding to what is in d.
-__device__ __forceinline__ void mma_ss_add(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
-}
-__device__ __forceinline__ void mma_ts_add(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc) : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -200,6 +196,22 @@ __device__ __forceinline__ int share(int total, int w, int workers) {
   return q * w + r * w / workers;
 }
 
+// Tiles [t0, t1) of a worker.  Tiles of prefixes and of sequences' own positions have workers of their own, as many as their time asks for: a tile of own
+// positions, in short units, takes OWN_COST / PREFIX_COST times as long as one of a prefix.  No worker among those that share is without a tile.
+constexpr int PREFIX_COST = 2, OWN_COST = 3;
+__device__ __forceinline__ void share_of(int tp, int to, int W, int w, int& t0, int& t1) {
+  int wp = tp, wo = to;                                             // fewer tiles than workers: one each
+  if ((unsigned)tp + (unsigned)to > (unsigned)W) {
+    const float cp = (float)tp * PREFIX_COST, co = (float)to * OWN_COST;
+    wp = min(tp, max(tp > 0 ? 1 : 0, min(to > 0 ? W - 1 : W, (int)((float)W * cp / (cp + co) + 0.5f))));
+    wo = min(to, W - wp);
+    wp = min(tp, W - wo);                                           // (what the sequences do not need)
+  }
+  t0 = t1 = 0;
+  if (w < wp) { t0 = share(tp, w, wp); t1 = share(tp, w + 1, wp); }
+  else if (w < wp + wo) { t0 = tp + share(to, w - wp, wo); t1 = tp + share(to, w - wp + 1, wo); }
+}
+
 // The first unit of group g's prefix: no more units lie before it than sequences / spt + groups, for each kv head.
 __device__ __forceinline__ int prefix_unit(const Params& P, int g) { return (P.groups.first[g] / P.y.spt + g) * P.a.NKV; }
 
@@ -251,7 +263,7 @@ constexpr int SEGS = 8;                       // segments known ahead
 template <int SLOTS>
 struct Shared {
   uint64_t full[SLOTS], empty[SLOTS];         // ring of key / value tiles: K0 K1 V0 K2 V1 .. (V of tile n: use 2 n + 2)
-  uint64_t s_full[2], p_full[2], pv_done[2], o_full[2], o_free[2], q_full[4], q_free[4], seg_full[SEGS], seg_free[SEGS], pair[4];
+  uint64_t s_full[3], p_full[3], pv_done[3], o_full, o_free, q_full[4], q_free[4], seg_full[SEGS], seg_free[SEGS], pair[4];
   Segment seg[SEGS];
   float part[2][2][ROWS];                     // what the two warps of a row tell each other: by turn, by half
   uint32_t tmem;
@@ -266,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
   extern __shared__ __align__(256) unsigned char dyn[];
   __shared__ Shared<SLOTS> sh;
   constexpr int PAGES = TP / BS, HALF = TP / 2;                     // pages of a tile; columns of S that one half of the pages' positions take
-  constexpr int NO = TP == 128 ? 2 : 1;                             // accumulators of O: two where they fit
+  constexpr int C_O = 3 * TP;                                       // columns of tensor memory: three tiles of S, over which P is written, then O
   const etxb_attn_shared_args& a = P.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, HD = a.HD, worker = blockIdx.x;
   const uint32_t page_bytes = (uint32_t)HD * BS * 2, q_bytes = ROWS * (uint32_t)HD * 2;
@@ -279,7 +291,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
   cumulate(P, cum);
   if (tid == W_Q * 32) {
     for (int i = 0; i < SLOTS; ++i) { bar_init(&sh.full[i], 1); bar_init(&sh.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { bar_init(&sh.s_full[i], 1); bar_init(&sh.pv_done[i], 1); bar_init(&sh.p_full[i], SM_WARPS); bar_init(&sh.o_full[i], 1); bar_init(&sh.o_free[i], SM_WARPS); }
+    for (int i = 0; i < 3; ++i) { bar_init(&sh.s_full[i], 1); bar_init(&sh.p_full[i], SM_WARPS); bar_init(&sh.pv_done[i], 1); }
+    bar_init(&sh.o_full, 1); bar_init(&sh.o_free, SM_WARPS);
     for (int i = 0; i < 4; ++i) { bar_init(&sh.q_full[i], 32); bar_init(&sh.q_free[i], 1); bar_init(&sh.pair[i], 2); }
     for (int i = 0; i < SEGS; ++i) { bar_init(&sh.seg_full[i], 1); bar_init(&sh.seg_free[i], SM_WARPS + 3); }
     sh.stop = 0;
@@ -294,8 +307,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
-  const int total = cum.p[a.groups] + cum.s[a.seqs], workers = min(P.y.workers, total);        // (no worker without a tile among those that share)
-  const int t0 = worker < workers ? share(total, worker, workers) : 0, t1 = worker < workers ? share(total, worker + 1, workers) : 0;
+  int t0, t1;
+  share_of(cum.p[a.groups], cum.s[a.seqs], P.y.workers, worker, t0, t1);
   // A role's next segment (false: a wait ran out), and the end of its use.
   auto next_segment = [&](uint32_t k, Segment& s) {
     if (!bar_wait(&sh.seg_full[k % SEGS], k / SEGS, stop)) return false;
@@ -326,54 +339,63 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
       return y;
     };
     // Results of the segment before, written while the present one's first products run.
-    Segment prev = {};
+    int prev_rows = 0, prev_stride = 0;
+    float* prev_O = nullptr;
+    float2* prev_ml = nullptr;
     float prev_m = 0.f, prev_l = 0.f;
     auto write_out = [&](uint32_t sg) {
-      const uint32_t ob = sg % NO;
-      ok = ok && bar_wait(&sh.o_full[ob], sg / NO, stop);
+      ok = ok && bar_wait(&sh.o_full, sg, stop);
       ok = __all_sync(~0u, ok);
       fence_after();
-      if (ok && quarter * 32 < prev.rows) {
-        const int stride = prev.own ? P.y.G : P.y.prows;
-        const long long slot = (long long)(prev.own ? prev.unit - P.y.punits : prev.unit) + worker;
-        float* O = (prev.own ? P.y.oO : P.y.pO) + slot * stride * HD + (size_t)row * 4;
-        const float l2 = exchange(prev_l);
-        if (hf == 0 && row < prev.rows) *(float2*)((prev.own ? P.y.oml : P.y.pml) + (slot * stride + row) * 2) = make_float2(prev_m, prev_l + l2);
-        const int mid = (HD / 16 + 1) / 2 * 16;
-#pragma unroll 1
-        for (int c = hf ? mid : 0; c < (hf ? HD : mid); c += 16) {
-          uint32_t r[16];
-          tmem_ld16(tmem + lanes + 2 * TP + ob * HD + c, r);
-          tmem_wait_ld();
-          if (row < prev.rows) {
+      const bool mine = ok && quarter * 32 < prev_rows;
+      const float l2 = mine ? exchange(prev_l) : 0.f;
+      const int mid = (HD / 16 + 1) / 2 * 16, c0 = hf ? mid : 0, c1 = hf ? HD : mid;             // this warp's columns
+      for (int cc = c0; cc < c1; cc += 64) {                        // (once up to 128 elements per head)
+        uint32_t r[64];
+        if (mine) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) *(uint4*)(O + (size_t)(c / 4 + k) * stride * 4) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
-          }
+          for (int k = 0; k < 4; ++k) if (cc + 16 * k < c1) tmem_ld16(tmem + lanes + C_O + cc + 16 * k, r + 16 * k);
+          tmem_wait_ld();
+        }
+        if (cc + 64 >= c1) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&sh.o_free);
+        }
+        if (mine && row < prev_rows) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (cc + 4 * k < c1) *(uint4*)(prev_O + (size_t)(cc / 4 + k) * prev_stride * 4) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
         }
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&sh.o_free[ob]);
+      if (c0 >= c1) {                                               // (16 elements per head: the other warp has them all)
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sh.o_free);
+      }
+      if (mine && hf == 0 && row < prev_rows) *prev_ml = make_float2(prev_m, prev_l + l2);
     };
-    for (int t = t0; t < t1 && ok; ++seg) {
+    for (int t = t0; ok; ++seg) {
       Segment s;
-      ok = __all_sync(~0u, next_segment(seg, s));
+      s.n = 1;                                                      // (a round behind the last segment, for its results)
+      const bool more = t < t1;
+      if (more) ok = __all_sync(~0u, next_segment(seg, s));
       if (!ok) break;
       const bool busy = quarter * 32 < s.rows;                      // (a warp without rows only keeps the others' time)
       for (int i = 0; i < s.n && ok; ++i, ++n) {
-        const uint32_t sb = n & 1, scol = tmem + lanes + sb * TP + hf * (MINE / 2);
-        ok = bar_wait(&sh.s_full[sb], n >> 1, stop);
+        if (more) {
+        const uint32_t sb = n % 3, scol = tmem + lanes + sb * TP + hf * (MINE / 2);
+        ok = bar_wait(&sh.s_full[sb], n / 3, stop);
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         fence_after();
         if (busy) {
-          // r: position p of the warp's is at p / 8 % 2 * (MINE / 2) + p / 16 * 8 + p % 8
+          // position p of the warp's is at p / 8 % 2 * (MINE / 2) + p / 16 * 8 + p % 8
           uint32_t r[MINE];
           if (MINE == 64) { tmem_ld32(scol, r); tmem_ld32(scol + HALF, r + MINE / 2); }
           else { tmem_ld16(scol, r); tmem_ld16(scol + HALF, r + MINE / 2); }
           tmem_wait_ld();
           const int valid = s.len - (s.tile0 + i) * TP - hf * MINE;
-          if (valid < MINE) {
+          if (valid < MINE) {                                       // scores behind the last position become minus infinity
 #pragma unroll
             for (int c = 0; c < MINE; ++c) if (c % (MINE / 2) / 8 * 16 + c / (MINE / 2) * 8 + c % 8 >= valid) r[c] = 0xff800000u;
           }
@@ -391,11 +413,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
             const bool up = row < s.rows && m != -INFINITY && (mt - m) * sl > 8.f;
             if (__any_sync(~0u, up)) {
               const float f = up ? ex2((m - mt) * sl) : 1.f;
-              ok = bar_wait(&sh.pv_done[(n - 1) & 1], (n - 1) >> 1, stop);
+              ok = bar_wait(&sh.pv_done[(n - 1) % 3], (n - 1) / 3, stop);
               ok = __all_sync(~0u, ok);
               if (!ok) break;
               fence_after();
-              const uint32_t ocol = tmem + lanes + 2 * TP + (seg % NO) * HD;
+              const uint32_t ocol = tmem + lanes + C_O;
               const int mid = (HD / 16 + 1) / 2 * 16;
 #pragma unroll 1
               for (int c = hf ? mid : 0; c < (hf ? HD : mid); c += 16) {
@@ -424,13 +446,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
                   const int pos = 32 * j + 2 * k + e;
                   p[e] = ex2(__fmaf_rn(__uint_as_float(r[pos / 8 % 2 * (MINE / 2) + pos / 16 * 8 + pos % 8]), sl, -ms));
                   ls[k & 3] += p[e];
-                  // hi: the upper 16 bits; lo: what is left and 2^-22 of p more, so that it is never 0 where p is not (0 x inf would spoil the sum of
-                  // an infinite value) nor negative
-                  y[e] = __fmaf_rn(p[e], 1.0f + 0x1p-22f, -__uint_as_float(__float_as_uint(p[e]) & 0xffff0000u));
+                  // hi: the upper 16 bits; lo: the upper 16 bits of what is left and 2^-17 of p more -- what the cut takes off on the average, and so
+                  // that lo is never 0 where p is not (0 x inf would spoil the sum of an infinite value) nor negative
+                  y[e] = __fmaf_rn(p[e], 1.0f + 0x1p-17f, -__uint_as_float(__float_as_uint(p[e]) & 0xffff0000u));
                 }
                 hi[k] = __byte_perm(__float_as_uint(p[0]), __float_as_uint(p[1]), 0x7632);
-                const __nv_bfloat162 b2 = __floats2bfloat162_rn(y[0], y[1]);
-                lo[k] = *(const uint32_t*)&b2;
+                lo[k] = __byte_perm(__float_as_uint(y[0]), __float_as_uint(y[1]), 0x7632);
               }
               tmem_st16(scol + 16 * j, hi);
               tmem_st16(scol + HALF + 16 * j, lo);
@@ -442,14 +463,21 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
         fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&sh.p_full[sb]);
+        }
         if (i == 0 && seg > 0) write_out(seg - 1);
       }
-      prev = s; prev_m = m == -INFINITY ? m : m * sl; prev_l = l;
+      if (!more) break;
+      {
+        const long long slot = (long long)(s.own ? s.unit - P.y.punits : s.unit) + worker;
+        prev_rows = s.rows; prev_stride = s.own ? P.y.G : P.y.prows;
+        prev_O = (s.own ? P.y.oO : P.y.pO) + slot * prev_stride * HD + (size_t)row * 4;
+        prev_ml = (float2*)(s.own ? P.y.oml : P.y.pml) + slot * prev_stride + row;
+      }
+      prev_m = m == -INFINITY ? m : m * sl; prev_l = l;
       __syncwarp();
       if (lane == 0) bar_arrive(&sh.seg_free[seg % SEGS]);
       t += s.n;
     }
-    if (ok && seg > 0) write_out(seg - 1);
   } else if (warp == W_COPY) {
     // ---- copies: a lane per page
     uint32_t use = 0, filled[SLOTS] = {}, seg = 0;                  // running number of ring slots taken; how often each was
@@ -525,29 +553,20 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
         for (int i = 0; i < s.n && ok; ++i, ++n) {
           const int np = min(PAGES, (s.len + BS - 1) / BS - (s.tile0 + i) * PAGES);
           const uint32_t use = n == 0 ? 0 : 2 * n - 1, sl = use % SLOTS;
-          if (n >= 2) ok = bar_wait(&sh.pv_done[n & 1], (n >> 1) - 1, stop);         // (P of tile n - 2 lies where S of this one goes)
+          const uint32_t sb = n % 3;
+          if (n >= 3) ok = bar_wait(&sh.pv_done[sb], n / 3 - 1, stop);               // (P of tile n - 3 lies where S of this one goes)
           ok = ok && bar_wait(&sh.full[sl], use / SLOTS, stop);
           if (!ok) break;
           fence_after();
           const uint32_t id = idesc | ((uint32_t)((np + 1) & ~1) << 17);             // N = 8 positions of each page, a multiple of 16
-          const uint32_t d = tmem + (n & 1) * TP;
+          const uint32_t d = tmem + sb * TP;
           const uint64_t b0 = desc(smem_u32(base + sl * SLOT_BYTES), 256, page_bytes, 0);
-          mma_ss(d, ad, b0, id, 0u);
-          mma_ss(d + HALF, ad, b0 + (128 >> 4), id, 0u);
-          if (TP == 128 && HD == 128) {
-#pragma unroll
-            for (int k = 1; k < 8; ++k) {
-              mma_ss_add(d, ad + k * astep, b0 + k * (512 >> 4), id);
-              mma_ss_add(d + HALF, ad + k * astep, b0 + k * (512 >> 4) + (128 >> 4), id);
-            }
-          } else {
 #pragma unroll 1
-            for (int k = 1; k < HD / 16; ++k) {
-              mma_ss_add(d, ad + k * astep, b0 + k * (512 >> 4), id);
-              mma_ss_add(d + HALF, ad + k * astep, b0 + k * (512 >> 4) + (128 >> 4), id);
-            }
+          for (int k = 0; k < HD / 16; ++k) {
+            mma_ss(d, ad + k * astep, b0 + k * (512 >> 4), id, k);
+            mma_ss(d + HALF, ad + k * astep, b0 + k * (512 >> 4) + (128 >> 4), id, k);
           }
-          mma_commit(&sh.s_full[n & 1]);
+          mma_commit(&sh.s_full[sb]);
           mma_commit(&sh.empty[sl]);
           if (i == s.n - 1) mma_commit(&sh.q_free[seg & 3]);
         }
@@ -566,12 +585,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
     for (int t = t0; t < t1 && ok; ++seg) {
       Segment s;
       ok = next_segment(seg, s);
-      const uint32_t ob = seg % NO, d = tmem + 2 * TP + ob * HD;
-      if (seg >= NO) ok = ok && bar_wait(&sh.o_free[ob], seg / NO - 1, stop);
+      const uint32_t d = tmem + C_O;
+      if (seg > 0) ok = ok && bar_wait(&sh.o_free, seg - 1, stop);
       ok = __all_sync(~0u, ok);
       for (int i = 0; i < s.n && ok; ++i, ++n) {
         const int np = min(PAGES, (s.len + BS - 1) / BS - (s.tile0 + i) * PAGES);
-        const uint32_t use = 2 * n + 2, sl = use % SLOTS, pc = tmem + (n & 1) * TP;
+        const uint32_t use = 2 * n + 2, sl = use % SLOTS, sb = n % 3, pc = tmem + sb * TP;
         ok = bar_wait(&sh.full[sl], use / SLOTS, stop);
         const int rem = s.len % BS, page = (s.len - 1) / BS - (s.tile0 + i) * PAGES;
         if (ok && rem && page < PAGES) {
@@ -591,30 +610,20 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
           }
           fence_async();
         }
-        ok = ok && bar_wait(&sh.p_full[n & 1], n >> 1, stop);
+        ok = ok && bar_wait(&sh.p_full[sb], n / 3, stop);
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         fence_after();
         if (elect()) {
           const uint64_t b = desc(smem_u32(base + sl * SLOT_BYTES), 16, 256, 6);
-          mma_ts(d, pc, b, idesc, i == 0 ? 0u : 1u);
-          mma_ts_add(d, pc + TP / 2, b, idesc);
-          if (np == PAGES) {
-#pragma unroll
-            for (int k = 1; k < PAGES; ++k) {
-              mma_ts_add(d, pc + 8 * k, b + k * step, idesc);
-              mma_ts_add(d, pc + TP / 2 + 8 * k, b + k * step, idesc);
-            }
-          } else {
 #pragma unroll 1
-            for (int k = 1; k < np; ++k) {
-              mma_ts_add(d, pc + 8 * k, b + k * step, idesc);
-              mma_ts_add(d, pc + TP / 2 + 8 * k, b + k * step, idesc);
-            }
+          for (int k = 0; k < np; ++k) {
+            mma_ts(d, pc + 8 * k, b + k * step, idesc, i + k);
+            mma_ts(d, pc + TP / 2 + 8 * k, b + k * step, idesc, 1u);
           }
-          mma_commit(&sh.pv_done[n & 1]);
+          mma_commit(&sh.pv_done[sb]);
           mma_commit(&sh.empty[sl]);
-          if (i == s.n - 1) mma_commit(&sh.o_full[ob]);
+          if (i == s.n - 1) mma_commit(&sh.o_full);
         }
         __syncwarp();
       }

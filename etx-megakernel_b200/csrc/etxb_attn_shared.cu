@@ -32,8 +32,8 @@
 
 namespace etxb_shared {
 
-constexpr int BS = 16, ROWS = 128, SLOT_BYTES = 32768, OWN_ROWS = 16;
-constexpr int SM_WARPS = 8, W_COPY = 8, W_QK = 9, W_PV = 10, W_Q = 11, THREADS = 384;
+constexpr int BS = 16, ROWS = 128, OWN_ROWS = 16, MAX_SLOTS = 16;
+constexpr int SETS = 2, SET_WARPS = 8, W_COPY = 16, W_QK = 17, W_PV = 18, W_Q = 19, THREADS = 640;
 constexpr unsigned long long WAIT_NS = 2000000000ull;
 
 struct Groups { int32_t first[ETXB_SHARED_MAX_SEQS + 1]; };
@@ -44,6 +44,7 @@ struct Layout {
   int tp;                     // positions of a tile
   int workers;
   int prows;                  // rows of a slot of a prefix
+  int slots, qrows;           // of the kernel's shared memory: tiles of keys or values in the ring (even), rows of Q kept for a prefix
   int punits;                 // units of prefixes, counted generously (see prefix_unit); a unit's parts lie in the slots unit + worker
   long long pslots, oslots;   // slots of prefixes / of own positions
   float* pO; float* pml; float* oO; float* oml;      // [slot][HD / 4][rows][4], [slot][rows][2] (m in units of log2, l)
@@ -143,6 +144,29 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) { return pack2(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+  lo = __uint_as_float(a); hi = __uint_as_float(b);
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 // ------------------------------------------------------------------------------------------------ shares
@@ -260,41 +284,44 @@ __device__ __forceinline__ void segment_at(const Params& P, const Cum& c, int t,
 
 // ------------------------------------------------------------------------------------------------ the tiles
 constexpr int SEGS = 8;                       // segments known ahead
-template <int SLOTS>
 struct Shared {
-  uint64_t full[SLOTS], empty[SLOTS];         // ring of key / value tiles: K0 K1 V0 K2 V1 .. (V of tile n: use 2 n + 2)
-  uint64_t s_full[3], p_full[3], pv_done[3], o_full, o_free, q_full[4], q_free[4], seg_full[SEGS], seg_free[SEGS], pair[4];
+  uint64_t full[MAX_SLOTS], empty[MAX_SLOTS];       // ring of key / value tiles: K0 K1 V0 K2 V1 .. (V of tile n: use 2 n + 2)
+  uint64_t s_full[3], p_full[3], pv_done[3], o_full[SETS], o_free, q_full[4], q_free[4], seg_full[SEGS], seg_free[SEGS], pair[SETS][4], m_full[3][4];
   Segment seg[SEGS];
-  float part[2][2][ROWS];                     // what the two warps of a row tell each other: by turn, by half
+  float part[SETS][2][2][ROWS];               // maxima that the two warps of a row tell each other: by set, turn, half
+  float m[3][ROWS];                           // each row's maximum after tile n, at n % 3
+  float2 l[2][SETS][2][ROWS];                 // a set's sums of a segment and the maximum they are relative to: by turn of segments, set, half
   uint32_t tmem;
   int stop;
 };
 
-// Shared memory: SLOTS tiles of keys or values, Q, the tiles before each group and sequence and their lengths.
-// SLOTS is even: values always lie in the even slots, so that whoever looks at values alone sees every use of its slots (but the first of slot 0).
-constexpr int fixed_bytes(int hd, int slots) { return 256 + slots * SLOT_BYTES + ROWS * hd * 2; }
-template <int TP, int SLOTS>
+// Dynamic shared memory: the ring (y.slots tiles), Q (y.qrows rows, four sequences' at least), the tiles before each group and sequence and their lengths.
+// The number of slots is even: values always lie in the even slots, so that whoever looks at values alone sees every use of its slots (but the first of slot
+// 0).  Behind it all 2 KB: an instruction reads 128 rows of Q, and where there are fewer the last ones lie behind the buffer.
+__host__ __device__ __forceinline__ int q_size(int hd, int qrows) { return (qrows > 4 * OWN_ROWS ? qrows : 4 * OWN_ROWS) * hd * 2; }
+template <int TP>
 __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant__ Params P) {
   extern __shared__ __align__(256) unsigned char dyn[];
-  __shared__ Shared<SLOTS> sh;
+  __shared__ Shared sh;
   constexpr int PAGES = TP / BS, HALF = TP / 2;                     // pages of a tile; columns of S that one half of the pages' positions take
   constexpr int C_O = 3 * TP;                                       // columns of tensor memory: three tiles of S, over which P is written, then O
   const etxb_attn_shared_args& a = P.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, HD = a.HD, worker = blockIdx.x;
-  const uint32_t page_bytes = (uint32_t)HD * BS * 2, q_bytes = ROWS * (uint32_t)HD * 2;
+  const uint32_t page_bytes = (uint32_t)HD * BS * 2, q_bytes = q_size(HD, P.y.qrows), slot_bytes = PAGES * page_bytes, SLOTS = P.y.slots;
   unsigned char* const base = (unsigned char*)(((uintptr_t)dyn + 255) & ~(uintptr_t)255);
-  unsigned char* const qbuf = base + SLOTS * SLOT_BYTES;
+  unsigned char* const qbuf = base + SLOTS * slot_bytes;
   const Cum cum = {(int32_t*)(qbuf + q_bytes), (int32_t*)(qbuf + q_bytes) + a.groups + 1, (int32_t*)(qbuf + q_bytes) + a.groups + a.seqs + 2};
   volatile int* const stop = &sh.stop;
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (what follows on the device waits for this grid before it reads)
   cumulate(P, cum);
   if (tid == W_Q * 32) {
     for (int i = 0; i < SLOTS; ++i) { bar_init(&sh.full[i], 1); bar_init(&sh.empty[i], 1); }
-    for (int i = 0; i < 3; ++i) { bar_init(&sh.s_full[i], 1); bar_init(&sh.p_full[i], SM_WARPS); bar_init(&sh.pv_done[i], 1); }
-    bar_init(&sh.o_full, 1); bar_init(&sh.o_free, SM_WARPS);
-    for (int i = 0; i < 4; ++i) { bar_init(&sh.q_full[i], 32); bar_init(&sh.q_free[i], 1); bar_init(&sh.pair[i], 2); }
-    for (int i = 0; i < SEGS; ++i) { bar_init(&sh.seg_full[i], 1); bar_init(&sh.seg_free[i], SM_WARPS + 3); }
+    for (int i = 0; i < 3; ++i) { bar_init(&sh.s_full[i], 1); bar_init(&sh.p_full[i], SET_WARPS); bar_init(&sh.pv_done[i], 1); }
+    for (int i = 0; i < 12; ++i) bar_init(&sh.m_full[i / 4][i % 4], 1);
+    for (int i = 0; i < SETS; ++i) bar_init(&sh.o_full[i], 1);
+    bar_init(&sh.o_free, SET_WARPS);
+    for (int i = 0; i < 4; ++i) { bar_init(&sh.q_full[i], 32); bar_init(&sh.q_free[i], 1); bar_init(&sh.pair[0][i], 2); bar_init(&sh.pair[1][i], 2); }
+    for (int i = 0; i < SEGS; ++i) { bar_init(&sh.seg_full[i], 1); bar_init(&sh.seg_free[i], SETS * SET_WARPS + 3); }
     sh.stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -316,188 +343,198 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
     return true;
   };
 
-  if (warp < SM_WARPS) {
-    // ---- softmax: a row belongs to a lane of two warps, each of which has half of a tile's positions: blocks of 16 columns of S in both halves
+  if (warp < SETS * SET_WARPS) {
+    // ---- softmax: set n % 2 has tile n, so that one set's waits are the other's work.  In a set, a row belongs to a lane of two warps, each of which has half
+    // of the tile's positions: blocks of 16 columns of S in both halves.
     constexpr int MINE = TP / 2;                                    // positions of a warp
-    const int quarter = warp & 3, hf = warp >> 2, row = quarter * 32 + lane;
+    const int set = warp / SET_WARPS, quarter = warp & 3, hf = (warp >> 2) & 1, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     // scores in units of log2 (a scale of 0 as the least there is: a masked score stays minus infinity)
     const float sl = fmaxf(a.scale * 1.4426950408889634f, 1e-37f);
-    uint32_t n = 0, seg = 0, turn = 0;
-    float m = -INFINITY, l = 0.f;
+    uint32_t n = 0, seg = 0, turn = 0, outs = 0;                    // tiles and segments so far, of both sets; exchanges, and segments that this set wrote out
+    float m = -INFINITY, l = 0.f;                                   // the row's maximum, and this warp's sum relative to it
     bool ok = true;
-    // tells the other warp of the row x and gets its value
-    auto exchange = [&](float x) {
-      float* mine = &sh.part[turn & 1][hf][row];
-      *mine = x;
-      __syncwarp();
-      if (lane == 0) bar_arrive(&sh.pair[quarter]);
-      ok = ok && bar_wait(&sh.pair[quarter], turn, stop);
-      ok = __all_sync(~0u, ok);
-      const float y = sh.part[turn & 1][hf ^ 1][row];
-      ++turn;
-      return y;
-    };
-    // Results of the segment before, written while the present one's first products run.
-    int prev_rows = 0, prev_stride = 0;
-    float* prev_O = nullptr;
-    float2* prev_ml = nullptr;
-    float prev_m = 0.f, prev_l = 0.f;
-    auto write_out = [&](uint32_t sg) {
-      ok = ok && bar_wait(&sh.o_full, sg, stop);
-      ok = __all_sync(~0u, ok);
-      fence_after();
-      const bool mine = ok && quarter * 32 < prev_rows;
-      const float l2 = mine ? exchange(prev_l) : 0.f;
-      const int mid = (HD / 16 + 1) / 2 * 16, c0 = hf ? mid : 0, c1 = hf ? HD : mid;             // this warp's columns
-      for (int cc = c0; cc < c1; cc += 64) {                        // (once up to 128 elements per head)
-        uint32_t r[64];
-        if (mine) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) if (cc + 16 * k < c1) tmem_ld16(tmem + lanes + C_O + cc + 16 * k, r + 16 * k);
-          tmem_wait_ld();
-        }
-        if (cc + 64 >= c1) {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(&sh.o_free);
-        }
-        if (mine && row < prev_rows) {
-#pragma unroll
-          for (int k = 0; k < 16; ++k)
-            if (cc + 4 * k < c1) *(uint4*)(prev_O + (size_t)(cc / 4 + k) * prev_stride * 4) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
-        }
-      }
-      if (c0 >= c1) {                                               // (16 elements per head: the other warp has them all)
-        __syncwarp();
-        if (lane == 0) bar_arrive(&sh.o_free);
-      }
-      if (mine && hf == 0 && row < prev_rows) *prev_ml = make_float2(prev_m, prev_l + l2);
-    };
-    for (int t = t0; ok; ++seg) {
+    for (int t = t0; t < t1 && ok; ++seg) {
       Segment s;
-      s.n = 1;                                                      // (a round behind the last segment, for its results)
-      const bool more = t < t1;
-      if (more) ok = __all_sync(~0u, next_segment(seg, s));
-      if (!ok) break;
+      ok = __all_sync(~0u, next_segment(seg, s));
       const bool busy = quarter * 32 < s.rows;                      // (a warp without rows only keeps the others' time)
-      for (int i = 0; i < s.n && ok; ++i, ++n) {
-        if (more) {
-        const uint32_t sb = n % 3, scol = tmem + lanes + sb * TP + hf * (MINE / 2);
-        ok = bar_wait(&sh.s_full[sb], n / 3, stop);
+      const int mine = set ^ (n & 1);                               // the first tile of this segment that is the set's
+      m = -INFINITY; l = 0.f;
+      for (int i = mine; i < s.n && ok; i += 2) {
+        const uint32_t tile = n + i, sb = tile % 3, scol = tmem + lanes + sb * TP + hf * (MINE / 2);
+        ok = bar_wait(&sh.s_full[sb], tile / 3, stop);
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         fence_after();
         if (busy) {
-          // position p of the warp's is at p / 8 % 2 * (MINE / 2) + p / 16 * 8 + p % 8
-          uint32_t r[MINE];
-          if (MINE == 64) { tmem_ld32(scol, r); tmem_ld32(scol + HALF, r + MINE / 2); }
-          else { tmem_ld16(scol, r); tmem_ld16(scol + HALF, r + MINE / 2); }
-          tmem_wait_ld();
           const int valid = s.len - (s.tile0 + i) * TP - hf * MINE;
-          if (valid < MINE) {                                       // scores behind the last position become minus infinity
-#pragma unroll
-            for (int c = 0; c < MINE; ++c) if (c % (MINE / 2) / 8 * 16 + c / (MINE / 2) * 8 + c % 8 >= valid) r[c] = 0xff800000u;
-          }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int c = 0; c < MINE; c += 8)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1])));
-          float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          mt = fmaxf(mt, exchange(mt));
-          if (!ok) break;
-          if (i == 0) { m = mt; l = 0.f; }
-          else {
-            // the maximum moves only when the new one is above it by a factor of 2^8 or more: till then probabilities of up to 2^8 do no harm
-            const bool up = row < s.rows && m != -INFINITY && (mt - m) * sl > 8.f;
-            if (__any_sync(~0u, up)) {
-              const float f = up ? ex2((m - mt) * sl) : 1.f;
-              ok = bar_wait(&sh.pv_done[(n - 1) % 3], (n - 1) / 3, stop);
-              ok = __all_sync(~0u, ok);
-              if (!ok) break;
-              fence_after();
-              const uint32_t ocol = tmem + lanes + C_O;
-              const int mid = (HD / 16 + 1) / 2 * 16;
 #pragma unroll 1
-              for (int c = hf ? mid : 0; c < (hf ? HD : mid); c += 16) {
-                uint32_t o[16];
-                tmem_ld16(ocol + c, o);
-                tmem_wait_ld();
+          for (int j = 0; j < MINE / 32; ++j) {                     // 32 positions: page 2 j + k / 8, half h of it, its position k % 8 (k < 16)
+            uint32_t r[32];
+            tmem_ld16(scol + 16 * j, r);
+            tmem_ld16(scol + HALF + 16 * j, r + 16);
+            tmem_wait_ld();
+            const int left = valid - 32 * j;
+            if (left < 32) {                                        // scores behind the last position become minus infinity
 #pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                tmem_st16(ocol + c, o);
-              }
-              l *= f;
+              for (int c = 0; c < 32; ++c) if (c % 16 / 8 * 16 + c / 16 * 8 + c % 8 >= left) r[c] = 0xff800000u;
+              tmem_st16(scol + 16 * j, r);
+              tmem_st16(scol + HALF + 16 * j, r + 16);
+              tmem_wait_st();
             }
-            if (up || m == -INFINITY) m = mt;
+#pragma unroll
+            for (int c = 0; c < 32; c += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1])));
           }
-          if (valid > 0) {                                          // (nothing multiplies the pages behind the last)
-            const float ms = m == -INFINITY ? 0.f : m * sl;
-            float ls[4] = {0.f, 0.f, 0.f, 0.f};
+          float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          // the other warp's, and the maximum after the tile before
+          sh.part[set][turn & 1][hf][row] = mt;
+          __syncwarp();
+          if (lane == 0) bar_arrive(&sh.pair[set][quarter]);
+          ok = bar_wait(&sh.pair[set][quarter], turn, stop);
+          if (tile > 0) ok = ok && bar_wait(&sh.m_full[(tile - 1) % 3][quarter], (tile - 1) / 3, stop);
+          ok = __all_sync(~0u, ok);
+          if (!ok) break;
+          mt = fmaxf(mt, sh.part[set][turn & 1][hf ^ 1][row]);
+          ++turn;
+          const float m0 = i == 0 ? -INFINITY : sh.m[(tile - 1) % 3][row];
+          // the maximum moves only when the new one is above it by a factor of 2^8 or more: till then probabilities of up to 2^8 do no harm
+          const bool up = row < s.rows && m0 != -INFINITY && (mt - m0) * sl > 8.f;
+          const float m1 = up || m0 == -INFINITY ? mt : m0;
+          if (hf == 0) {
+            sh.m[sb][row] = m1;
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.m_full[sb][quarter]);
+          }
+          if (m1 != m) { l = l == 0.f ? 0.f : l * ex2((m - m1) * sl); m = m1; }
+          if (__any_sync(~0u, up)) {
+            const float f = up ? ex2((m0 - m1) * sl) : 1.f;
+            ok = bar_wait(&sh.pv_done[(tile - 1) % 3], (tile - 1) / 3, stop);
+            ok = __all_sync(~0u, ok);
+            if (!ok) break;
+            fence_after();
+            const uint32_t ocol = tmem + lanes + C_O;
+            const int mid = (HD / 16 + 1) / 2 * 16;
+#pragma unroll 1
+            for (int c = hf ? mid : 0; c < (hf ? HD : mid); c += 16) {
+              uint32_t o[16];
+              tmem_ld16(ocol + c, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < MINE / 32; ++j) {                   // two pages at a time: 16 columns of hi, 16 of lo
-              uint32_t hi[16], lo[16];
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                float p[2], y[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int pos = 32 * j + 2 * k + e;
-                  p[e] = ex2(__fmaf_rn(__uint_as_float(r[pos / 8 % 2 * (MINE / 2) + pos / 16 * 8 + pos % 8]), sl, -ms));
-                  ls[k & 3] += p[e];
-                  // hi: the upper 16 bits; lo: the upper 16 bits of what is left and 2^-17 of p more -- what the cut takes off on the average, and so
-                  // that lo is never 0 where p is not (0 x inf would spoil the sum of an infinite value) nor negative
-                  y[e] = __fmaf_rn(p[e], 1.0f + 0x1p-17f, -__uint_as_float(__float_as_uint(p[e]) & 0xffff0000u));
-                }
-                hi[k] = __byte_perm(__float_as_uint(p[0]), __float_as_uint(p[1]), 0x7632);
-                lo[k] = __byte_perm(__float_as_uint(y[0]), __float_as_uint(y[1]), 0x7632);
-              }
-              tmem_st16(scol + 16 * j, hi);
-              tmem_st16(scol + HALF + 16 * j, lo);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st16(ocol + c, o);
             }
-            l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-            tmem_wait_st();
+          }
+          const float ms = m == -INFINITY ? 0.f : m * sl;
+          const uint64_t sl2 = pack2(sl, sl), ms2 = pack2(-ms, -ms), c2 = pack2(1.0f + 0x1p-17f, 1.0f + 0x1p-17f);
+          uint64_t ls[2] = {0, 0};
+          // two pages at a time, over whose scores 16 columns of hi and 16 of lo are written (pages behind the last are not multiplied).  The scores are read
+          // twice, and in loops: more registers would cost warps, and code that an SM does not keep costs more.
+#pragma unroll 1
+          for (int j = 0; j < MINE / 32 && 32 * j < valid; ++j) {
+            uint32_t a0[16], a1[16];
+            tmem_ld16(scol + 16 * j, a0);
+            tmem_ld16(scol + HALF + 16 * j, a1);
+            tmem_wait_ld();
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {                          // positions 2 k and 2 k + 1
+              const int pos = 2 * k, c = pos / 16 * 8 + pos % 8;
+              const uint64_t v = (pos & 8) ? pack2(a1[c], a1[c + 1]) : pack2(a0[c], a0[c + 1]);
+              float p0, p1, y0, y1;
+              unpack2(fma2(v, sl2, ms2), p0, p1);
+              p0 = ex2(p0); p1 = ex2(p1);
+              const uint64_t p = pack2(p0, p1);
+              ls[k & 1] = add2(ls[k & 1], p);
+              // hi: the upper 16 bits; lo: the upper 16 bits of what is left and 2^-17 of p more -- what the cut takes off on the average, and so that lo
+              // is never 0 where p is not (0 x inf would spoil the sum of an infinite value) nor negative
+              const uint32_t u0 = __float_as_uint(p0), u1 = __float_as_uint(p1);
+              unpack2(fma2(p, c2, pack2((u0 & 0xffff0000u) ^ 0x80000000u, (u1 & 0xffff0000u) ^ 0x80000000u)), y0, y1);
+              hi[k] = __byte_perm(u0, u1, 0x7632);
+              lo[k] = __byte_perm(__float_as_uint(y0), __float_as_uint(y1), 0x7632);
+            }
+            tmem_st16(scol + 16 * j, hi);
+            tmem_st16(scol + HALF + 16 * j, lo);
+          }
+          {
+            float x, y;
+            unpack2(add2(ls[0], ls[1]), x, y);
+            l += x + y;
+          }
+          if (i + 2 >= s.n) sh.l[seg & 1][set][hf][row] = make_float2(m, l);
+          tmem_wait_st();
+        } else if (hf == 0 && lane == 0) bar_arrive(&sh.m_full[sb][quarter]);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sh.p_full[sb]);
+        if (i + 1 < s.n) continue;
+        // the unit's part in this segment: its set of the last tile writes it out, when the other set's warps have left their sums
+        if (busy) {
+          if (lane == 0) bar_arrive(&sh.pair[set][quarter]);
+          ok = bar_wait(&sh.pair[set][quarter], turn++, stop);
+        }
+        ok = ok && bar_wait(&sh.o_full[set], outs++, stop);
+        if (s.n > 1) ok = ok && bar_wait(&sh.p_full[(tile - 1) % 3], (tile - 1) / 3, stop);
+        ok = __all_sync(~0u, ok);
+        fence_after();
+        const int mid = (HD / 16 + 1) / 2 * 16, c0 = hf ? mid : 0, c1 = hf ? HD : mid;           // this warp's columns
+        const int stride = s.own ? P.y.G : P.y.prows;
+        const long long slot = (long long)(s.own ? s.unit - P.y.punits : s.unit) + worker;
+        const bool writes = ok && row < s.rows;
+        float* O = (s.own ? P.y.oO : P.y.pO) + slot * stride * HD + (size_t)row * 4;
+#pragma unroll 1
+        for (int c = c0; c < c1; c += 32) {
+          uint32_t r[32];
+          if (ok && busy) {
+            tmem_ld16(tmem + lanes + C_O + c, r);
+            if (c + 16 < c1) tmem_ld16(tmem + lanes + C_O + c + 16, r + 16);
+            tmem_wait_ld();
+          }
+          if (writes) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (c + 4 * k < c1) *(uint4*)(O + (size_t)(c / 4 + k) * stride * 4) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
           }
         }
         fence_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(&sh.p_full[sb]);
+        if (lane == 0) bar_arrive(&sh.o_free);
+        if (writes && hf == 0) {
+          float L = 0.f;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {                             // the set's own two, then the other's
+            if (x >= 2 && s.n == 1) break;
+            const float2 p = sh.l[seg & 1][set ^ (x >> 1)][x & 1][row];
+            if (p.y != 0.f) L += p.x == m ? p.y : p.y * ex2((p.x - m) * sl);
+          }
+          *((float2*)(s.own ? P.y.oml : P.y.pml) + slot * stride + row) = make_float2(m == -INFINITY ? m : m * sl, L);
         }
-        if (i == 0 && seg > 0) write_out(seg - 1);
       }
-      if (!more) break;
-      {
-        const long long slot = (long long)(s.own ? s.unit - P.y.punits : s.unit) + worker;
-        prev_rows = s.rows; prev_stride = s.own ? P.y.G : P.y.prows;
-        prev_O = (s.own ? P.y.oO : P.y.pO) + slot * prev_stride * HD + (size_t)row * 4;
-        prev_ml = (float2*)(s.own ? P.y.oml : P.y.pml) + slot * prev_stride + row;
-      }
-      prev_m = m == -INFINITY ? m : m * sl; prev_l = l;
+      n += s.n;
       __syncwarp();
       if (lane == 0) bar_arrive(&sh.seg_free[seg % SEGS]);
       t += s.n;
     }
   } else if (warp == W_COPY) {
     // ---- copies: a lane per page
-    uint32_t use = 0, filled[SLOTS] = {}, seg = 0;                  // running number of ring slots taken; how often each was
+    uint32_t use = 0, sl = 0, round = 0, seg = 0;                   // running number of ring slots taken, the next one, how often it was before
     bool ok = true, have = false;
     int vp = 0, vn = 0, vh = 0;                                     // the tile whose values follow
     auto put = [&](int n_pages, int page, int h, bool values) {
-      const uint32_t sl = use % SLOTS, round = use / SLOTS;
       if (round > 0) ok = ok && bar_wait(&sh.empty[sl], round - 1, stop);
       ok = __all_sync(~0u, ok);
       if (!ok) return;
-#pragma unroll
-      for (int i = 0; i < SLOTS; ++i) if (sl == i) filled[i] = round + 1;
       if (lane == 0) bar_expect(&sh.full[sl], n_pages * page_bytes);
       __syncwarp();
-      unsigned char* dst = base + sl * SLOT_BYTES + lane * page_bytes;
+      unsigned char* dst = base + sl * slot_bytes + lane * page_bytes;
       if (lane < n_pages) {
         if (values) tma_load_3d(dst, &P.vmap, h * HD, page, &sh.full[sl]);
         else bulk_load(dst, (const __nv_bfloat16*)a.kc + page * a.k_stride + (long long)h * HD * BS, page_bytes, &sh.full[sl]);
       }
       ++use;
+      if (++sl == SLOTS) { sl = 0; ++round; }
     };
     for (int t = t0; t < t1 && ok; ++seg) {
       Segment s;
@@ -529,38 +566,41 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
       }
       t += s.n;
     }
-    ++use;
-    if (have && ok) put(vn, vp, vh, true);
-    // before the block ends, nothing is on its way into its memory any more (also when it gave up)
-#pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
+    if (have && ok) {                                               // the use behind the last K is left out
+      ++use;
+      if (++sl == SLOTS) { sl = 0; ++round; }
+      put(vn, vp, vh, true);
+    }
+    // before the block ends, nothing is on its way into its memory any more (also when it gave up): the last use of every slot
+    const uint32_t left_out = have && use > 0 ? use - 2 : ~0u;
+    for (uint32_t u = use > SLOTS + 2 ? use - SLOTS - 2 : 0; u < use; ++u) {
+      if (u == left_out || (u + SLOTS < use && u + SLOTS != left_out)) continue;
       const unsigned long long w0 = now_ns();
-      while (filled[i] && !bar_try(&sh.full[i], (filled[i] - 1) & 1) && now_ns() - w0 < WAIT_NS) {}
+      while (!bar_try(&sh.full[u % SLOTS], (u / SLOTS) & 1) && now_ns() - w0 < WAIT_NS) {}
     }
   } else if (warp == W_QK) {
     // ---- S = Q K^T: one thread, and another one for O += P V, so that neither waits behind what the other waits for
     if (elect()) {
       const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(ROWS >> 4) << 24);
-      uint32_t n = 0, seg = 0;
+      uint32_t n = 0, seg = 0, sl = 0, round = 0;                     // (K of tile n is use 2 n - 1, but 0 for the first)
       bool ok = true;
       for (int t = t0; t < t1 && ok; ++seg) {
         Segment s;
         ok = next_segment(seg, s);
         ok = ok && bar_wait(&sh.q_full[seg & 3], seg >> 2, stop);
         // (a sequence's own rows lie close together: what the other rows of the instruction read there reaches accumulator rows that nobody reads)
-        const uint32_t qrows = s.own ? OWN_ROWS : ROWS;
+        const uint32_t qrows = s.own ? OWN_ROWS : P.y.qrows;
         const uint64_t ad = desc(smem_u32(qbuf + (s.own ? (seg & 3) * (OWN_ROWS * (uint32_t)HD * 2) : 0u)), qrows * 16, 128, 0), astep = 2 * qrows;
         for (int i = 0; i < s.n && ok; ++i, ++n) {
           const int np = min(PAGES, (s.len + BS - 1) / BS - (s.tile0 + i) * PAGES);
-          const uint32_t use = n == 0 ? 0 : 2 * n - 1, sl = use % SLOTS;
           const uint32_t sb = n % 3;
           if (n >= 3) ok = bar_wait(&sh.pv_done[sb], n / 3 - 1, stop);               // (P of tile n - 3 lies where S of this one goes)
-          ok = ok && bar_wait(&sh.full[sl], use / SLOTS, stop);
+          ok = ok && bar_wait(&sh.full[sl], round, stop);
           if (!ok) break;
           fence_after();
           const uint32_t id = idesc | ((uint32_t)((np + 1) & ~1) << 17);             // N = 8 positions of each page, a multiple of 16
           const uint32_t d = tmem + sb * TP;
-          const uint64_t b0 = desc(smem_u32(base + sl * SLOT_BYTES), 256, page_bytes, 0);
+          const uint64_t b0 = desc(smem_u32(base + sl * slot_bytes), 256, page_bytes, 0);
 #pragma unroll 1
           for (int k = 0; k < HD / 16; ++k) {
             mma_ss(d, ad + k * astep, b0 + k * (512 >> 4), id, k);
@@ -569,6 +609,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
           mma_commit(&sh.s_full[sb]);
           mma_commit(&sh.empty[sl]);
           if (i == s.n - 1) mma_commit(&sh.q_free[seg & 3]);
+          sl += n == 0 ? 1 : 2;
+          if (sl >= SLOTS) { sl -= SLOTS; ++round; }
         }
         bar_arrive(&sh.seg_free[seg % SEGS]);
         t += s.n;
@@ -579,7 +621,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
     // ---- O += P V, behind the clearing of the values behind the unit's last position
     const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
     const uint64_t step = page_bytes >> 4;
-    uint32_t n = 0, seg = 0;
+    uint32_t n = 0, seg = 0, sl = 2, round = 0;      // (V of tile n is use 2 n + 2)
     bool ok = true;
     if (t0 < t1) ok = bar_wait(&sh.full[0], 0, stop);                 // (K0: the one use of slot 0 that is not V's; a wait for V1 would take it for its own)
     for (int t = t0; t < t1 && ok; ++seg) {
@@ -590,11 +632,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
       ok = __all_sync(~0u, ok);
       for (int i = 0; i < s.n && ok; ++i, ++n) {
         const int np = min(PAGES, (s.len + BS - 1) / BS - (s.tile0 + i) * PAGES);
-        const uint32_t use = 2 * n + 2, sl = use % SLOTS, sb = n % 3, pc = tmem + sb * TP;
-        ok = bar_wait(&sh.full[sl], use / SLOTS, stop);
+        const uint32_t sb = n % 3, pc = tmem + sb * TP;
+        ok = bar_wait(&sh.full[sl], round, stop);
         const int rem = s.len % BS, page = (s.len - 1) / BS - (s.tile0 + i) * PAGES;
         if (ok && rem && page < PAGES) {
-          unsigned char* v = base + sl * SLOT_BYTES + page * page_bytes;
+          unsigned char* v = base + sl * slot_bytes + page * page_bytes;
           for (int row = lane; row < HD; row += 32) {
             const int sw = (row >> 2) & 1;                            // a row's two 16-byte pieces change places in every other group of four rows
             for (int k = 0; k < 2; ++k) {
@@ -615,7 +657,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
         if (!ok) break;
         fence_after();
         if (elect()) {
-          const uint64_t b = desc(smem_u32(base + sl * SLOT_BYTES), 16, 256, 6);
+          const uint64_t b = desc(smem_u32(base + sl * slot_bytes), 16, 256, 6);
 #pragma unroll 1
           for (int k = 0; k < np; ++k) {
             mma_ts(d, pc + 8 * k, b + k * step, idesc, i + k);
@@ -623,9 +665,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
           }
           mma_commit(&sh.pv_done[sb]);
           mma_commit(&sh.empty[sl]);
-          if (i == s.n - 1) mma_commit(&sh.o_full);
+          if (i == s.n - 1) mma_commit(&sh.o_full[n & 1]);
         }
         __syncwarp();
+        sl += 2;
+        if (sl >= SLOTS) { sl -= SLOTS; ++round; }
       }
       if (lane == 0) bar_arrive(&sh.seg_free[seg % SEGS]);
       t += s.n;
@@ -646,7 +690,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
       ok = __all_sync(~0u, ok);
       if (!ok) break;
       own = s.own;
-      const int qrows = s.own ? OWN_ROWS : ROWS;
+      const int qrows = s.own ? OWN_ROWS : P.y.qrows;
       const uint32_t dst = smem_u32(qbuf + (s.own ? (seg & 3) * (OWN_ROWS * (uint32_t)HD * 2) : 0u));
       int sq = qr / P.y.G, j = qr - sq * P.y.G;                       // a lane has piece qc of every qn-th row
       for (int row = qr; row < s.rows; row += qn) {
@@ -671,87 +715,92 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------------------ joining the segments
-// A block has the G rows of one sequence and kv head: it adds the parts of the prefix's unit and of the sequence's own one, each weighted with 2^(m - M).
+// A warp has one row: it adds the parts of the prefix's unit and of the sequence's own one, each weighted with 2^(m - M).  Lanes have parts where the weights
+// are worked out and four (eight above 128) elements of the output where the parts are added; the order of the sums depends on nothing but the shares.
+// What it takes is three trips to L2 behind one another (which workers, their maxima and sums, their results), so each asks for all it can at once.
 constexpr int JOIN_THREADS = 128, MAX_WORKERS = 256;
-__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ Params P) {
-  __shared__ float f[2 * MAX_WORKERS][16], sum[16];                 // weight of a part in a row
-  __shared__ int s_bad;
-  const etxb_attn_shared_args& a = P.a;
-  const int tid = threadIdx.x, HD = a.HD, G = P.y.G, W = P.y.workers, h = blockIdx.x, b = blockIdx.y;
-  int lo = 0, hi = a.groups - 1;                                    // the group of b: the last that begins at or before it
-  while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (P.groups.first[mid] <= b) lo = mid; else hi = mid - 1; }
-  const int g = lo, first = P.groups.first[g], mt = units_of(P, g), um = (b - first) / P.y.spt;
-  int bad = 0;
-  if (bad_length(a.prefix_lens[g], a.prefix_width) || bad_length(a.lens[b], a.table_width)) bad = ETXB_SHARED_BAD_LENGTH;
-  if (tid == 0) s_bad = 0;
-  const int unit[2] = {prefix_unit(P, g) + h * mt + um, P.y.punits + b * a.NKV + h};
-  const long long slot[2] = {unit[0], (long long)b * a.NKV + h};      // of worker 0
-  const int stride[2] = {P.y.prows, G}, row[2] = {(b - first - um * P.y.spt) * G, 0};
-  const bool has[2] = {!bad && a.prefix_lens[g] > 0, !bad && a.lens[b] > 0};
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  int w0[2], n[2], lost = 0;
-  for (int w = tid; w < W; w += JOIN_THREADS) lost |= __ldcg(P.y.gave_up + w);
+struct JoinParams {                           // (of its own: the first read of every line of a kernel's parameters is a trip to memory)
+  const int32_t* prefix_lens; const int32_t* lens; const int32_t* of; const int32_t* gave_up; const int32_t* hdr;
+  const float* pO; const float* oO; const float* pml; const float* oml;
+  void* out; int32_t* status;
+  long long out_stride, pslots;
+  int seqs, NH, NKV, HD, G, spt, groups, prows, punits, workers, prefix_max, own_max;          // (positions that the tables have room for)
+  Groups first;
+};
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ JoinParams P) {
+  const int lane = threadIdx.x & 31, id = blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5);
+  if (id >= P.seqs * P.NH) return;
+  const int HD = P.HD, G = P.G, b = id / P.NH, head = id - b * P.NH, h = head / G, j = head - h * G;
+  int g = 0, hi = P.groups - 1;                                     // the group of b: the last that begins at or before it
+  while (g < hi) { const int mid = (g + hi + 1) >> 1; if (P.first.first[mid] <= b) g = mid; else hi = mid - 1; }
+  const int first = P.first.first[g], um = (b - first) / P.spt, mt = (P.first.first[g + 1] - first + P.spt - 1) / P.spt;
+  const int pu = (first / P.spt + g) * P.NKV + h * mt + um, ou = b * P.NKV + h;                 // (see prefix_unit)
+  const int prow = (b - first - um * P.spt) * G + j;
+  const int pl = __ldg(P.prefix_lens + g), ol = __ldg(P.lens + b);
+  int2 po = __ldcg((const int2*)P.of + pu), oo = __ldcg((const int2*)P.of + P.punits + ou);
+  int lost = 0;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int2 of = has[k] ? __ldcg((const int2*)P.y.of + unit[k]) : make_int2(0, -1);
-    w0[k] = of.x; n[k] = of.y - of.x + 1;
+  for (int w = 0; w < MAX_WORKERS; w += 32) if (w + lane < P.workers) lost |= __ldcg(P.gave_up + w + lane);
+  int bad = pl < 0 || pl > P.prefix_max || ol < 0 || ol > P.own_max ? ETXB_SHARED_BAD_LENGTH : 0;
+  if (__any_sync(~0u, lost)) bad |= ETXB_SHARED_GAVE_UP;            // (something is unwritten: nothing is looked at)
+  const int n0 = bad || pl <= 0 ? 0 : po.y - po.x + 1, n = n0 + (bad || ol <= 0 ? 0 : oo.y - oo.x + 1);
+  // part i: the prefix's from worker po.x on, then the own ones
+  const int64_t ps = (int64_t)pu + po.x, os = (int64_t)ou + oo.x;
+  auto sums = [&](int i) {
+    return __ldcg(i < n0 ? (const float2*)P.pml + (ps + i) * P.prows + prow : (const float2*)P.oml + (os + i - n0) * G + j);
+  };
+  float M = -INFINITY, L = 0.f;
+  float2 mine = make_float2(-INFINITY, 0.f);
+  for (int i = lane; i < n; i += 32) {
+    const float2 s = sums(i);
+    bad |= __ldcg(P.hdr + (i < n0 ? ps + i : P.pslots + os + i - n0));
+    M = fmaxf(M, s.x);
+    if (i < 32) mine = s;
   }
-  if (__syncthreads_or(lost)) { bad |= ETXB_SHARED_GAVE_UP; n[0] = n[1] = 0; }     // (a worker that gave up left something unwritten: nothing is looked at)
-  const int parts = n[0] + n[1];
-  for (int i = tid; i < parts; i += JOIN_THREADS) {
-    const int k = i >= n[0], w = w0[k] + i - (k ? n[0] : 0);
-    bad |= __ldcg(P.y.hdr + (k ? P.y.pslots : 0) + slot[k] + w);
-  }
-  if (bad) atomicOr(&s_bad, bad);
-  for (int j = tid >> 5; j < G; j += JOIN_THREADS / 32) {           // a warp has a row
-    const int lane = tid & 31;
-    float M = -INFINITY, L = 0.f;
-    for (int pass = 0; pass < 2; ++pass) {
-      for (int i = lane; i < parts; i += 32) {
-        const int k = i >= n[0], w = w0[k] + i - (k ? n[0] : 0);
-        const float2 ml = __ldcg((const float2*)(k ? P.y.oml : P.y.pml) + (slot[k] + w) * stride[k] + row[k] + j);
-        if (pass == 0) M = fmaxf(M, ml.x);
-        else {
-          // (a part with nothing but scores of minus infinity has no weight; one that is NaN goes on)
-          const float x = ml.y == 0.f ? 0.f : ml.x == M ? 1.f : ex2(ml.x - M);
-          f[i][j] = x;
-          if (ml.y != 0.f) L = __fmaf_rn(ml.y, x, L);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) { M = fmaxf(M, __shfl_xor_sync(~0u, M, o)); bad |= __shfl_xor_sync(~0u, bad, o); }
+  const int pieces = HD / 4;
+  float4 y[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    if (i0 > 0) mine = i0 + lane < n ? sums(i0 + lane) : make_float2(-INFINITY, 0.f);
+    // (a part with nothing but scores of minus infinity has no weight; one that is NaN goes on)
+    const float w = mine.y == 0.f ? 0.f : mine.x == M ? 1.f : ex2(mine.x - M);
+    if (mine.y != 0.f) L = __fmaf_rn(mine.y, w, L);
+    const int left = min(32, n - i0);
+#pragma unroll 1
+    for (int c = 0; c * 32 < pieces; ++c) {
+      const int piece = min(c * 32 + lane, pieces - 1);
+#pragma unroll 1
+      for (int i1 = 0; i1 < left; i1 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int i = i0 + min(i1 + k, left - 1);
+          v[k] = __ldcg(i < n0 ? (const float4*)P.pO + ((ps + i) * pieces + piece) * P.prows + prow : (const float4*)P.oO + ((os + i - n0) * pieces + piece) * G + j);
         }
-      }
-      if (pass == 0)
-        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
-    }
-    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
-    if (lane == 0) sum[j] = L;
-  }
-  __syncthreads();
-  bad = s_bad;
-  if (bad && a.status && tid == 0) atomicOr(a.status, bad);
-  for (int x = tid; x < G * HD / 4; x += JOIN_THREADS) {            // four output elements of a row
-    const int j = x % G, c = x / G;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float4* O = (const float4*)(k ? P.y.oO : P.y.pO) + (slot[k] + w0[k]) * stride[k] * (HD / 4) + (size_t)c * stride[k] + row[k] + j;
-      const size_t step = (size_t)stride[k] * (HD / 4);
-      const int at = k ? n[0] : 0;
-      for (int i0 = 0; i0 < n[k]; i0 += 8) {                        // (eight loads in flight)
-        float4 o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = __ldcg(O + min(i0 + i, n[k] - 1) * step);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float w = i0 + i < n[k] ? f[at + i0 + i][j] : 0.f;
-          if (w != 0.f) { y.x = __fmaf_rn(o[i].x, w, y.x); y.y = __fmaf_rn(o[i].y, w, y.y); y.z = __fmaf_rn(o[i].z, w, y.z); y.w = __fmaf_rn(o[i].w, w, y.w); }
+        for (int k = 0; k < 8; ++k) {
+          const float wi = __shfl_sync(~0u, w, (i1 + k) & 31);
+          if (i1 + k < left && wi != 0.f) {
+            float4& z = c ? y[1] : y[0];
+            z.x = __fmaf_rn(v[k].x, wi, z.x); z.y = __fmaf_rn(v[k].y, wi, z.y); z.z = __fmaf_rn(v[k].z, wi, z.z); z.w = __fmaf_rn(v[k].w, wi, z.w);
+          }
         }
       }
     }
-    const float L = sum[j];
-    const float z[4] = {y.x / L, y.y / L, y.z / L, y.w / L};
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
+  if (bad && P.status && lane == 0) atomicOr(P.status, bad);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    if (c * 32 + lane >= pieces) break;
+    const float z[4] = {y[c].x / L, y[c].y / L, y[c].z / L, y[c].w / L};
     __nv_bfloat162 out[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) out[e] = __floats2bfloat162_rn(bad ? NAN : L == 0.f ? 0.f : z[2 * e], bad ? NAN : L == 0.f ? 0.f : z[2 * e + 1]);
-    *(uint2*)((__nv_bfloat16*)a.out + b * a.out_stride + (long long)(h * G + j) * HD + 4 * c) = *(const uint2*)out;
+    *(uint2*)((__nv_bfloat16*)P.out + b * P.out_stride + (int64_t)head * HD + 4 * (c * 32 + lane)) = *(const uint2*)out;
   }
 }
 
@@ -875,23 +924,27 @@ extern "C" int32_t etxb_attn_shared(int device, const etxb_attn_shared_args* arg
   const CUresult r = encode(&P.vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)a.vc, dim, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return refuse(ETXB_E_CUDA, "cuTensorMapEncodeTiled failed for the values");
-  // six tiles in the ring where they fit beside the counts of up to 300 groups and sequences, else four.  (Four where six would do: prefixes of 32500
-  // positions for 64 sequences, @@; the ring is then empty when a product's operands are asked for.)
-  const int count = (a.groups + a.seqs + 1) * 8, limit = 232448 - 3328;
-  const bool six = a.HD <= 128 && fixed_bytes(a.HD, 6) + count <= limit;
-  const void* k = a.HD > 128 ? (const void*)tiles_kernel<64, 4> : six ? (const void*)tiles_kernel<128, 6> : (const void*)tiles_kernel<128, 4>;
-  const int smem = fixed_bytes(a.HD, six ? 6 : 4) + count;
+  const void* k = a.HD > 128 ? (const void*)tiles_kernel<64> : (const void*)tiles_kernel<128>;
+  P.y.qrows = P.y.prows <= OWN_ROWS ? OWN_ROWS : (P.y.prows + 7) & ~7;
+  const int slot = P.y.tp * a.HD * 2, other = 256 + q_size(a.HD, P.y.qrows) + (a.groups + a.seqs + 1) * 8 + 2048;
+  const int slots = (232448 - (int)sizeof(Shared) - 1024 - other) / slot & ~1;
+  P.y.slots = slots > MAX_SLOTS ? MAX_SLOTS : slots;                // (four at least: 128 rows of Q and 1024 sequences leave 130 KB)
+  const int smem = other + P.y.slots * slot;
   ETXB_HOST_CU(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = dim3((unsigned)P.y.workers); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = (size_t)smem; cfg.stream = (cudaStream_t)cuda_stream;
   void* kargs[] = {(void*)&P};
   ETXB_HOST_CU(cudaLaunchKernelExC(&cfg, k, kargs));
-  cfg.gridDim = dim3((unsigned)a.NKV, (unsigned)a.seqs); cfg.blockDim = dim3(JOIN_THREADS); cfg.dynamicSmemBytes = 0;
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at; cfg.numAttrs = 1;
-  ETXB_HOST_CU(cudaLaunchKernelExC(&cfg, (const void*)join_kernel, kargs));
+  static thread_local JoinParams J;
+  const Layout& y = P.y;
+  J.prefix_lens = a.prefix_lens; J.lens = a.lens; J.of = y.of; J.gave_up = y.gave_up; J.hdr = y.hdr;
+  J.pO = y.pO; J.oO = y.oO; J.pml = y.pml; J.oml = y.oml; J.out = a.out; J.status = a.status; J.out_stride = a.out_stride; J.pslots = y.pslots;
+  J.seqs = a.seqs; J.NH = a.NH; J.NKV = a.NKV; J.HD = a.HD; J.G = y.G; J.spt = y.spt; J.groups = a.groups; J.prows = y.prows; J.punits = y.punits; J.workers = y.workers;
+  J.prefix_max = a.prefix_width * BS; J.own_max = a.table_width * BS;
+  J.first = P.groups;
+  cfg.gridDim = dim3((unsigned)((a.seqs * a.NH + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32))); cfg.blockDim = dim3(JOIN_THREADS); cfg.dynamicSmemBytes = 0;
+  void* jargs[] = {(void*)&J};
+  ETXB_HOST_CU(cudaLaunchKernelExC(&cfg, (const void*)join_kernel, jargs));
   return ETXB_OK;
 }

@@ -7,8 +7,16 @@
 //   min-p   those with w_r >= min_p
 // so together they keep the first n (at least one).  Drawn is the first token whose inclusive sum exceeds u * W_n.
 //
-// The sums have to be right next to every border, and the order of atomics must not change them: weights are integers, exp in 64 bits times 2^S with
-// S = 62 - ceil(log2 V), so a row's sum fits 63 bits, is exact, and a weight is off by 2^-(S+1) <= 2^-43 of the largest.
+// The sums have to be right next to every border, and the order of atomics must not change them.
+//
+// Logits of 16 bits (counts_kernel).  A row has at most 65536 different values, and a real one some thousands: the row is counted value by value, exactly, with
+// 16-bit counters in shared memory, and then one exp in 64 bits per value that occurs, and sums over values in their order, give all three cuts and the
+// draw.  Nothing is sorted.  A row belongs to a cluster of C blocks, each of which counts a part of it; values are joined through distributed shared
+// memory, 32 neighbouring ones (a group) at a time, and only groups that occur.
+// Logits of 32 bits (sums_kernel).  Bins by the first 11 bits of the value, then the next 11 and the last 10 of one bin: three passes for a border.  A bin has a
+// number of tokens and a sum of weights, which are integers: exp in 64 bits times 2^S with S = 62 - ceil(log2 V), so that a row's sum fits 63 bits, is
+// exact whatever the order, and a weight is off by 2^-(S+1) <= 2^-43 of the largest.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdio.h>
@@ -17,9 +25,371 @@
 #include "etxb_host.h"
 
 namespace etxb_draw {
+namespace cg = cooperative_groups;
 
-constexpr int THREADS = 1024, WARPS = THREADS / 32, BINS = 2048;
+constexpr int THREADS = 1024, WARPS = THREADS / 32, MAX_CLUSTER = 8;
 
+// A row's settings, in the form the kernels use.
+struct Settings {
+  float T, top_p, min_p;
+  int k;
+  double u;
+};
+__device__ __forceinline__ Settings settings(const etxb_sample_args& a, int row) {
+  Settings s;
+  s.T = a.temperature ? a.temperature[row] : a.temperature_all;
+  s.k = a.top_k ? a.top_k[row] : a.top_k_all;
+  s.top_p = a.top_p ? a.top_p[row] : a.top_p_all;
+  s.min_p = a.min_p ? a.min_p[row] : a.min_p_all;
+  const float u = a.u[row];
+  s.u = u > 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
+  return s;
+}
+__device__ __forceinline__ void store(const etxb_sample_args& a, int row, int token, float logp, int kept) {
+  a.tokens[row] = token;
+  if (a.next) a.next[row] = token;
+  if (a.logprobs) a.logprobs[row] = logp;
+  if (a.kept) a.kept[row] = kept;
+}
+
+// What a lookup asks for: the token of a rank; the last token with less than `x` before it; the first with more than `x` up to it.
+enum { BY_RANK, BY_MASS_BEFORE, BY_MASS_UPTO };
+template <typename M>
+__device__ __forceinline__ bool falls(int how, uint32_t rank, double x, uint32_t c0, uint32_t c, M m0, M m1) {
+  if (how == BY_RANK) return c0 <= rank && rank < c0 + c;
+  if (how == BY_MASS_BEFORE) return c > 0u && (double)m0 < x && (double)m1 >= x;
+  return (double)m0 <= x && (double)m1 > x;
+}
+
+// ================================================================================================ logits of 16 bits
+// Keys: values as unsigned numbers in the values' order; 0 for -inf and NaN; -0 is +0.  INF: the key of +inf (bf16 0x7f80, fp16 0x7c00).
+template <uint32_t INF>
+struct Key16 {
+  static constexpr uint32_t LOWEST = (uint32_t)(0xffffu - (INF - 1u + 0x8000u)) & 0xffffu;         // the key of the type's lowest number
+  static __device__ __forceinline__ uint32_t of(uint32_t u) {                                       // u: 16 bits
+    uint32_t k = (u & 0x8000u) ? (~u & 0xffffu) : (u | 0x8000u);
+    if (k == 0x7fffu) k = 0x8000u;
+    return k - LOWEST <= INF + 0x8000u - LOWEST ? k : 0u;
+  }
+};
+template <typename T> __device__ __forceinline__ float value16(uint32_t key);
+template <> __device__ __forceinline__ float value16<__nv_bfloat16>(uint32_t key) {
+  return __uint_as_float(((key & 0x8000u) ? (key & 0x7fffu) : (~key & 0xffffu)) << 16);
+}
+template <> __device__ __forceinline__ float value16<__half>(uint32_t key) {
+  return __half2float(__ushort_as_half((unsigned short)((key & 0x8000u) ? (key & 0x7fffu) : (~key & 0xffffu))));
+}
+
+constexpr int GROUPS = 2048, CHUNK = 8191;                          // groups of 32 values; vectors of 8 logits a block counts (16 bits hold their number)
+struct Counts {
+  uint32_t hist[32768];                                             // two counters a word
+  double mass[GROUPS], mass_min[GROUPS];                            // of the groups this block joins (a C-th of them): sum of weights, and of those min-p keeps
+  uint32_t count[GROUPS], count_min[GROUPS];
+  uint16_t list[GROUPS];                                            // of these, the ones that occur
+  uint32_t bits[GROUPS / 32];                                       // the groups that occur in this block's part
+  uint32_t wc[WARPS], wcm[WARPS];
+  double wm[WARPS], wmm[WARPS];
+  uint32_t maxkey, n_list;
+  uint32_t hit_group, hit_count, place_key, place_before, place_count;
+  double hit_mass, place_mass, place_weight;
+  int found;
+  uint32_t entry, entry_before;
+};
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_args a) {
+  using K = Key16<sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Counts& s = *(Counts*)smem;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), r = (int)cluster.block_rank(), row = blockIdx.x / C;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
+  const Settings st = settings(a, row);
+  const bool greedy = !(st.T > 0.f);
+
+  // this block's vectors of 8 logits, from the last 16-byte boundary before the row on: logit v * 8 - shift + j
+  const T* l = (const T*)a.logits + (long long)row * a.row_stride;
+  const int shift = (int)((uintptr_t)l & 15) / 2, nvec = (shift + V + 7) / 8;
+  const int v0 = (int)((long long)nvec * r / C), v1 = (int)((long long)nvec * (r + 1) / C);
+  uint4 key[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = v0 + i * THREADS + tid;
+    key[i] = make_uint4(0u, 0u, 0u, 0u);
+    const int e = v * 8 - shift;
+    if (v < v1 && e >= 0 && e + 8 <= V) key[i] = __ldg((const uint4*)(l + e));
+    else if (v < v1) {                                              // the row's ends, one by one (0xffff is no number)
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int x = e + 2 * j;
+        const uint32_t lo = x >= 0 && x < V ? ((const unsigned short*)l)[x] : 0xffffu, hi = x + 1 >= 0 && x + 1 < V ? ((const unsigned short*)l)[x + 1] : 0xffffu;
+        w[j] = lo | (hi << 16);
+      }
+      key[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    } else key[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+  }
+  if (!greedy)
+    for (int i = tid; i < 32768 / 4; i += THREADS) ((uint4*)s.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+  for (int i = tid; i < GROUPS / C; i += THREADS) { s.mass[i] = 0.0; s.mass_min[i] = 0.0; s.count[i] = 0u; s.count_min[i] = 0u; }
+  if (tid == 0) { s.maxkey = 0u; s.n_list = 0u; }
+  __syncthreads();
+  uint32_t mx = 0u, low = 0u;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    uint32_t* w = (uint32_t*)&key[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t k0 = K::of(w[j] & 0xffffu), k1 = K::of(w[j] >> 16);
+      w[j] = k0 | (k1 << 16);
+      mx = max(mx, max(k0, k1));
+      if (!greedy) {
+        // (a mask of the type's lowest number makes most of a row equal: those are counted without memory)
+        if (k0 == K::LOWEST) ++low; else if (k0) atomicAdd(&s.hist[k0 >> 1], 1u << ((k0 & 1u) * 16u));
+        if (k1 == K::LOWEST) ++low; else if (k1) atomicAdd(&s.hist[k1 >> 1], 1u << ((k1 & 1u) * 16u));
+      }
+    }
+  }
+  mx = __reduce_max_sync(~0u, mx); low = __reduce_add_sync(~0u, low);
+  if (lane == 0) { atomicMax(&s.maxkey, mx); if (low) atomicAdd(&s.hist[K::LOWEST >> 1], low << ((K::LOWEST & 1u) * 16u)); }
+  __syncthreads();
+  if (!greedy) {
+    // groups that occur: four lanes look at the 64 bytes of one
+    for (int i = 0; i < GROUPS * 4 / THREADS; ++i) {
+      const uint4 q = ((const uint4*)s.hist)[i * THREADS + tid];
+      uint32_t any = q.x | q.y | q.z | q.w;
+      any |= __shfl_xor_sync(~0u, any, 1); any |= __shfl_xor_sync(~0u, any, 2);
+      uint32_t b = __ballot_sync(~0u, any != 0u);                   // 8 groups, a nibble each
+      if (lane == 0) {
+        b &= 0x11111111u;
+        b = (b | b >> 3) & 0x03030303u; b = (b | b >> 6) & 0x000f000fu; b = (b | b >> 12) & 0xffu;
+        ((unsigned char*)s.bits)[i * (THREADS / 32) + warp] = (unsigned char)b;
+      }
+    }
+  }
+  cluster.sync();
+  uint32_t maxkey = 0u;
+  int first_with_max = 0;
+  for (int c = C - 1; c >= 0; --c) {
+    const uint32_t m = *cluster.map_shared_rank(&s.maxkey, c);
+    if (m >= maxkey) { maxkey = m; first_with_max = c; }
+  }
+  if (maxkey == 0u) {                                               // nothing is allowed
+    if (r == 0 && tid == 0) store(a, row, -1, -INFINITY, 0);
+    cluster.sync();
+    return;
+  }
+  const double dmax = (double)value16<T>(maxkey), inv_t = 1.0 / (double)st.T;
+  auto log_weight = [&](uint32_t k) { const double d = (double)value16<T>(k) - dmax; return d == d ? d * inv_t : 0.0; };      // (inf - inf: the largest itself)
+  auto weight = [&](uint32_t k) { const double d = (double)value16<T>(k) - dmax; return d < 0.0 ? (d == -INFINITY ? 0.0 : exp(d * inv_t)) : 1.0; };
+  // tokens of value k in the whole row
+  auto tokens_of = [&](uint32_t k) {
+    uint32_t n = 0u;
+    for (int c = 0; c < C; ++c) n += ((const uint16_t*)cluster.map_shared_rank(&s.hist[0], c))[k];
+    return n;
+  };
+
+  uint32_t nth = 0u, at = maxkey;                                   // the drawn token: the nth one, by index, of the value `at`
+  int kept = 1;
+  float logp = 0.f;
+  if (!greedy) {
+    // this block joins the groups [g0, g0 + GROUPS / C): the list of those that occur, then a warp a group
+    const int per = GROUPS / C, g0 = r * per;
+    if (tid < per / 32) {
+      uint32_t b = 0u;
+      for (int c = 0; c < C; ++c) b |= cluster.map_shared_rank(&s.bits[0], c)[g0 / 32 + tid];
+      uint32_t n = atomicAdd(&s.n_list, (uint32_t)__popc(b));
+      for (; b; b &= b - 1u) s.list[n++] = (uint16_t)(tid * 32 + __ffs(b) - 1);
+    }
+    __syncthreads();
+    for (uint32_t i = warp; i < s.n_list; i += WARPS) {
+      const uint32_t g = s.list[i], k = (uint32_t)(g0 + g) * 32u + 31u - (uint32_t)lane;           // lanes from the group's largest value down
+      const uint32_t n = tokens_of(k);
+      const double w = n ? weight(k) : 0.0;
+      const bool in = n && w >= (double)st.min_p;
+      double m = (double)n * w, mm = in ? m : 0.0;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) { m += __shfl_xor_sync(~0u, m, o); mm += __shfl_xor_sync(~0u, mm, o); }
+      const uint32_t c = __reduce_add_sync(~0u, n), cm = __reduce_add_sync(~0u, in ? n : 0u);
+      if (lane == 0) { s.mass[g] = m; s.mass_min[g] = mm; s.count[g] = c; s.count_min[g] = cm; }
+    }
+    cluster.sync();
+    // every block goes over all groups in descending order, two a thread: tokens and mass before each
+    uint32_t gc[2], gb, cm = 0u, total = 0u, total_min = 0u;
+    double gm[2], mb, mm = 0.0, total_m = 0.0, total_mm = 0.0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int g = GROUPS - 1 - (2 * tid + k), c = g / per, x = g - c * per;
+      const Counts* o = cluster.map_shared_rank(&s, c);
+      gc[k] = o->count[x]; gm[k] = o->mass[x];
+      cm += o->count_min[x]; mm += o->mass_min[x];
+    }
+    gb = gc[0] + gc[1]; mb = gm[0] + gm[1];
+    const uint32_t own_c = gb;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(~0u, gb, o);
+      const double y = __shfl_up_sync(~0u, mb, o);
+      if (lane >= o) { gb += x; mb += y; }
+    }
+    cm = __reduce_add_sync(~0u, cm);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mm += __shfl_xor_sync(~0u, mm, o);
+    if (lane == 31) { s.wc[warp] = gb; s.wm[warp] = mb; s.wcm[warp] = cm; s.wmm[warp] = mm; }
+    __syncthreads();
+    double me;                                                      // mass up to and with this thread's groups
+    gb -= own_c;
+    {
+      const double before = __shfl_up_sync(~0u, mb, 1);
+      // the warps' sums in order: each lane one of them
+      uint32_t c = s.wc[lane];
+      double m = s.wm[lane], mmin = s.wmm[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(~0u, c, o);
+        const double y = __shfl_up_sync(~0u, m, o);
+        if (lane >= o) { c += x; m += y; }
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mmin += __shfl_xor_sync(~0u, mmin, o);
+      total = __shfl_sync(~0u, c, 31); total_m = __shfl_sync(~0u, m, 31); total_mm = mmin;
+      total_min = __reduce_add_sync(~0u, s.wcm[lane]);
+      const uint32_t cw = __shfl_sync(~0u, c, (warp + 31) & 31);
+      const double mw = __shfl_sync(~0u, m, (warp + 31) & 31), here = warp ? mw : 0.0, next = __shfl_sync(~0u, m, warp);
+      gb += warp ? cw : 0u;
+      me = lane < 31 ? mb + here : next;
+      mb = lane ? before + here : here;
+    }
+    // a border: the thread whose group it falls into names it, and a warp goes over the group's values
+    auto lookup = [&](int how, uint32_t rank, double x) {
+      __syncthreads();
+      if (tid == 0) s.found = 0;
+      __syncthreads();
+      uint32_t c0 = gb;
+      double m0 = mb;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const double m1 = k == 0 ? fmin(mb + gm[0], me) : me;       // (what a group ends with is, to the bit, what the next one begins with)
+        if (gc[k] && falls(how, rank, x, c0, gc[k], m0, m1)) { s.hit_group = (uint32_t)(GROUPS - 1 - (2 * tid + k)); s.hit_count = c0; s.hit_mass = m0; s.found = 1; }
+        c0 += gc[k]; m0 = m1;
+      }
+      __syncthreads();
+      if (s.found && warp == 0) {
+        const uint32_t k = s.hit_group * 32u + 31u - (uint32_t)lane, n = tokens_of(k);
+        const double w = n ? weight(k) : 0.0;
+        uint32_t c = n;
+        double m = (double)n * w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t x1 = __shfl_up_sync(~0u, c, o);
+          const double y1 = __shfl_up_sync(~0u, m, o);
+          if (lane >= o) { c += x1; m += y1; }
+        }
+        uint32_t cb = __shfl_up_sync(~0u, c, 1);
+        double mbef = __shfl_up_sync(~0u, m, 1);
+        if (lane == 0) { cb = 0u; mbef = 0.0; }
+        cb += s.hit_count;
+        const double m0 = s.hit_mass + mbef, m1 = s.hit_mass + m;
+        uint32_t hits = __ballot_sync(~0u, n && falls(how, rank, x, cb, n, m0, m1));
+        // (sums within a group are rounded apart from the group's: a border on its very end belongs to its last value)
+        if (!hits) { const uint32_t some = __ballot_sync(~0u, n != 0u); hits = 1u << (31 - __clz(some)); }
+        if (lane == __ffs(hits) - 1) { s.place_key = k; s.place_before = cb; s.place_count = n; s.place_mass = m0; s.place_weight = w; }
+      }
+      __syncthreads();
+      return s.found != 0;
+    };
+    uint32_t n = total;
+    double Wn = total_m;
+    if (st.k > 0 && (uint32_t)st.k < total) {
+      lookup(BY_RANK, (uint32_t)st.k - 1u, 0.0);
+      n = (uint32_t)st.k;
+      Wn = s.place_mass + (double)(n - s.place_before) * s.place_weight;
+    }
+    if (st.top_p < 1.f) {
+      const double x = (double)st.top_p * Wn;
+      uint32_t np = 1u;
+      double Wp = 1.0;
+      if (x > 0.0 && lookup(BY_MASS_BEFORE, 0u, x)) {
+        const double q = ceil((x - s.place_mass) / s.place_weight);
+        const uint32_t in = (uint32_t)fmin(fmax(q, 1.0), (double)s.place_count);
+        np = s.place_before + in; Wp = s.place_mass + (double)in * s.place_weight;
+      }
+      if (np < n) { n = np; Wn = Wp; }
+    }
+    if (st.min_p > 0.f && total_min < n) {
+      n = total_min ? total_min : 1u;
+      Wn = total_min ? total_mm : 1.0;
+    }
+    const double x = st.u * Wn;
+    const bool found = lookup(BY_MASS_UPTO, 0u, x);
+    if (found) nth = (uint32_t)fmin(fmax(floor((x - s.place_mass) / s.place_weight), 0.0), (double)(s.place_count - 1u));
+    if (!found || s.place_before + nth >= n) {                      // rounding next to the last border: the last token that is kept
+      lookup(BY_RANK, n - 1u, 0.0);
+      nth = n - 1u - s.place_before;
+    }
+    at = s.place_key;
+    logp = (float)(log_weight(at) - log(Wn));
+    kept = (int)n;
+  }
+  // which block has it: the tokens of that value in the blocks before
+  bool mine;
+  if (greedy) mine = r == first_with_max;
+  else {
+    uint32_t before = 0u, here = 0u;
+    for (int c = 0; c <= r; ++c) { before += here; here = ((const uint16_t*)cluster.map_shared_rank(&s.hist[0], c))[at]; }
+    mine = before <= nth && nth < before + here;
+    nth -= before;
+  }
+  if (mine) {
+    uint32_t* cnt = (uint32_t*)s.list;                              // matches by vector number and warp: the order of the indices
+    uint32_t match[NV];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t* w = (const uint32_t*)&key[i];
+      match[i] = 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) match[i] |= ((w[j] & 0xffffu) == at ? 1u << (2 * j) : 0u) | ((w[j] >> 16) == at ? 2u << (2 * j) : 0u);
+      const uint32_t c = __reduce_add_sync(~0u, (uint32_t)__popc(match[i]));
+      if (lane == 0) cnt[i * WARPS + warp] = c;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      uint32_t c = 0u;
+#pragma unroll
+      for (int q = 0; q < NV; ++q) c += cnt[lane * NV + q];
+      uint32_t before = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(~0u, before, o); if (lane >= o) before += x; }
+      before -= c;
+      if (before <= nth && nth < before + c) {
+        int q = 0;
+        while (before + cnt[lane * NV + q] <= nth) before += cnt[lane * NV + q++];
+        s.entry = (uint32_t)(lane * NV + q); s.entry_before = before;
+      }
+    }
+    __syncthreads();
+    if ((int)(s.entry & (WARPS - 1)) == warp) {
+      const int i = (int)(s.entry / WARPS);
+      uint32_t m = 0u;
+#pragma unroll
+      for (int q = 0; q < NV; ++q) if (q == i) m = match[q];
+      const uint32_t c = (uint32_t)__popc(m), want = nth - s.entry_before;
+      uint32_t before = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(~0u, before, o); if (lane >= o) before += x; }
+      before -= c;
+      if (before <= want && want < before + c) {
+        for (uint32_t q = before; q < want; ++q) m &= m - 1u;
+        store(a, row, (v0 + i * THREADS + tid) * 8 - shift + __ffs(m) - 1, logp, kept);
+      }
+    }
+  }
+  cluster.sync();                                                   // (no block leaves while another one reads its counters)
+}
+
+// ================================================================================================ logits of 32 bits
+constexpr int BINS = 2048;
 // Logits as keys whose order as unsigned numbers is the order of the values; 0: not live (-inf, NaN).  -0 counts as +0.
 __device__ __forceinline__ uint32_t key_of(float l) {
   uint32_t u = __float_as_uint(l);
@@ -76,7 +446,7 @@ __device__ __forceinline__ double log_weight(const Row& r, uint32_t key) {
 }
 __device__ __forceinline__ double real_weight(const Row& r, uint32_t key) {
   const double d = (double)value_of(key) - r.max;
-  return d < 0.0 ? exp(d * r.inv_t) : 1.0;
+  return d < 0.0 ? (d == -INFINITY ? 0.0 : exp(d * r.inv_t)) : 1.0;     // (beside an infinite logit a finite one has none, at any temperature)
 }
 __device__ __forceinline__ unsigned long long weight(const Row& r, uint32_t key) { return __double2ull_rn(real_weight(r, key) * r.scale); }
 __device__ __forceinline__ void add(Bins& b, uint32_t i, unsigned long long w) {
@@ -88,8 +458,6 @@ __device__ __forceinline__ void add(Bins& b, uint32_t i, unsigned long long w) {
 }
 __device__ __forceinline__ unsigned long long mass(const Bins& b, int i) { return ((unsigned long long)b.hi[i] << 32) | b.lo[i]; }
 
-// What a lookup asks for: the token of a rank; the last token with less than `x` before it; the first with more than `x` up to it.
-enum { BY_RANK, BY_MASS_BEFORE, BY_MASS_UPTO };
 struct Place {
   uint32_t key, before_count, count;          // a value, the tokens before its first one, its tokens
   unsigned long long before_mass;
@@ -114,11 +482,7 @@ __device__ bool find_bin(Shared& s, const Bins& b, int nbins, int how, uint32_t 
   cb += c0; mb += m0;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    bool hit;
-    if (how == BY_RANK) hit = cb <= rank && rank < cb + c[k];
-    else if (how == BY_MASS_BEFORE) hit = c[k] && (double)mb < x && (double)(mb + m[k]) >= x;
-    else hit = (double)mb <= x && (double)(mb + m[k]) > x;
-    if (hit) { s.bin = (uint32_t)(nbins - 1 - (2 * t + k)); s.before_count = cb; s.before_mass = mb; s.count = c[k]; }
+    if (falls(how, rank, x, cb, c[k], mb, mb + m[k])) { s.bin = (uint32_t)(nbins - 1 - (2 * t + k)); s.before_count = cb; s.before_mass = mb; s.count = c[k]; }
     cb += c[k]; mb += m[k];
   }
   __syncthreads();
@@ -278,9 +642,36 @@ extern "C" int32_t etxb_sample(int device, const etxb_sample_args* args, size_t 
       (uintptr_t)a.top_k | (uintptr_t)a.top_p | (uintptr_t)a.min_p) & 3)) return etxb_host_fail(ETXB_E_ARG, "sample: a pointer is not aligned to its elements");
   EtxbDeviceScope scope(device);
   ETXB_HOST_CU(scope.err);
-  const void* k = a.dtype == ETXB_F32 ? (const void*)rows_kernel<float> : a.dtype == ETXB_F16 ? (const void*)rows_kernel<__half> : (const void*)rows_kernel<__nv_bfloat16>;
-  ETXB_HOST_CU(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
+  int sms = 0;
+  ETXB_HOST_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
   void* kargs[] = {(void*)&a};
-  ETXB_HOST_CU(cudaLaunchKernel(k, dim3((unsigned)a.rows), dim3(THREADS), kargs, sizeof(Shared), (cudaStream_t)cuda_stream));
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof cfg);
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  cfg.blockDim = dim3(THREADS); cfg.stream = (cudaStream_t)cuda_stream; cfg.attrs = &at; cfg.numAttrs = 1;
+  // blocks of a row: as many as its counters need, and more while the device has room and each block still has 8192 logits
+  int C = 1;
+  const long long vectors = ((long long)a.V + 7 + 7) / 8;
+  while ((vectors + C - 1) / C > CHUNK) C *= 2;
+  const void* k;
+  if (a.dtype == ETXB_F32 || C > MAX_CLUSTER) {
+    k = a.dtype == ETXB_F32 ? (const void*)rows_kernel<float> : a.dtype == ETXB_F16 ? (const void*)rows_kernel<__half> : (const void*)rows_kernel<__nv_bfloat16>;
+    C = 1;
+    cfg.dynamicSmemBytes = sizeof(Shared);
+  } else {
+    while (C < MAX_CLUSTER && (long long)a.rows * 2 * C <= sms && vectors / C > 1024) C *= 2;
+    const int nv = (int)((vectors + C - 1) / C + THREADS - 1) / THREADS;
+    const bool half = a.dtype == ETXB_F16;
+    k = nv <= 1 ? (half ? (const void*)counts_kernel<__half, 1> : (const void*)counts_kernel<__nv_bfloat16, 1>)
+      : nv <= 2 ? (half ? (const void*)counts_kernel<__half, 2> : (const void*)counts_kernel<__nv_bfloat16, 2>)
+      : nv <= 4 ? (half ? (const void*)counts_kernel<__half, 4> : (const void*)counts_kernel<__nv_bfloat16, 4>)
+                : (half ? (const void*)counts_kernel<__half, 8> : (const void*)counts_kernel<__nv_bfloat16, 8>);
+    cfg.dynamicSmemBytes = sizeof(Counts);
+  }
+  at.val.clusterDim.x = (unsigned)C; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(a.rows * C));
+  ETXB_HOST_CU(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes));
+  ETXB_HOST_CU(cudaLaunchKernelExC(&cfg, k, kargs));
   return ETXB_OK;
 }

@@ -81,20 +81,26 @@ template <> __device__ __forceinline__ float value16<__half>(uint32_t key) {
 }
 
 constexpr int GROUPS = 2048, CHUNK = 8191;                          // groups of 32 values; vectors of 8 logits a block counts (16 bits hold their number)
+struct Group {
+  double mass, mass_min;                                            // sum of the weights of its tokens, and of those that min-p keeps
+  uint32_t count, count_min;
+};
 struct Counts {
   uint32_t hist[32768];                                             // two counters a word
-  double mass[GROUPS], mass_min[GROUPS];                            // of the groups this block joins (a C-th of them): sum of weights, and of those min-p keeps
-  uint32_t count[GROUPS], count_min[GROUPS];
-  uint16_t list[GROUPS];                                            // of these, the ones that occur
+  Group group[GROUPS];                                              // of the whole row: each block joins a C-th of them and tells the others
+  double before_mass[GROUPS + 1];                                   // of the groups above (index: from the largest value down)
+  uint32_t before_count[GROUPS + 1];
+  uint16_t list[GROUPS];                                            // of the groups this block joins, the ones that occur
   uint32_t bits[GROUPS / 32];                                       // the groups that occur in this block's part
   uint32_t wc[WARPS], wcm[WARPS];
   double wm[WARPS], wmm[WARPS];
   uint32_t maxkey, n_list;
-  uint32_t hit_group, hit_count, place_key, place_before, place_count;
-  double hit_mass, place_mass, place_weight;
-  int found;
+  uint32_t at, nth, here;                                           // what was drawn: a value, and which of its tokens in this block
+  int kept, mine;
+  float logp;
   uint32_t entry, entry_before;
 };
+static_assert(sizeof(Counts) <= 231424, "a block's shared memory");
 
 template <typename T, int NV>
 __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_args a) {
@@ -131,7 +137,8 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
   }
   if (!greedy)
     for (int i = tid; i < 32768 / 4; i += THREADS) ((uint4*)s.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
-  for (int i = tid; i < GROUPS / C; i += THREADS) { s.mass[i] = 0.0; s.mass_min[i] = 0.0; s.count[i] = 0u; s.count_min[i] = 0u; }
+  if (!greedy)
+    for (int i = tid; i < (int)(sizeof s.group / 16); i += THREADS) ((uint4*)s.group)[i] = make_uint4(0u, 0u, 0u, 0u);
   if (tid == 0) { s.maxkey = 0u; s.n_list = 0u; }
   __syncthreads();
   uint32_t mx = 0u, low = 0u;
@@ -168,12 +175,17 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
     }
   }
   cluster.sync();
+  // one word from every block of the cluster, all on their way at once
+  auto from_all = [&](const void* mine, auto type, auto use) {
+    decltype(type) v[MAX_CLUSTER];
+#pragma unroll
+    for (int c = 0; c < MAX_CLUSTER; ++c) if (c < C) v[c] = *(const decltype(type)*)cluster.map_shared_rank((void*)mine, c);
+#pragma unroll
+    for (int c = 0; c < MAX_CLUSTER; ++c) if (c < C) use(c, v[c]);
+  };
   uint32_t maxkey = 0u;
   int first_with_max = 0;
-  for (int c = C - 1; c >= 0; --c) {
-    const uint32_t m = *cluster.map_shared_rank(&s.maxkey, c);
-    if (m >= maxkey) { maxkey = m; first_with_max = c; }
-  }
+  from_all(&s.maxkey, uint32_t(), [&](int c, uint32_t m) { if (m > maxkey) { maxkey = m; first_with_max = c; } });
   if (maxkey == 0u) {                                               // nothing is allowed
     if (r == 0 && tid == 0) store(a, row, -1, -INFINITY, 0);
     cluster.sync();
@@ -185,97 +197,90 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
   // tokens of value k in the whole row
   auto tokens_of = [&](uint32_t k) {
     uint32_t n = 0u;
-    for (int c = 0; c < C; ++c) n += ((const uint16_t*)cluster.map_shared_rank(&s.hist[0], c))[k];
+    from_all((const uint16_t*)s.hist + k, uint16_t(), [&](int, uint16_t x) { n += x; });
     return n;
   };
 
-  uint32_t nth = 0u, at = maxkey;                                   // the drawn token: the nth one, by index, of the value `at`
-  int kept = 1;
-  float logp = 0.f;
-  if (!greedy) {
-    // this block joins the groups [g0, g0 + GROUPS / C): the list of those that occur, then a warp a group
-    const int per = GROUPS / C, g0 = r * per;
-    if (tid < per / 32) {
+  if (greedy) {
+    if (tid == 0) { s.at = maxkey; s.nth = 0u; s.kept = 1; s.logp = 0.f; s.mine = r == first_with_max; }
+  } else {
+    // this block joins the groups g with g % C = r (the ones that occur lie close together): their list, then a warp a group
+    if (tid < GROUPS / 32) {
       uint32_t b = 0u;
-      for (int c = 0; c < C; ++c) b |= cluster.map_shared_rank(&s.bits[0], c)[g0 / 32 + tid];
-      uint32_t n = atomicAdd(&s.n_list, (uint32_t)__popc(b));
+      from_all(&s.bits[tid], uint32_t(), [&](int, uint32_t x) { b |= x; });
+      b &= (C == 1 ? ~0u : C == 2 ? 0x55555555u : C == 4 ? 0x11111111u : 0x01010101u) << r;
+      uint32_t n = b ? atomicAdd(&s.n_list, (uint32_t)__popc(b)) : 0u;
       for (; b; b &= b - 1u) s.list[n++] = (uint16_t)(tid * 32 + __ffs(b) - 1);
     }
     __syncthreads();
     for (uint32_t i = warp; i < s.n_list; i += WARPS) {
-      const uint32_t g = s.list[i], k = (uint32_t)(g0 + g) * 32u + 31u - (uint32_t)lane;           // lanes from the group's largest value down
+      const uint32_t g = s.list[i], k = g * 32u + 31u - (uint32_t)lane;                            // lanes from the group's largest value down
       const uint32_t n = tokens_of(k);
       const double w = n ? weight(k) : 0.0;
       const bool in = n && w >= (double)st.min_p;
       double m = (double)n * w, mm = in ? m : 0.0;
 #pragma unroll
       for (int o = 16; o; o >>= 1) { m += __shfl_xor_sync(~0u, m, o); mm += __shfl_xor_sync(~0u, mm, o); }
-      const uint32_t c = __reduce_add_sync(~0u, n), cm = __reduce_add_sync(~0u, in ? n : 0u);
-      if (lane == 0) { s.mass[g] = m; s.mass_min[g] = mm; s.count[g] = c; s.count_min[g] = cm; }
+      Group x;
+      x.mass = m; x.mass_min = mm; x.count = __reduce_add_sync(~0u, n); x.count_min = __reduce_add_sync(~0u, in ? n : 0u);
+      if (lane < C) *cluster.map_shared_rank(&s.group[g], lane) = x;
     }
     cluster.sync();
     // every block goes over all groups in descending order, two a thread: tokens and mass before each
-    uint32_t gc[2], gb, cm = 0u, total = 0u, total_min = 0u;
-    double gm[2], mb, mm = 0.0, total_m = 0.0, total_mm = 0.0;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int g = GROUPS - 1 - (2 * tid + k), c = g / per, x = g - c * per;
-      const Counts* o = cluster.map_shared_rank(&s, c);
-      gc[k] = o->count[x]; gm[k] = o->mass[x];
-      cm += o->count_min[x]; mm += o->mass_min[x];
-    }
-    gb = gc[0] + gc[1]; mb = gm[0] + gm[1];
+    Group x[2];
+    x[0] = s.group[GROUPS - 1 - 2 * tid]; x[1] = s.group[GROUPS - 2 - 2 * tid];
+    uint32_t gb = x[0].count + x[1].count, cm = __reduce_add_sync(~0u, x[0].count_min + x[1].count_min);
     const uint32_t own_c = gb;
+    double mb = x[0].mass + x[1].mass, mm = x[0].mass_min + x[1].mass_min;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(~0u, gb, o);
-      const double y = __shfl_up_sync(~0u, mb, o);
-      if (lane >= o) { gb += x; mb += y; }
+      const uint32_t y = __shfl_up_sync(~0u, gb, o);
+      const double z = __shfl_up_sync(~0u, mb, o);
+      if (lane >= o) { gb += y; mb += z; }
     }
-    cm = __reduce_add_sync(~0u, cm);
 #pragma unroll
     for (int o = 16; o; o >>= 1) mm += __shfl_xor_sync(~0u, mm, o);
     if (lane == 31) { s.wc[warp] = gb; s.wm[warp] = mb; s.wcm[warp] = cm; s.wmm[warp] = mm; }
-    __syncthreads();
-    double me;                                                      // mass up to and with this thread's groups
     gb -= own_c;
+    const double before = __shfl_up_sync(~0u, mb, 1);
+    __syncthreads();
     {
-      const double before = __shfl_up_sync(~0u, mb, 1);
       // the warps' sums in order: each lane one of them
       uint32_t c = s.wc[lane];
-      double m = s.wm[lane], mmin = s.wmm[lane];
+      double m = s.wm[lane];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(~0u, c, o);
-        const double y = __shfl_up_sync(~0u, m, o);
-        if (lane >= o) { c += x; m += y; }
+        const uint32_t y = __shfl_up_sync(~0u, c, o);
+        const double z = __shfl_up_sync(~0u, m, o);
+        if (lane >= o) { c += y; m += z; }
       }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) mmin += __shfl_xor_sync(~0u, mmin, o);
-      total = __shfl_sync(~0u, c, 31); total_m = __shfl_sync(~0u, m, 31); total_mm = mmin;
-      total_min = __reduce_add_sync(~0u, s.wcm[lane]);
       const uint32_t cw = __shfl_sync(~0u, c, (warp + 31) & 31);
-      const double mw = __shfl_sync(~0u, m, (warp + 31) & 31), here = warp ? mw : 0.0, next = __shfl_sync(~0u, m, warp);
+      const double mw = __shfl_sync(~0u, m, (warp + 31) & 31);
       gb += warp ? cw : 0u;
-      me = lane < 31 ? mb + here : next;
-      mb = lane ? before + here : here;
+      mb = (lane ? before : 0.0) + (warp ? mw : 0.0);
+      s.before_count[2 * tid] = gb; s.before_mass[2 * tid] = mb;
+      s.before_count[2 * tid + 1] = gb + x[0].count; s.before_mass[2 * tid + 1] = mb + x[0].mass;
+      if (tid == THREADS - 1) { s.before_count[GROUPS] = __shfl_sync(1u << 31, c, 31); s.before_mass[GROUPS] = __shfl_sync(1u << 31, m, 31); }
     }
-    // a border: the thread whose group it falls into names it, and a warp goes over the group's values
-    auto lookup = [&](int how, uint32_t rank, double x) {
-      __syncthreads();
-      if (tid == 0) s.found = 0;
-      __syncthreads();
-      uint32_t c0 = gb;
-      double m0 = mb;
+    __syncthreads();
+    if (warp == 0) {
+      uint32_t total_min = __reduce_add_sync(~0u, s.wcm[lane]);
+      double total_mm = s.wmm[lane];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const double m1 = k == 0 ? fmin(mb + gm[0], me) : me;       // (what a group ends with is, to the bit, what the next one begins with)
-        if (gc[k] && falls(how, rank, x, c0, gc[k], m0, m1)) { s.hit_group = (uint32_t)(GROUPS - 1 - (2 * tid + k)); s.hit_count = c0; s.hit_mass = m0; s.found = 1; }
-        c0 += gc[k]; m0 = m1;
-      }
-      __syncthreads();
-      if (s.found && warp == 0) {
-        const uint32_t k = s.hit_group * 32u + 31u - (uint32_t)lane, n = tokens_of(k);
+      for (int o = 16; o; o >>= 1) total_mm += __shfl_xor_sync(~0u, total_mm, o);
+      const uint32_t total = s.before_count[GROUPS];
+      const double total_m = s.before_mass[GROUPS];
+      // A border: the group it falls into -- the last that begins at or before it, found 32 at a time -- and then the value in it, a lane each.
+      uint32_t place_key = 0u, place_before = 0u, place_count = 0u;
+      double place_mass = 0.0, place_weight = 1.0;
+      auto lookup = [&](int how, uint32_t rank, double y) {
+        auto begins = [&](int i) { return how == BY_RANK ? s.before_count[i] <= rank : how == BY_MASS_BEFORE ? s.before_mass[i] < y : s.before_mass[i] <= y; };
+        // (beginnings do not fall, but by a rounding between two groups that hold next to nothing: the last one that holds is taken)
+        int i = 64 * (31 - __clz(__ballot_sync(~0u, begins(64 * lane)) | 1u));
+        i += 2 * (31 - __clz(__ballot_sync(~0u, begins(i + 2 * lane)) | 1u));
+        if (begins(i + 1)) ++i;
+        while (i > 0 && s.group[GROUPS - 1 - i].count == 0u) --i;     // (groups without tokens begin where the next one does)
+        const uint32_t k = (uint32_t)(GROUPS - 1 - i) * 32u + 31u - (uint32_t)lane, n = tokens_of(k);
         const double w = n ? weight(k) : 0.0;
         uint32_t c = n;
         double m = (double)n * w;
@@ -288,62 +293,64 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
         uint32_t cb = __shfl_up_sync(~0u, c, 1);
         double mbef = __shfl_up_sync(~0u, m, 1);
         if (lane == 0) { cb = 0u; mbef = 0.0; }
-        cb += s.hit_count;
-        const double m0 = s.hit_mass + mbef, m1 = s.hit_mass + m;
-        uint32_t hits = __ballot_sync(~0u, n && falls(how, rank, x, cb, n, m0, m1));
+        cb += s.before_count[i];
+        const double m0 = s.before_mass[i] + mbef, m1 = s.before_mass[i] + m;
+        uint32_t hits = __ballot_sync(~0u, n && falls(how, rank, y, cb, n, m0, m1));
         // (sums within a group are rounded apart from the group's: a border on its very end belongs to its last value)
-        if (!hits) { const uint32_t some = __ballot_sync(~0u, n != 0u); hits = 1u << (31 - __clz(some)); }
-        if (lane == __ffs(hits) - 1) { s.place_key = k; s.place_before = cb; s.place_count = n; s.place_mass = m0; s.place_weight = w; }
+        if (!hits) hits = 1u << (31 - __clz(__ballot_sync(~0u, n != 0u)));
+        const int x1 = __ffs(hits) - 1;
+        place_key = __shfl_sync(~0u, k, x1); place_before = __shfl_sync(~0u, cb, x1); place_count = __shfl_sync(~0u, n, x1);
+        place_mass = __shfl_sync(~0u, m0, x1); place_weight = __shfl_sync(~0u, w, x1);
+      };
+      uint32_t n = total;
+      double Wn = total_m;
+      if (st.k > 0 && (uint32_t)st.k < total) {
+        lookup(BY_RANK, (uint32_t)st.k - 1u, 0.0);
+        n = (uint32_t)st.k;
+        Wn = place_mass + (double)(n - place_before) * place_weight;
       }
-      __syncthreads();
-      return s.found != 0;
-    };
-    uint32_t n = total;
-    double Wn = total_m;
-    if (st.k > 0 && (uint32_t)st.k < total) {
-      lookup(BY_RANK, (uint32_t)st.k - 1u, 0.0);
-      n = (uint32_t)st.k;
-      Wn = s.place_mass + (double)(n - s.place_before) * s.place_weight;
-    }
-    if (st.top_p < 1.f) {
-      const double x = (double)st.top_p * Wn;
-      uint32_t np = 1u;
-      double Wp = 1.0;
-      if (x > 0.0 && lookup(BY_MASS_BEFORE, 0u, x)) {
-        const double q = ceil((x - s.place_mass) / s.place_weight);
-        const uint32_t in = (uint32_t)fmin(fmax(q, 1.0), (double)s.place_count);
-        np = s.place_before + in; Wp = s.place_mass + (double)in * s.place_weight;
+      if (st.top_p < 1.f) {
+        const double y = (double)st.top_p * Wn;
+        uint32_t np = 1u;
+        double Wp = 1.0;
+        if (y > 0.0) {
+          lookup(BY_MASS_BEFORE, 0u, y);
+          const double q = ceil((y - place_mass) / place_weight);
+          const uint32_t in = (uint32_t)fmin(fmax(q, 1.0), (double)place_count);
+          np = place_before + in; Wp = place_mass + (double)in * place_weight;
+        }
+        if (np < n) { n = np; Wn = Wp; }
       }
-      if (np < n) { n = np; Wn = Wp; }
+      if (st.min_p > 0.f && total_min < n) {
+        n = total_min ? total_min : 1u;
+        Wn = total_min ? total_mm : 1.0;
+      }
+      const double y = st.u * Wn;
+      lookup(BY_MASS_UPTO, 0u, y);
+      uint32_t nth = (uint32_t)fmin(fmax(floor((y - place_mass) / place_weight), 0.0), (double)(place_count - 1u));
+      if (place_before + nth >= n) {                                // rounding next to the last border: the last token that is kept
+        lookup(BY_RANK, n - 1u, 0.0);
+        nth = n - 1u - place_before;
+      }
+      // which block has it: the tokens of that value in the blocks before
+      uint32_t ahead = 0u, here = 0u;
+      from_all((const uint16_t*)s.hist + place_key, uint16_t(), [&](int c, uint16_t z) { if (c < r) ahead += z; if (c == r) here = z; });
+      if (lane == 0) {
+        s.at = place_key; s.nth = nth - ahead; s.mine = ahead <= nth && nth < ahead + here;
+        s.kept = (int)n; s.logp = (float)(log_weight(place_key) - log(Wn));
+      }
     }
-    if (st.min_p > 0.f && total_min < n) {
-      n = total_min ? total_min : 1u;
-      Wn = total_min ? total_mm : 1.0;
-    }
-    const double x = st.u * Wn;
-    const bool found = lookup(BY_MASS_UPTO, 0u, x);
-    if (found) nth = (uint32_t)fmin(fmax(floor((x - s.place_mass) / s.place_weight), 0.0), (double)(s.place_count - 1u));
-    if (!found || s.place_before + nth >= n) {                      // rounding next to the last border: the last token that is kept
-      lookup(BY_RANK, n - 1u, 0.0);
-      nth = n - 1u - s.place_before;
-    }
-    at = s.place_key;
-    logp = (float)(log_weight(at) - log(Wn));
-    kept = (int)n;
   }
-  // which block has it: the tokens of that value in the blocks before
-  bool mine;
-  if (greedy) mine = r == first_with_max;
-  else {
-    uint32_t before = 0u, here = 0u;
-    for (int c = 0; c <= r; ++c) { before += here; here = ((const uint16_t*)cluster.map_shared_rank(&s.hist[0], c))[at]; }
-    mine = before <= nth && nth < before + here;
-    nth -= before;
-  }
+  __syncthreads();
+  // nobody reads another block's memory from here on; a block leaves when all have come so far
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  const uint32_t at = s.at, nth = s.nth;
+  const float logp = s.logp;
+  const int kept = s.kept;
+  const bool mine = s.mine != 0;
   if (mine) {
     uint32_t* cnt = (uint32_t*)s.list;                              // matches by vector number and warp: the order of the indices
     uint32_t match[NV];
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t* w = (const uint32_t*)&key[i];
@@ -385,11 +392,11 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
       }
     }
   }
-  cluster.sync();                                                   // (no block leaves while another one reads its counters)
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ================================================================================================ logits of 32 bits
-constexpr int BINS = 2048;
+// (also 16-bit ones of a vocabulary that the counters of a cluster do not hold)
 // Logits as keys whose order as unsigned numbers is the order of the values; 0: not live (-inf, NaN).  -0 counts as +0.
 __device__ __forceinline__ uint32_t key_of(float l) {
   uint32_t u = __float_as_uint(l);
@@ -403,39 +410,18 @@ __device__ __forceinline__ float load(const float* p, int i) { return p[i]; }
 __device__ __forceinline__ float load(const __nv_bfloat16* p, int i) { return __bfloat162float(p[i]); }
 __device__ __forceinline__ float load(const __half* p, int i) { return __half2float(p[i]); }
 
-struct Bins {
-  uint32_t count[BINS], lo[BINS], hi[BINS];
+constexpr int BINS = 2048;
+struct Sums {
+  uint32_t count[BINS], lo[BINS], hi[BINS];                         // of this block's part
+  uint32_t all_count[2][BINS];                                      // of the row: by the first 11 bits of the key; by the next ones of one of those bins
+  unsigned long long all_mass[2][BINS];
+  uint32_t wc[WARPS], wcm[WARPS];
+  unsigned long long wm[WARPS], wmm[WARPS];
+  uint32_t maxkey, live, kept_min, here;
+  unsigned long long mass_min;
+  uint32_t bin, before_count, n;
+  unsigned long long before_mass;
 };
-struct Shared {
-  Bins top, sub;                              // by the first 11 bits of the key; by the next ones of one of those bins
-  uint32_t wc[WARPS];
-  unsigned long long wm[WARPS];
-  uint32_t bin, before_count, count, maxkey, live, kept_min;
-  unsigned long long before_mass, mass_min;
-  int token;
-};
-
-// (a, b) -> sums over the threads before this one, and over all
-__device__ void block_scan(Shared& s, uint32_t c, unsigned long long m, uint32_t& cb, unsigned long long& mb, uint32_t& ct, unsigned long long& mt) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t ci = c;
-  unsigned long long mi = m;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t co = __shfl_up_sync(~0u, ci, o);
-    const unsigned long long mo = __shfl_up_sync(~0u, mi, o);
-    if (lane >= o) { ci += co; mi += mo; }
-  }
-  __syncthreads();
-  if (lane == 31) { s.wc[warp] = ci; s.wm[warp] = mi; }
-  __syncthreads();
-  cb = ci - c; mb = mi - m; ct = 0; mt = 0;
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) { cb += s.wc[w]; mb += s.wm[w]; }
-    ct += s.wc[w]; mt += s.wm[w];
-  }
-}
-
 struct Row {
   double max, inv_t;
   double scale;                               // 2^S
@@ -449,179 +435,207 @@ __device__ __forceinline__ double real_weight(const Row& r, uint32_t key) {
   return d < 0.0 ? (d == -INFINITY ? 0.0 : exp(d * r.inv_t)) : 1.0;     // (beside an infinite logit a finite one has none, at any temperature)
 }
 __device__ __forceinline__ unsigned long long weight(const Row& r, uint32_t key) { return __double2ull_rn(real_weight(r, key) * r.scale); }
-__device__ __forceinline__ void add(Bins& b, uint32_t i, unsigned long long w) {
-  atomicAdd(&b.count[i], 1u);
-  const uint32_t lo = (uint32_t)w;
-  uint32_t hi = (uint32_t)(w >> 32);
-  if (lo) { const uint32_t old = atomicAdd(&b.lo[i], lo); hi += (old + lo < old) ? 1u : 0u; }
-  if (hi) atomicAdd(&b.hi[i], hi);
-}
-__device__ __forceinline__ unsigned long long mass(const Bins& b, int i) { return ((unsigned long long)b.hi[i] << 32) | b.lo[i]; }
 
-struct Place {
-  uint32_t key, before_count, count;          // a value, the tokens before its first one, its tokens
-  unsigned long long before_mass;
-  bool found;
-};
-
-// The bin (in descending order) that a lookup falls into, given the tokens and mass before all of them.
-__device__ bool find_bin(Shared& s, const Bins& b, int nbins, int how, uint32_t rank, double x, uint32_t c0, unsigned long long m0) {
-  const int t = threadIdx.x;
-  uint32_t c[2];
-  unsigned long long m[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int i = nbins - 1 - (2 * t + k);
-    c[k] = i >= 0 ? b.count[i] : 0u; m[k] = i >= 0 ? mass(b, i) : 0ull;
-  }
-  uint32_t cb, ct;
-  unsigned long long mb, mt;
-  block_scan(s, c[0] + c[1], m[0] + m[1], cb, mb, ct, mt);
-  if (t == 0) s.bin = ~0u;
-  __syncthreads();
-  cb += c0; mb += m0;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (falls(how, rank, x, cb, c[k], mb, mb + m[k])) { s.bin = (uint32_t)(nbins - 1 - (2 * t + k)); s.before_count = cb; s.before_mass = mb; s.count = c[k]; }
-    cb += c[k]; mb += m[k];
-  }
-  __syncthreads();
-  return s.bin != ~0u;
-}
-
+// C blocks have a row together; each goes over its part of it once for the first bins and once for every refinement (the part stays in its L1).
 template <typename T>
-__device__ Place lookup(Shared& s, const T* l, int V, const Row& r, int how, uint32_t rank, double x) {
-  Place p;
-  p.found = find_bin(s, s.top, BINS, how, rank, x, 0u, 0ull);
-  if (!p.found) return p;
-  uint32_t prefix = s.bin, cb = s.before_count, n = s.count;
-  unsigned long long mb = s.before_mass;
-  for (int level = 1; level < 3; ++level) {
-    const int bits = level == 1 ? 11 : 10, shift = level == 1 ? 10 : 0, nb = 1 << bits;
-    __syncthreads();
-    for (int i = threadIdx.x; i < nb; i += THREADS) { s.sub.count[i] = 0u; s.sub.lo[i] = 0u; s.sub.hi[i] = 0u; }
-    __syncthreads();
-    for (int i = threadIdx.x; i < V; i += THREADS) {
-      const uint32_t k = key_of(load(l, i));
-      if (k && (k >> (shift + bits)) == prefix) add(s.sub, (k >> shift) & (nb - 1), weight(r, k));
-    }
-    __syncthreads();
-    p.found = find_bin(s, s.sub, nb, how, rank, x, cb, mb);
-    if (!p.found) return p;                   // (cannot be: the sums of a bin are the bin's)
-    prefix = (prefix << bits) | s.bin; cb = s.before_count; mb = s.before_mass; n = s.count;
-  }
-  p.key = prefix; p.before_count = cb; p.before_mass = mb; p.count = n;
-  return p;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(THREADS) rows_kernel(const etxb_sample_args a) {
+__global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  Shared& s = *(Shared*)smem;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, V = a.V;
+  Sums& s = *(Sums*)smem;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), r = (int)cluster.block_rank(), row = blockIdx.x / C;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int i0 = (int)((long long)a.V * r / C), i1 = (int)((long long)a.V * (r + 1) / C);
   const T* l = (const T*)a.logits + (long long)row * a.row_stride;
-  const float Tm = a.temperature ? a.temperature[row] : a.temperature_all;
-  const int k = a.top_k ? a.top_k[row] : a.top_k_all;
-  const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
+  const Settings st = settings(a, row);
 
-  if (tid == 0) { s.maxkey = 0u; s.live = 0u; s.kept_min = 0u; s.mass_min = 0ull; s.token = -1; }
-  for (int i = tid; i < BINS; i += THREADS) { s.top.count[i] = 0u; s.top.lo[i] = 0u; s.top.hi[i] = 0u; }
+  if (tid == 0) { s.maxkey = 0u; s.live = 0u; s.kept_min = 0u; s.mass_min = 0ull; }
+  auto clear = [&]() { for (int i = tid; i < BINS; i += THREADS) { s.count[i] = 0u; s.lo[i] = 0u; s.hi[i] = 0u; } };
+  clear();
   __syncthreads();
   uint32_t mx = 0u, live = 0u;
-  for (int i = tid; i < V; i += THREADS) { const uint32_t key = key_of(load(l, i)); mx = max(mx, key); live += key ? 1u : 0u; }
+  for (int i = i0 + tid; i < i1; i += THREADS) { const uint32_t key = key_of(load(l, i)); mx = max(mx, key); live += key ? 1u : 0u; }
   mx = __reduce_max_sync(~0u, mx); live = __reduce_add_sync(~0u, live);
   if (lane == 0) { atomicMax(&s.maxkey, mx); atomicAdd(&s.live, live); }
-  __syncthreads();
-  mx = s.maxkey; live = s.live;
+  cluster.sync();
+  mx = live = 0u;
+  for (int c = 0; c < C; ++c) { mx = max(mx, *cluster.map_shared_rank(&s.maxkey, c)); live += *cluster.map_shared_rank(&s.live, c); }
 
   int token = -1, kept = 0;
   float logp = -INFINITY;
-  if (live > 0u) {
-    Place at;
-    uint32_t nth = 0u;                        // the drawn token: the nth one (by index) of the value at.key
-    at.key = mx; at.found = true;
-    logp = 0.f; kept = 1;
-    if (Tm > 0.f) {
-      Row r;
-      r.max = (double)value_of(mx); r.inv_t = 1.0 / (double)Tm;
-      r.scale = (double)(1ull << (62 - (32 - __clz(V - 1 | 1))));
-      uint32_t cm = 0u;
-      unsigned long long mm = 0ull;
-      for (int i = tid; i < V; i += THREADS) {
-        const uint32_t key = key_of(load(l, i));
-        if (!key) continue;
-        const double e = real_weight(r, key);
-        const unsigned long long w = __double2ull_rn(e * r.scale);
-        add(s.top, key >> 21, w);
-        if (e >= (double)min_p) { ++cm; mm += w; }
+  uint32_t at = mx, nth = 0u;                 // the drawn token: the nth one (by index) of that value
+  if (live > 0u) { logp = 0.f; kept = 1; }
+  if (live > 0u && st.T > 0.f) {
+    Row w;
+    w.max = (double)value_of(mx); w.inv_t = 1.0 / (double)st.T;
+    w.scale = (double)(1ull << (62 - (32 - __clz((a.V - 1) | 1))));
+    auto add = [&](uint32_t i, unsigned long long x) {
+      atomicAdd(&s.count[i], 1u);
+      const uint32_t lo = (uint32_t)x;
+      uint32_t hi = (uint32_t)(x >> 32);
+      if (lo) { const uint32_t old = atomicAdd(&s.lo[i], lo); hi += (old + lo < old) ? 1u : 0u; }
+      if (hi) atomicAdd(&s.hi[i], hi);
+    };
+    // the blocks' bins into the row's, which every block gets
+    auto join = [&](int level) {
+      cluster.sync();
+      for (int i = r * (BINS / C) + tid; i < (r + 1) * (BINS / C); i += THREADS) {
+        uint32_t n = 0u;
+        unsigned long long m = 0ull;
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; ++c)
+          if (c < C) {
+            const Sums* o = cluster.map_shared_rank(&s, c);
+            n += o->count[i]; m += ((unsigned long long)o->hi[i] << 32) + o->lo[i];
+          }
+        for (int c = 0; c < C; ++c) { Sums* o = cluster.map_shared_rank(&s, c); o->all_count[level][i] = n; o->all_mass[level][i] = m; }
       }
-      uint32_t cb, ct;
-      unsigned long long mb, mt;
+      cluster.sync();
+    };
+    uint32_t cm = 0u;
+    unsigned long long mm = 0ull;
+    for (int i = i0 + tid; i < i1; i += THREADS) {
+      const uint32_t key = key_of(load(l, i));
+      if (!key) continue;
+      const double e = real_weight(w, key);
+      const unsigned long long x = __double2ull_rn(e * w.scale);
+      add(key >> 21, x);
+      if (e >= (double)st.min_p) { ++cm; mm += x; }
+    }
+    cm = __reduce_add_sync(~0u, cm);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mm += __shfl_xor_sync(~0u, mm, o);
+    if (lane == 0) { atomicAdd(&s.kept_min, cm); atomicAdd(&s.mass_min, mm); }
+    join(0);
+    uint32_t n_min = 0u;
+    unsigned long long mass_min = 0ull;
+    for (int c = 0; c < C; ++c) { n_min += *cluster.map_shared_rank(&s.kept_min, c); mass_min += *cluster.map_shared_rank(&s.mass_min, c); }
+    // the bin (in descending order) that a lookup falls into, given the tokens and mass before all of them; the mass of all
+    auto find_bin = [&](int level, int nbins, int how, uint32_t rank, double x, uint32_t c0, unsigned long long m0) -> unsigned long long {
+      uint32_t c[2], ci;
+      unsigned long long m[2], mi;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int i = nbins - 1 - (2 * tid + k);
+        c[k] = i >= 0 ? s.all_count[level][i] : 0u; m[k] = i >= 0 ? s.all_mass[level][i] : 0ull;
+      }
+      ci = c[0] + c[1]; mi = m[0] + m[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(~0u, ci, o);
+        const unsigned long long z = __shfl_up_sync(~0u, mi, o);
+        if (lane >= o) { ci += y; mi += z; }
+      }
       __syncthreads();
-      block_scan(s, cm, mm, cb, mb, ct, mt);
-      const uint32_t n_min = ct;
-      const unsigned long long mass_min = mt;
-      uint32_t c2 = 0u;
-      unsigned long long m2 = 0ull;
-      for (int i = tid; i < BINS; i += THREADS) { c2 += s.top.count[i]; m2 += mass(s.top, i); }
-      block_scan(s, c2, m2, cb, mb, ct, mt);
-      uint32_t n = live;
-      unsigned long long Wn = mt;
-      if (k > 0 && (uint32_t)k < live) {
-        const Place p = lookup(s, l, V, r, BY_RANK, (uint32_t)k - 1u, 0.0);
-        n = (uint32_t)k;
-        Wn = p.before_mass + (unsigned long long)(n - p.before_count) * weight(r, p.key);
+      if (lane == 31) { s.wc[warp] = ci; s.wm[warp] = mi; }
+      if (tid == 0) s.bin = ~0u;
+      __syncthreads();
+      uint32_t cw = s.wc[lane];
+      unsigned long long mw = s.wm[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(~0u, cw, o);
+        const unsigned long long z = __shfl_up_sync(~0u, mw, o);
+        if (lane >= o) { cw += y; mw += z; }
       }
-      if (top_p < 1.f) {
-        const double x = (double)top_p * (double)Wn;
-        const Place p = lookup(s, l, V, r, BY_MASS_BEFORE, 0u, x);
-        uint32_t np = 1u;
-        unsigned long long Wp = (unsigned long long)r.scale;
-        if (x > 0.0 && p.found) {
-          const unsigned long long w = weight(r, p.key);
-          const double q = ceil((x - (double)p.before_mass) / (double)w);
-          const uint32_t in = (uint32_t)fmin(fmax(q, 1.0), (double)p.count);
-          np = p.before_count + in; Wp = p.before_mass + in * w;
+      const unsigned long long total = __shfl_sync(~0u, mw, 31);
+      const uint32_t cb = __shfl_sync(~0u, cw, (warp + 31) & 31);
+      const unsigned long long mb = __shfl_sync(~0u, mw, (warp + 31) & 31);
+      ci = c0 + (warp ? cb : 0u) + ci - c[0] - c[1]; mi = m0 + (warp ? mb : 0ull) + mi - m[0] - m[1];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (falls(how, rank, x, ci, c[k], mi, mi + m[k])) { s.bin = (uint32_t)(nbins - 1 - (2 * tid + k)); s.before_count = ci; s.before_mass = mi; s.n = c[k]; }
+        ci += c[k]; mi += m[k];
+      }
+      __syncthreads();
+      return total;
+    };
+    uint32_t place_key = 0u, place_before = 0u, place_count = 0u;
+    unsigned long long place_mass = 0ull;
+    auto lookup = [&](int how, uint32_t rank, double x) {
+      find_bin(0, BINS, how, rank, x, 0u, 0ull);
+      if (s.bin == ~0u) return false;
+      uint32_t prefix = s.bin, cb = s.before_count;
+      unsigned long long mb = s.before_mass;
+      for (int level = 1; level < 3; ++level) {
+        const int bits = level == 1 ? 11 : 10, shift = level == 1 ? 10 : 0, nb = 1 << bits;
+        clear();
+        __syncthreads();
+        for (int i = i0 + tid; i < i1; i += THREADS) {
+          const uint32_t k = key_of(load(l, i));
+          if (k && (k >> (shift + bits)) == prefix) add((k >> shift) & (nb - 1), weight(w, k));
         }
-        if (np < n) { n = np; Wn = Wp; }
+        join(1);
+        find_bin(1, nb, how, rank, x, cb, mb);
+        if (s.bin == ~0u) return false;       // (cannot be: the sums of a bin are the bin's)
+        prefix = (prefix << bits) | s.bin; cb = s.before_count; mb = s.before_mass;
       }
-      if (min_p > 0.f && n_min < n) {
-        if (n_min > 0u) { n = n_min; Wn = mass_min; }
-        else { n = 1u; Wn = (unsigned long long)r.scale; }
-      }
-      const float uf = a.u[row];
-      const double u = uf > 0.f ? fmin((double)uf, 1.0 - 0x1p-24) : 0.0;
-      const double x = u * (double)Wn;
-      at = lookup(s, l, V, r, BY_MASS_UPTO, 0u, x);
-      if (at.found) nth = (uint32_t)fmin(floor((x - (double)at.before_mass) / (double)weight(r, at.key)), (double)(at.count - 1u));
-      if (!at.found || at.before_count + nth >= n) {               // rounding next to the last border: the last token that is kept
-        at = lookup(s, l, V, r, BY_RANK, n - 1u, 0.0);
-        nth = n - 1u - at.before_count;
-      }
-      logp = (float)(log_weight(r, at.key) - log((double)Wn / r.scale));
-      kept = (int)n;
+      place_key = prefix; place_before = cb; place_mass = mb; place_count = s.n;
+      return true;
+    };
+    uint32_t n = live;
+    unsigned long long Wn = find_bin(0, BINS, BY_RANK, ~0u, 0.0, 0u, 0ull);
+    if (st.k > 0 && (uint32_t)st.k < live) {
+      lookup(BY_RANK, (uint32_t)st.k - 1u, 0.0);
+      n = (uint32_t)st.k;
+      Wn = place_mass + (unsigned long long)(n - place_before) * weight(w, place_key);
     }
-    // the nth token of that value, by index
-    uint32_t before = 0u;
-    for (int i0 = 0; i0 < V; i0 += THREADS) {
-      const int i = i0 + tid;
-      const bool is = i < V && key_of(load(l, i)) == at.key;
-      uint32_t cb, ct;
-      unsigned long long mb, mt;
-      block_scan(s, is ? 1u : 0u, 0ull, cb, mb, ct, mt);
-      if (is && before + cb == nth) s.token = i;
-      before += ct;
-      if (before > nth) break;
+    if (st.top_p < 1.f) {
+      const double x = (double)st.top_p * (double)Wn;
+      uint32_t np = 1u;
+      unsigned long long Wp = (unsigned long long)w.scale;
+      if (x > 0.0 && lookup(BY_MASS_BEFORE, 0u, x)) {
+        const unsigned long long y = weight(w, place_key);
+        const double q = ceil((x - (double)place_mass) / (double)y);
+        const uint32_t in = (uint32_t)fmin(fmax(q, 1.0), (double)place_count);
+        np = place_before + in; Wp = place_mass + in * y;
+      }
+      if (np < n) { n = np; Wn = Wp; }
     }
-    __syncthreads();
-    token = s.token;
+    if (st.min_p > 0.f && n_min < n) {
+      n = n_min ? n_min : 1u;
+      Wn = n_min ? mass_min : (unsigned long long)w.scale;
+    }
+    const double x = st.u * (double)Wn;
+    const bool found = lookup(BY_MASS_UPTO, 0u, x);
+    if (found) nth = (uint32_t)fmin(fmax(floor((x - (double)place_mass) / (double)weight(w, place_key)), 0.0), (double)(place_count - 1u));
+    if (!found || place_before + nth >= n) {                        // rounding next to the last border: the last token that is kept
+      lookup(BY_RANK, n - 1u, 0.0);
+      nth = n - 1u - place_before;
+    }
+    at = place_key;
+    logp = (float)(log_weight(w, at) - log((double)Wn / w.scale));
+    kept = (int)n;
   }
-  if (tid == 0) {
-    a.tokens[row] = token;
-    if (a.next) a.next[row] = token;
-    if (a.logprobs) a.logprobs[row] = logp;
-    if (a.kept) a.kept[row] = kept;
+  if (live == 0u) {
+    if (r == 0 && tid == 0) store(a, row, token, logp, kept);
+    cluster.sync();
+    return;
   }
+  // its nth token, by index: a warp has 32nd parts of the block's part
+  const int per = (i1 - i0 + WARPS - 1) / WARPS, w0 = i0 + warp * per, w1 = min(i1, w0 + per);
+  uint32_t c = 0u;
+  for (int i = w0 + lane; i < w1; i += 32) c += key_of(load(l, i)) == at ? 1u : 0u;
+  c = __reduce_add_sync(~0u, c);
+  if (tid == 0) s.here = 0u;
+  __syncthreads();
+  if (lane == 0) { s.wcm[warp] = c; atomicAdd(&s.here, c); }
+  cluster.sync();
+  uint32_t before = 0u;
+  for (int b = 0; b < r; ++b) before += *cluster.map_shared_rank(&s.here, b);
+  for (int b = 0; b < warp; ++b) before += s.wcm[b];
+  if (before <= nth && nth < before + c)
+    for (int i = w0; i < w1; i += 32) {
+      const bool is = i + lane < w1 && key_of(load(l, i + lane)) == at;
+      uint32_t hits = __ballot_sync(~0u, is);
+      const uint32_t some = (uint32_t)__popc(hits);
+      if (nth < before + some) {
+        for (uint32_t q = before; q < nth; ++q) hits &= hits - 1u;
+        if (lane == 0) store(a, row, i + __ffs(hits) - 1, logp, kept);
+        break;
+      }
+      before += some;
+    }
+  cluster.sync();                                                   // (no block leaves while another one reads its memory)
 }
 
 }  // namespace etxb_draw
@@ -656,9 +670,10 @@ extern "C" int32_t etxb_sample(int device, const etxb_sample_args* args, size_t 
   while ((vectors + C - 1) / C > CHUNK) C *= 2;
   const void* k;
   if (a.dtype == ETXB_F32 || C > MAX_CLUSTER) {
-    k = a.dtype == ETXB_F32 ? (const void*)rows_kernel<float> : a.dtype == ETXB_F16 ? (const void*)rows_kernel<__half> : (const void*)rows_kernel<__nv_bfloat16>;
+    k = a.dtype == ETXB_F32 ? (const void*)sums_kernel<float> : a.dtype == ETXB_F16 ? (const void*)sums_kernel<__half> : (const void*)sums_kernel<__nv_bfloat16>;
     C = 1;
-    cfg.dynamicSmemBytes = sizeof(Shared);
+    while (C < MAX_CLUSTER && (long long)a.rows * 2 * C <= sms && a.V / C > 2048) C *= 2;
+    cfg.dynamicSmemBytes = sizeof(Sums);
   } else {
     while (C < MAX_CLUSTER && (long long)a.rows * 2 * C <= sms && vectors / C > 1024) C *= 2;
     const int nv = (int)((vectors + C - 1) / C + THREADS - 1) / THREADS;

@@ -873,7 +873,7 @@ typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, voi
 static int32_t sizes(int device, const etxb_attn_shared_args& a, unsigned char* work, etxb_shared::Layout& y, size_t& bytes) {
   using namespace etxb_shared;
   int sms = 0;
-  ETXB_HOST_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  ETXB_HOST_CU(etxb_host_sms(device, &sms));
   if (sms > MAX_WORKERS) sms = MAX_WORKERS;
   if (!lay_out(a, sms, work, y, bytes)) return refuse(ETXB_E_UNSUPPORTED, "the tables' widths allow 2^31 tiles");
   return ETXB_OK;
@@ -930,7 +930,8 @@ extern "C" int32_t etxb_attn_shared(int device, const etxb_attn_shared_args* arg
   const int slots = (232448 - (int)sizeof(Shared) - 1024 - other) / slot & ~1;
   P.y.slots = slots > MAX_SLOTS ? MAX_SLOTS : slots;                // (four at least: 128 rows of Q and 1024 sequences leave 130 KB)
   const int smem = other + P.y.slots * slot;
-  ETXB_HOST_CU(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<char> ready[2][64];
+  ETXB_HOST_CU(etxb_host_smem(k, 232448 - (int)sizeof(Shared) - 1024, device, ready[a.HD > 128]));
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = dim3((unsigned)P.y.workers); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = (size_t)smem; cfg.stream = (cudaStream_t)cuda_stream;

@@ -2,6 +2,9 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <stdio.h>
+
+#include <atomic>
 
 #include "../../include/etxb200.h"
 
@@ -17,6 +20,26 @@ __attribute__((visibility("hidden"))) int32_t etxb_host_fail(int32_t code, const
       return etxb_host_fail(ETXB_E_CUDA, m_);                                                   \
     }                                                                                           \
   } while (0)
+
+// The number of a device's processors (asked once).
+inline cudaError_t etxb_host_sms(int device, int* sms) {
+  static std::atomic<int> known[64];
+  int n = known[device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    const cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return e;
+    known[device].store(n, std::memory_order_relaxed);
+  }
+  *sms = n;
+  return cudaSuccess;
+}
+// Lets a kernel have `bytes` of dynamic shared memory on the current device; `done`: 64 flags of the kernel's own, one a device (asked for once).
+inline cudaError_t etxb_host_smem(const void* kernel, int bytes, int device, std::atomic<char>* done) {
+  if (done[device].load(std::memory_order_relaxed)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done[device].store(1, std::memory_order_relaxed);
+  return e;
+}
 
 // The device of a call is current while the call runs; the caller's own is current again behind it.
 struct EtxbDeviceScope {

@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <mutex>
 #include <new>
 #include <vector>
 
@@ -219,10 +220,256 @@ extern "C" int32_t etxb_pages_update(int device, const etxb_pages_args* args, si
     EtxbDeviceScope scope(device);
     ETXB_HOST_CU(scope.err);
     int sms = 0;
-    ETXB_HOST_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    ETXB_HOST_CU(etxb_host_sms(device, &sms));
     ETXB_HOST_CU(etxb_pages::run_all(*args, sms, (cudaStream_t)cuda_stream));
   } catch (const std::bad_alloc&) {
     return etxb_host_fail(ETXB_E_ARG, "pages: the lists do not fit the host's memory");
   }
   return ETXB_OK;
+}
+
+// ---- the books of a pool -------------------------------------------------------------------------------------------
+struct etxb_pool {
+  int device = 0, page_len = 16;
+  etxb_pages_args base{};                       // the pool as source and destination, its tables
+  etxb_pages_fn update = nullptr;
+  std::mutex mutex;
+  std::vector<int32_t> users;                   // sequences that hold a page
+  int32_t n_free = 0, lowest = 0;               // free pages, and a page below which none is
+  std::vector<std::vector<int32_t>> pages;      // of a row, in order
+  std::vector<int32_t> length;                  // -1: no sequence
+};
+
+namespace etxb_pages {
+
+static int32_t refuse(int32_t code, const char* fmt, long long x = 0, long long y = 0, long long z = 0) {
+  char m[160], text[200];
+  snprintf(m, sizeof m, fmt, x, y, z);
+  snprintf(text, sizeof text, "pool: %s", m);
+  return etxb_host_fail(code, text);
+}
+// One call on a pool: excludes others, and turns what the host's memory refuses into a status.
+template <typename F>
+static int32_t with(etxb_pool* p, F f) {
+  if (!p) return refuse(ETXB_E_ARG, "null");
+  try {
+    std::lock_guard<std::mutex> lock(p->mutex);
+    return f(*p);
+  } catch (const std::exception&) {
+    return refuse(ETXB_E_ARG, "the books do not fit the host's memory");
+  }
+}
+static bool holds(const etxb_pool& p, int32_t row) { return row >= 0 && row < (int32_t)p.length.size() && p.length[(size_t)row] >= 0; }
+static int32_t need(const etxb_pool& p, int32_t length) { return (int32_t)(((long long)length + p.page_len - 1) / p.page_len); }
+// n free pages, the lowest first (nothing is marked yet)
+static int32_t take(const etxb_pool& p, long long n, std::vector<int32_t>& out) {
+  if (n > p.n_free) return refuse(ETXB_E_FULL, "%lld free pages, %lld are needed", p.n_free, n);
+  out.reserve((size_t)n);
+  for (int32_t i = p.lowest; (long long)out.size() < n; ++i) if (p.users[(size_t)i] == 0) out.push_back(i);
+  return ETXB_OK;
+}
+static int32_t free_rows(const etxb_pool& p, int32_t n, std::vector<int32_t>& out) {
+  for (int32_t r = 0; r < (int32_t)p.length.size() && (int32_t)out.size() < n; ++r) if (p.length[(size_t)r] < 0) out.push_back(r);
+  return (int32_t)out.size() < n ? refuse(ETXB_E_FULL, "%lld free rows in the tables, %lld are needed", (long long)out.size(), n) : ETXB_OK;
+}
+static void hold(etxb_pool& p, const std::vector<int32_t>& fresh) {
+  for (int32_t i : fresh) p.users[(size_t)i] = 1;
+  p.n_free -= (int32_t)fresh.size();
+  if (!fresh.empty() && fresh.front() == p.lowest) p.lowest = fresh.back() + 1;      // (they were the lowest free ones)
+}
+static int32_t carry_out(etxb_pool& p, etxb_pages_args& a, void* stream) { return p.update(p.device, &a, sizeof a, stream); }
+static int32_t rows_once(const etxb_pool& p, const int32_t* rows, int32_t n) {
+  if (n < 0 || (n && !rows)) return refuse(ETXB_E_ARG, "a list is null");
+  std::vector<uint8_t> seen(p.length.size(), 0);
+  for (int32_t i = 0; i < n; ++i) {
+    if (!holds(p, rows[i])) return refuse(ETXB_E_ARG, "row %lld holds no sequence", rows[i]);
+    if (seen[(size_t)rows[i]]) return refuse(ETXB_E_ARG, "each row once");
+    seen[(size_t)rows[i]] = 1;
+  }
+  return ETXB_OK;
+}
+
+}  // namespace etxb_pages
+
+extern "C" int32_t etxb_pool_create(int device, const etxb_pages_args* layout, size_t bytes, int32_t page_len, etxb_pages_fn update, etxb_pool** out) {
+  using namespace etxb_pages;
+  if (!out || !layout || bytes != sizeof(etxb_pages_args)) return refuse(ETXB_E_ARG, "needs an etxb_pages_args");
+  if (page_len < 1 || layout->dst_pages < 1 || layout->table_rows < 1 || layout->table_width < 1) return refuse(ETXB_E_ARG, "at least one page, row, entry and position");
+  if (device < 0 || device >= 64) return refuse(ETXB_E_ARG, "device index out of range");
+  try {
+    etxb_pool* p = new etxb_pool;
+    p->device = device; p->page_len = page_len; p->update = update ? update : etxb_pages_update;
+    p->base = *layout;
+    for (etxb_page_tensor& t : p->base.t) { t.src = t.dst; t.src_layer = t.dst_layer; t.src_page = t.dst_page; }
+    p->base.src_pages = layout->dst_pages;
+    p->base.n_copy = p->base.n_set = p->base.n_share = p->base.n_remap = 0;
+    p->users.assign((size_t)layout->dst_pages, 0);
+    p->n_free = layout->dst_pages;
+    p->pages.resize((size_t)layout->table_rows);
+    p->length.assign((size_t)layout->table_rows, -1);
+    *out = p;
+  } catch (const std::exception&) {
+    return refuse(ETXB_E_ARG, "the books do not fit the host's memory");
+  }
+  return ETXB_OK;
+}
+
+extern "C" int32_t etxb_pool_destroy(etxb_pool* pool) {
+  delete pool;
+  return ETXB_OK;
+}
+
+extern "C" int32_t etxb_pool_open(etxb_pool* pool, int32_t length, int32_t* row, void* cuda_stream) {
+  using namespace etxb_pages;
+  return with(pool, [&](etxb_pool& p) -> int32_t {
+    if (!row || length < 0) return refuse(ETXB_E_ARG, "a length of %lld positions", length);
+    const int32_t n = need(p, length);
+    if (n > p.base.table_width) return refuse(ETXB_E_ARG, "%lld positions take %lld pages, a table has %lld", length, n, p.base.table_width);
+    std::vector<int32_t> r, fresh;
+    if (int32_t rc = free_rows(p, 1, r)) return rc;
+    if (int32_t rc = take(p, n, fresh)) return rc;
+    std::vector<int32_t> rows((size_t)n, r[0]), cols((size_t)n);
+    for (int32_t i = 0; i < n; ++i) cols[(size_t)i] = i;
+    std::vector<int32_t> mine = fresh;
+    if (n) {
+      etxb_pages_args a = p.base;
+      a.n_set = n; a.set_rows = rows.data(); a.set_cols = cols.data(); a.set_pages = fresh.data();
+      if (int32_t rc = carry_out(p, a, cuda_stream)) return rc;
+    }
+    hold(p, fresh);
+    p.pages[(size_t)r[0]].swap(mine);
+    p.length[(size_t)r[0]] = length;
+    *row = r[0];
+    return ETXB_OK;
+  });
+}
+
+extern "C" int32_t etxb_pool_extend(etxb_pool* pool, const int32_t* rows, const int32_t* lengths, int32_t n, void* cuda_stream) {
+  using namespace etxb_pages;
+  return with(pool, [&](etxb_pool& p) -> int32_t {
+    if (int32_t rc = rows_once(p, rows, n)) return rc;
+    if (n && !lengths) return refuse(ETXB_E_ARG, "a list is null");
+    long long more = 0;
+    for (int32_t i = 0; i < n; ++i) {
+      const int32_t have = p.length[(size_t)rows[i]], want = need(p, lengths[i]);
+      if (lengths[i] < have) return refuse(ETXB_E_ARG, "row %lld has %lld positions, not %lld", rows[i], have, lengths[i]);
+      if (want > p.base.table_width) return refuse(ETXB_E_ARG, "%lld positions take %lld pages, a table has %lld", lengths[i], want, p.base.table_width);
+      more += want - (int32_t)p.pages[(size_t)rows[i]].size();
+    }
+    std::vector<int32_t> fresh, r, c;
+    if (int32_t rc = take(p, more, fresh)) return rc;
+    r.reserve(fresh.size()); c.reserve(fresh.size());
+    for (int32_t i = 0; i < n; ++i) {
+      std::vector<int32_t>& mine = p.pages[(size_t)rows[i]];
+      mine.reserve((size_t)need(p, lengths[i]));
+      for (int32_t k = (int32_t)mine.size(); k < need(p, lengths[i]); ++k) { r.push_back(rows[i]); c.push_back(k); }
+    }
+    if (!fresh.empty()) {
+      etxb_pages_args a = p.base;
+      a.n_set = (int32_t)fresh.size(); a.set_rows = r.data(); a.set_cols = c.data(); a.set_pages = fresh.data();
+      if (int32_t rc = carry_out(p, a, cuda_stream)) return rc;
+    }
+    hold(p, fresh);
+    for (size_t i = 0; i < fresh.size(); ++i) p.pages[(size_t)r[i]].push_back(fresh[i]);
+    for (int32_t i = 0; i < n; ++i) p.length[(size_t)rows[i]] = lengths[i];
+    return ETXB_OK;
+  });
+}
+
+extern "C" int32_t etxb_pool_fork(etxb_pool* pool, int32_t row, int32_t n, int32_t length, int32_t* rows, void* cuda_stream) {
+  using namespace etxb_pages;
+  return with(pool, [&](etxb_pool& p) -> int32_t {
+    if (!holds(p, row)) return refuse(ETXB_E_ARG, "row %lld holds no sequence", row);
+    const int32_t have = p.length[(size_t)row], len = length == -1 ? have : length;
+    if (n < 0 || (n && !rows) || len < 0 || len > have) return refuse(ETXB_E_ARG, "fork: %lld sequences from %lld positions of %lld", n, len, have);
+    const int32_t full = len / p.page_len, part = len % p.page_len ? 1 : 0;
+    std::vector<int32_t> r, fresh;
+    if (int32_t rc = free_rows(p, n, r)) return rc;
+    if (int32_t rc = take(p, (long long)n * part, fresh)) return rc;
+    const std::vector<int32_t>& mine = p.pages[(size_t)row];
+    std::vector<std::vector<int32_t>> theirs((size_t)n);
+    for (int32_t i = 0; i < n; ++i) {
+      theirs[(size_t)i].reserve((size_t)(full + part));
+      theirs[(size_t)i].assign(mine.begin(), mine.begin() + full);
+      if (part) theirs[(size_t)i].push_back(fresh[(size_t)i]);
+    }
+    if (n && (full || part)) {
+      etxb_pages_args a = p.base;
+      const std::vector<int32_t> src((size_t)n, part ? mine[(size_t)full] : 0), cols((size_t)n, full);
+      if (part) {
+        a.n_copy = n; a.src_ids = src.data(); a.dst_ids = fresh.data();
+        a.n_set = n; a.set_rows = r.data(); a.set_cols = cols.data(); a.set_pages = fresh.data();
+      }
+      a.n_share = n; a.share_rows = r.data(); a.share_from = row; a.shared = full;
+      if (int32_t rc = carry_out(p, a, cuda_stream)) return rc;
+    }
+    for (int32_t i = 0; i < full; ++i) p.users[(size_t)mine[(size_t)i]] += n;
+    hold(p, fresh);
+    for (int32_t i = 0; i < n; ++i) {
+      p.pages[(size_t)r[(size_t)i]].swap(theirs[(size_t)i]);
+      p.length[(size_t)r[(size_t)i]] = len;
+      rows[i] = r[(size_t)i];
+    }
+    return ETXB_OK;
+  });
+}
+
+extern "C" int32_t etxb_pool_close(etxb_pool* pool, const int32_t* rows, int32_t n) {
+  using namespace etxb_pages;
+  return with(pool, [&](etxb_pool& p) -> int32_t {
+    if (int32_t rc = rows_once(p, rows, n)) return rc;
+    for (int32_t i = 0; i < n; ++i) {
+      for (int32_t page : p.pages[(size_t)rows[i]])
+        if (--p.users[(size_t)page] == 0) { ++p.n_free; p.lowest = std::min(p.lowest, page); }
+      p.pages[(size_t)rows[i]].clear();
+      p.length[(size_t)rows[i]] = -1;
+    }
+    return ETXB_OK;
+  });
+}
+
+extern "C" int32_t etxb_pool_compact(etxb_pool* pool, int32_t* moved, void* cuda_stream) {
+  using namespace etxb_pages;
+  return with(pool, [&](etxb_pool& p) -> int32_t {
+    const int32_t total = (int32_t)p.users.size(), used = total - p.n_free;
+    std::vector<int32_t> high, low;
+    for (int32_t i = total - 1; i >= used; --i) if (p.users[(size_t)i]) high.push_back(i);
+    for (int32_t i = p.lowest; i < used; ++i) if (!p.users[(size_t)i]) low.push_back(i);
+    if (moved) *moved = (int32_t)high.size();
+    if (high.empty()) return ETXB_OK;
+    std::vector<int32_t> to((size_t)total, -1), rows, entries;
+    for (size_t i = 0; i < high.size(); ++i) to[(size_t)high[i]] = low[i];
+    for (int32_t r = 0; r < (int32_t)p.length.size(); ++r)
+      if (!p.pages[(size_t)r].empty()) { rows.push_back(r); entries.push_back((int32_t)p.pages[(size_t)r].size()); }
+    etxb_pages_args a = p.base;
+    a.n_copy = (int32_t)high.size(); a.src_ids = high.data(); a.dst_ids = low.data();
+    a.n_remap = (int32_t)rows.size(); a.remap_rows = rows.data(); a.remap_entries = entries.data();
+    if (int32_t rc = carry_out(p, a, cuda_stream)) return rc;
+    for (size_t i = 0; i < high.size(); ++i) { p.users[(size_t)low[i]] = p.users[(size_t)high[i]]; p.users[(size_t)high[i]] = 0; }
+    for (int32_t r : rows)
+      for (int32_t& page : p.pages[(size_t)r]) if (to[(size_t)page] >= 0) page = to[(size_t)page];
+    p.lowest = used;
+    return ETXB_OK;
+  });
+}
+
+extern "C" int32_t etxb_pool_row(etxb_pool* pool, int32_t row, int32_t* length, int32_t* pages, int32_t capacity, int32_t* n) {
+  using namespace etxb_pages;
+  return with(pool, [&](etxb_pool& p) -> int32_t {
+    if (row < 0 || row >= (int32_t)p.length.size() || capacity < 0) return refuse(ETXB_E_ARG, "row %lld of %lld", row, (long long)p.length.size());
+    const std::vector<int32_t>& mine = p.pages[(size_t)row];
+    if (length) *length = p.length[(size_t)row];
+    if (n) *n = (int32_t)mine.size();
+    if (pages) std::copy(mine.begin(), mine.begin() + std::min((size_t)capacity, mine.size()), pages);
+    return ETXB_OK;
+  });
+}
+
+extern "C" int32_t etxb_pool_free(etxb_pool* pool, int32_t* pages) {
+  using namespace etxb_pages;
+  return with(pool, [&](etxb_pool& p) -> int32_t {
+    if (!pages) return refuse(ETXB_E_ARG, "null");
+    *pages = p.n_free;
+    return ETXB_OK;
+  });
 }

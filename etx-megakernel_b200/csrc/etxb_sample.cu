@@ -657,7 +657,7 @@ extern "C" int32_t etxb_sample(int device, const etxb_sample_args* args, size_t 
   EtxbDeviceScope scope(device);
   ETXB_HOST_CU(scope.err);
   int sms = 0;
-  ETXB_HOST_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  ETXB_HOST_CU(etxb_host_sms(device, &sms));
   void* kargs[] = {(void*)&a};
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
@@ -668,25 +668,27 @@ extern "C" int32_t etxb_sample(int device, const etxb_sample_args* args, size_t 
   int C = 1;
   const long long vectors = ((long long)a.V + 7 + 7) / 8;
   while ((vectors + C - 1) / C > CHUNK) C *= 2;
+  static std::atomic<char> ready[11][64];
   const void* k;
+  int which;
   if (a.dtype == ETXB_F32 || C > MAX_CLUSTER) {
-    k = a.dtype == ETXB_F32 ? (const void*)sums_kernel<float> : a.dtype == ETXB_F16 ? (const void*)sums_kernel<__half> : (const void*)sums_kernel<__nv_bfloat16>;
+    static const void* const kernels[3] = {(const void*)sums_kernel<__nv_bfloat16>, (const void*)sums_kernel<__half>, (const void*)sums_kernel<float>};
+    k = kernels[a.dtype]; which = 8 + a.dtype;
     C = 1;
     while (C < MAX_CLUSTER && (long long)a.rows * 2 * C <= sms && a.V / C > 2048) C *= 2;
     cfg.dynamicSmemBytes = sizeof(Sums);
   } else {
+    static const void* const kernels[2][4] = {
+        {(const void*)counts_kernel<__nv_bfloat16, 1>, (const void*)counts_kernel<__nv_bfloat16, 2>, (const void*)counts_kernel<__nv_bfloat16, 4>, (const void*)counts_kernel<__nv_bfloat16, 8>},
+        {(const void*)counts_kernel<__half, 1>, (const void*)counts_kernel<__half, 2>, (const void*)counts_kernel<__half, 4>, (const void*)counts_kernel<__half, 8>}};
     while (C < MAX_CLUSTER && (long long)a.rows * 2 * C <= sms && vectors / C > 1024) C *= 2;
-    const int nv = (int)((vectors + C - 1) / C + THREADS - 1) / THREADS;
-    const bool half = a.dtype == ETXB_F16;
-    k = nv <= 1 ? (half ? (const void*)counts_kernel<__half, 1> : (const void*)counts_kernel<__nv_bfloat16, 1>)
-      : nv <= 2 ? (half ? (const void*)counts_kernel<__half, 2> : (const void*)counts_kernel<__nv_bfloat16, 2>)
-      : nv <= 4 ? (half ? (const void*)counts_kernel<__half, 4> : (const void*)counts_kernel<__nv_bfloat16, 4>)
-                : (half ? (const void*)counts_kernel<__half, 8> : (const void*)counts_kernel<__nv_bfloat16, 8>);
+    const int nv = ((int)((vectors + C - 1) / C) + THREADS - 1) / THREADS, size = nv <= 1 ? 0 : nv <= 2 ? 1 : nv <= 4 ? 2 : 3;
+    k = kernels[a.dtype == ETXB_F16][size]; which = 4 * (a.dtype == ETXB_F16) + size;
     cfg.dynamicSmemBytes = sizeof(Counts);
   }
   at.val.clusterDim.x = (unsigned)C; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)(a.rows * C));
-  ETXB_HOST_CU(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes));
+  ETXB_HOST_CU(etxb_host_smem(k, (int)cfg.dynamicSmemBytes, device, ready[which]));
   ETXB_HOST_CU(cudaLaunchKernelExC(&cfg, k, kargs));
   return ETXB_OK;
 }

@@ -3,10 +3,13 @@ from __future__ import annotations
 
 import torch
 
+_Tensor = torch.Tensor
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
 
 def cuda_tensor(name: str, t, dtypes, shape=None, inner: bool = True):
     """`t` as a CUDA tensor of one of `dtypes`; `shape` with None for sizes that are free; inner: the last dimension's elements adjoin."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not isinstance(t, _Tensor) or not t.is_cuda:
         raise ValueError(f"{name}: a CUDA tensor, got {getattr(t, 'device', type(t).__name__)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name}: dtype {t.dtype} is none of {', '.join(str(d) for d in dtypes)}")
@@ -17,19 +20,29 @@ def cuda_tensor(name: str, t, dtypes, shape=None, inner: bool = True):
     return t
 
 
+def vector(name: str, t, dtype, n: int, index: int):
+    """`t` as `n` adjoining values on device `index` (the checks of cuda_tensor and same_device, quick where they pass)."""
+    if isinstance(t, _Tensor) and t.is_cuda and t.dtype is dtype and t.shape == (n,) and (n < 2 or t.stride(0) == 1) and t.get_device() == index:
+        return t
+    cuda_tensor(name, t, (dtype,), (n,))
+    raise ValueError(f"{name} is on {t.device}, the call runs on cuda:{index}")
+
+
 def same_device(device, **tensors):
     for name, t in tensors.items():
         if t is not None and t.device != device:
             raise ValueError(f"{name} is on {t.device}, the call runs on {device}")
 
 
-def stream_handle(device, stream, tensors) -> int:
-    """The raw handle of the call's stream: the current one of `device`, or `stream` (a raw handle or a torch stream), which the tensors' memory is then
-    kept for until it has passed the call."""
+def stream_handle(index: int, stream, tensors) -> int:
+    """The raw handle of the call's stream on device `index`: the current one, or `stream` (a raw handle or a torch stream), which the tensors' memory is
+    then kept for until it has passed the call."""
+    current = _raw_stream(index)
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
+        return current
     handle = int(getattr(stream, "cuda_stream", stream))
-    if handle != torch.cuda.current_stream(device).cuda_stream:
+    if handle != current:
+        device = torch.device("cuda", index)
         s = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
         for t in tensors:
             if t is not None:

@@ -4,14 +4,16 @@ Beside the tiles of the step (ops/attn.py), which read every sequence's whole co
 from __future__ import annotations
 
 import ctypes as C
+from itertools import accumulate
 
-import numpy as np
 import torch
 
 from . import lib as L
-from ._call import cuda_tensor, same_device, stream_handle
+from ._call import cuda_tensor, same_device, stream_handle, vector
 
 MAX_SEQS = 1024
+_BF16, _I32 = (torch.bfloat16,), (torch.int32,)
+_BYTES = C.sizeof(L.AttnSharedArgs)
 _BAD = {1: "a table names a page outside the cache", 2: "a length lies outside its table", 4: "a wait inside the kernel ran past two seconds"}
 
 
@@ -30,49 +32,54 @@ def attn_shared(q, kc, vc, tables, lens, prefix_tables, prefix_lens, groups=None
     stream       a raw handle or torch stream; None is the current one
 
     Scores, statistics and sums are fp32.  A sequence without any position has the output 0.  Equal inputs give equal outputs."""
-    cuda_tensor("kc", kc, (torch.bfloat16,), (None, None, None, 16, 8))
+    cuda_tensor("kc", kc, _BF16, (None, None, None, 16, 8), inner=False)
     pages, NKV, hd8 = kc.shape[:3]
-    HD = 8 * hd8
-    cuda_tensor("vc", vc, (torch.bfloat16,), (pages, NKV, HD, 16))
-    if not kc[0].is_contiguous() or not vc[0].is_contiguous():
+    HD, page = 8 * hd8, NKV * hd8 * 128
+    cuda_tensor("vc", vc, _BF16, (pages, NKV, HD, 16), inner=False)
+    if kc.stride()[1:] != (hd8 * 128, 128, 8, 1) or vc.stride()[1:] != (HD * 16, 16, 1):
         raise ValueError("kc, vc: a page has no gaps")
-    cuda_tensor("q", q, (torch.bfloat16,))
-    if q.dim() == 3 and q.shape[2] != HD or q.dim() not in (2, 3) or (q.dim() == 2 and q.shape[1] % HD) or (q.dim() == 3 and q.shape[1] > 1 and q.stride(1) != HD):
-        raise ValueError(f"q: shape {tuple(q.shape)} with strides {q.stride()}, expected [sequences][heads][{HD}] with adjoining heads")
-    seqs, NH = q.shape[0], q.shape[1] if q.dim() == 3 else q.shape[1] // HD
+    cuda_tensor("q", q, _BF16)
+    shape = q.shape
+    if len(shape) == 3 and (shape[2] != HD or (shape[1] > 1 and q.stride(1) != HD)) or len(shape) not in (2, 3) or (len(shape) == 2 and shape[1] % HD):
+        raise ValueError(f"q: shape {tuple(shape)} with strides {q.stride()}, expected [sequences][heads][{HD}] with adjoining heads")
+    seqs, NH, index = shape[0], shape[1] if len(shape) == 3 else shape[1] // HD, q.get_device()
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    cuda_tensor("out", out, (torch.bfloat16,), tuple(q.shape))
-    if out.dim() == 3 and NH > 1 and out.stride(1) != HD:
-        raise ValueError("out: the heads of a row adjoin")
-    cuda_tensor("tables", tables, (torch.int32,), (seqs, None))
-    cuda_tensor("lens", lens, (torch.int32,), (seqs,))
-    cuda_tensor("prefix_tables", prefix_tables, (torch.int32,), (None, None))
+        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+    else:
+        cuda_tensor("out", out, _BF16, shape)
+        if len(shape) == 3 and NH > 1 and out.stride(1) != HD:
+            raise ValueError("out: the heads of a row adjoin")
+    cuda_tensor("tables", tables, _I32, (seqs, None))
+    vector("lens", lens, torch.int32, seqs, index)
+    cuda_tensor("prefix_tables", prefix_tables, _I32, (None, None))
     n_groups = prefix_tables.shape[0]
-    cuda_tensor("prefix_lens", prefix_lens, (torch.int32,), (n_groups,))
+    vector("prefix_lens", prefix_lens, torch.int32, n_groups, index)
     if status is not None:
-        cuda_tensor("status", status, (torch.int32,), (1,))
-    sizes = [seqs] if groups is None else [int(n) for n in groups]
-    if len(sizes) != n_groups or any(n < 0 for n in sizes) or sum(sizes) != seqs:
-        raise ValueError(f"groups: {n_groups} sizes of {seqs} sequences altogether, got {sizes}")
+        vector("status", status, torch.int32, 1, index)
+    sizes = (seqs,) if groups is None else [int(n) for n in groups]
+    if len(sizes) != n_groups or min(sizes, default=0) < 0 or sum(sizes) != seqs:
+        raise ValueError(f"groups: {n_groups} sizes of {seqs} sequences altogether, got {list(sizes)}")
     if seqs > MAX_SEQS or n_groups > MAX_SEQS:
         raise ValueError(f"attn_shared: at most {MAX_SEQS} sequences and groups")
-    same_device(q.device, kc=kc, vc=vc, out=out, tables=tables, lens=lens, prefix_tables=prefix_tables, prefix_lens=prefix_lens, status=status)
-    first = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
-    a = L.AttnSharedArgs(q=q.data_ptr(), out=out.data_ptr(), kc=kc.data_ptr(), vc=vc.data_ptr(), tables=tables.data_ptr(), lens=lens.data_ptr(),
-                         prefix_tables=prefix_tables.data_ptr(), prefix_lens=prefix_lens.data_ptr(), group_first=first.ctypes.data,
-                         status=status.data_ptr() if status is not None else None,
-                         q_stride=q.stride(0) if seqs > 1 else NH * HD, out_stride=out.stride(0) if seqs > 1 else NH * HD, k_stride=kc.stride(0) if pages > 1 else kc[0].numel(),
-                         v_stride=vc.stride(0) if pages > 1 else vc[0].numel(), table_stride=tables.stride(0), prefix_stride=prefix_tables.stride(0),
-                         seqs=seqs, groups=n_groups, NH=NH, NKV=NKV, HD=HD, pages=pages, table_width=tables.shape[1], prefix_width=prefix_tables.shape[1],
-                         scale=HD ** -0.5 if scale is None else float(scale))
+    if not kc.get_device() == vc.get_device() == out.get_device() == tables.get_device() == prefix_tables.get_device() == index:
+        same_device(q.device, kc=kc, vc=vc, out=out, tables=tables, prefix_tables=prefix_tables)
+    first = (C.c_int32 * (n_groups + 1))(0, *accumulate(sizes))
+    a = L.AttnSharedArgs(q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), tables.data_ptr(), lens.data_ptr(), prefix_tables.data_ptr(), prefix_lens.data_ptr(),
+                         C.addressof(first), status.data_ptr() if status is not None else None, None, 0,
+                         q.stride(0) if seqs > 1 else NH * HD, out.stride(0) if seqs > 1 else NH * HD, kc.stride(0) if pages > 1 else page, vc.stride(0) if pages > 1 else page,
+                         tables.stride(0), prefix_tables.stride(0), seqs, n_groups, NH, NKV, HD, pages, tables.shape[1], prefix_tables.shape[1],
+                         HD ** -0.5 if scale is None else float(scale), 0)
     lib, n, work = L.load(), C.c_size_t(), None
-    L.check(lib.etxb_attn_shared_work(q.device.index, C.byref(a), C.sizeof(a), C.byref(n)))
+    rc = lib.etxb_attn_shared_work(index, C.byref(a), _BYTES, C.byref(n))
+    if rc:
+        L.check(rc)
     if n.value:                                                  # of this call alone: torch keeps it from others until the stream has passed
         work = torch.empty(n.value, dtype=torch.uint8, device=q.device)
         a.work, a.work_bytes = work.data_ptr(), n.value
-    handle = stream_handle(q.device, stream, [q, out, kc, vc, tables, lens, prefix_tables, prefix_lens, status, work])
-    L.check(lib.etxb_attn_shared(q.device.index, C.byref(a), C.sizeof(a), C.c_void_p(handle)))
+    handle = stream_handle(index, stream, (q, out, kc, vc, tables, lens, prefix_tables, prefix_lens, status, work))
+    rc = lib.etxb_attn_shared(index, C.byref(a), _BYTES, handle)
+    if rc:
+        L.check(rc)
     return out
 
 

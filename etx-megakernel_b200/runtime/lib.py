@@ -19,7 +19,7 @@ HEADERS = ["etxb_abi.h", "etxb_prims.cuh", "etxb_gemv.cuh", "etxb_gemv_nb.cuh", 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-fmad=false",
               "-shared", "-Xcompiler", "-fPIC"]
 
-STATUS = {0: "OK", 1: "E_ARG", 2: "E_PLAN", 3: "E_CUDA", 4: "E_RESIDENCY", 5: "E_TIMEOUT", 6: "E_ABORTED", 7: "E_UNSUPPORTED"}
+STATUS = {0: "OK", 1: "E_ARG", 2: "E_PLAN", 3: "E_CUDA", 4: "E_RESIDENCY", 5: "E_TIMEOUT", 6: "E_ABORTED", 7: "E_UNSUPPORTED", 8: "E_FULL"}
 BODY = {"nop": 0, "prologue": 1, "argmax": 2, "gemv": 3, "moe_up": 4, "moe_down": 5, "topk": 6, "attnprep": 7, "attn": 8,
         "attn_reduce": 9, "splitk_part": 10, "splitk_sum": 11, "attn_fused": 12, "norm_col": 13, "gemv_nb": 14, "route": 15,
         "moe_up_g": 16, "moe_down_g": 17, "prologue_nb": 18, "argmax_nb": 19, "gemv_tc": 20, "moe_up_tc": 21, "moe_down_tc": 22, "mla_attn": 23}
@@ -29,7 +29,8 @@ SYMBOLS = ["etxb_version", "etxb_last_error", "etxb_device_info", "etxb_create",
            "etxb_launch", "etxb_launch_unfused", "etxb_wait", "etxb_step", "etxb_status", "etxb_trace", "etxb_exec_counts", "etxb_destroy",
            "etxb_decode_host", "etxb_op_launch", "etxb_attn_fused_static", "etxb_exchange_alloc", "etxb_exchange_free", "etxb_exchange_open",
            "etxb_exchange_close", "etxb_set_exchange", "etxb_sample", "etxb_pages_update",
-           "etxb_attn_shared", "etxb_attn_shared_work"]
+           "etxb_attn_shared", "etxb_attn_shared_work", "etxb_pool_create", "etxb_pool_destroy", "etxb_pool_open", "etxb_pool_extend",
+           "etxb_pool_fork", "etxb_pool_close", "etxb_pool_compact", "etxb_pool_row", "etxb_pool_free"]
 DTYPES = {"bf16": 0, "f16": 1, "f32": 2}
 IPC_HANDLE_BYTES = 64
 
@@ -72,6 +73,9 @@ class PagesArgs(C.Structure):
                 ("src_ids", C.c_void_p), ("dst_ids", C.c_void_p), ("tables", C.c_void_p), ("table_stride", C.c_int64)] + \
                [(n, C.c_void_p) for n in ("set_rows", "set_cols", "set_pages", "share_rows", "remap_rows", "remap_entries")] + \
                [(n, C.c_int32) for n in ("n_copy", "table_rows", "table_width", "n_set", "n_share", "share_from", "shared", "n_remap")]
+
+
+PAGES_FN = C.CFUNCTYPE(C.c_int32, C.c_int, C.POINTER(PagesArgs), C.c_size_t, C.c_void_p)
 
 
 class AttnSharedArgs(C.Structure):
@@ -148,6 +152,9 @@ def load():
         "etxb_exchange_open": [C.c_int, vp, C.POINTER(vp)], "etxb_exchange_close": [C.c_int, vp],
         "etxb_set_exchange": [vp, i32, i32, vp, sz, C.POINTER(vp)],
         "etxb_sample": [C.c_int, C.POINTER(SampleArgs), sz, vp], "etxb_pages_update": [C.c_int, C.POINTER(PagesArgs), sz, vp],
+        "etxb_pool_create": [C.c_int, C.POINTER(PagesArgs), sz, i32, vp, C.POINTER(vp)], "etxb_pool_destroy": [vp], "etxb_pool_open": [vp, i32, C.POINTER(i32), vp],
+        "etxb_pool_extend": [vp, vp, vp, i32, vp], "etxb_pool_fork": [vp, i32, i32, i32, vp, vp], "etxb_pool_close": [vp, vp, i32],
+        "etxb_pool_compact": [vp, C.POINTER(i32), vp], "etxb_pool_row": [vp, i32, C.POINTER(i32), vp, i32, C.POINTER(i32)], "etxb_pool_free": [vp, C.POINTER(i32)],
         "etxb_attn_shared": [C.c_int, C.POINTER(AttnSharedArgs), sz, vp], "etxb_attn_shared_work": [C.c_int, C.POINTER(AttnSharedArgs), sz, C.POINTER(sz)],
     }
     for name, args in proto.items():

@@ -1,4 +1,4 @@
-"""Pages of a paged KV cache: copied between pools, shared by forked sequences, moved together, given back (etxb_pages_update).
+"""Pages of a paged KV cache: copied between pools, shared by forked sequences, moved together, given back (etxb_pages_update, etxb_pool_*).
 
 The layout is the programs': keys [layers][pages][NKV][HD / 8][16][8], values [layers][pages][NKV][HD][16]; a page is 16 positions of every layer and
 tensor.  Nothing here looks inside a page, so any tensors [layers][pages][...] serve.  No counterpart in the reference, whose requests each own their
@@ -6,12 +6,14 @@ blocks (examples/vllm_llm/model.py:194-211)."""
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
-import numpy as np
 import torch
 
 from . import lib as L
 from ._call import cuda_tensor, same_device, stream_handle
+
+_BYTES = C.sizeof(L.PagesArgs)
 
 
 def _pool(name, tensors):
@@ -26,38 +28,39 @@ def _pool(name, tensors):
     return tensors
 
 
-def _ids(name, v, n=None):
-    a = np.ascontiguousarray(v, np.int32).reshape(-1)
-    if not np.array_equal(a, np.asarray(v).reshape(-1)) or (n is not None and a.size != n):
-        raise ValueError(f"{name}: {'whole numbers' if n is None else f'{n} whole numbers'}")
-    return a
-
-
-def _update(src, dst, src_ids=(), dst_ids=(), tables=None, sets=((), (), ()), share=((), 0, 0), remap=((), ()), stream=None):
-    a, keep = L.PagesArgs(), []
-
-    def lst(field, v):
-        v = _ids(field, v)
-        keep.append(v)
-        setattr(a, field, v.ctypes.data if v.size else None)
-        return v.size
+def _layout(src, dst):
+    a = L.PagesArgs()
     a.n_tensors, a.layers, a.src_pages, a.dst_pages = len(src), src[0].shape[0], src[0].shape[1], dst[0].shape[1]
     for i, (s, d) in enumerate(zip(src, dst)):
         z = s.element_size()
         a.t[i] = L.PageTensor(s.data_ptr(), d.data_ptr(), s.stride(0) * z, s.stride(1) * z, d.stride(0) * z, d.stride(1) * z, s[0, 0].numel() * z)
-    a.n_copy = lst("src_ids", src_ids)
-    if lst("dst_ids", dst_ids) != a.n_copy:
-        raise ValueError(f"{a.n_copy} pages to copy to {len(dst_ids)}")
-    if tables is not None:
-        a.tables, a.table_stride, a.table_rows, a.table_width = tables.data_ptr(), tables.stride(0), tables.shape[0], tables.shape[1]
-    a.n_set = lst("set_rows", sets[0])
-    lst("set_cols", sets[1]), lst("set_pages", sets[2])
-    a.n_share, a.share_from, a.shared = lst("share_rows", share[0]), share[1], share[2]
-    a.n_remap = lst("remap_rows", remap[0])
-    lst("remap_entries", remap[1])
-    dev = src[0].device
-    handle = stream_handle(dev, stream, [*src, *dst, tables])
-    L.check(L.load().etxb_pages_update(dev.index, C.byref(a), C.sizeof(a), C.c_void_p(handle)))
+    return a
+
+
+def _ints(name, v):
+    """`v` as a C array of 32-bit numbers (a number is one of them)."""
+    v = v.tolist() if hasattr(v, "tolist") else v
+    try:
+        out = array("i", v if isinstance(v, (list, tuple, range)) else (v,))
+    except (TypeError, OverflowError) as e:
+        raise ValueError(f"{name}: whole numbers of 32 bits") from e
+    return (C.c_int32 * len(out)).from_buffer(out)
+
+
+def _int(name, v):
+    """`v` as a 32-bit number (ctypes would cut a larger one)."""
+    return _ints(name, [v])[0]
+
+
+def _check(rc):
+    """What the library refuses is the caller's error; a pool without room is not."""
+    if rc:
+        try:
+            L.check(rc)
+        except L.EtxbError as e:
+            if e.status == "E_ARG":
+                raise ValueError(str(e)) from None
+            raise
 
 
 def copy_pages(src, dst, src_ids, dst_ids, stream=None) -> None:
@@ -67,7 +70,12 @@ def copy_pages(src, dst, src_ids, dst_ids, stream=None) -> None:
     if len(src) != len(dst) or src[0].shape[0] != dst[0].shape[0] or any(s.shape[2:] != d.shape[2:] or s.dtype != d.dtype for s, d in zip(src, dst)):
         raise ValueError("copy_pages: pools of the same tensors, layers and pages")
     same_device(src[0].device, dst=dst[0])
-    _update(src, dst, _ids("src_ids", src_ids), _ids("dst_ids", dst_ids), stream=stream)
+    a, ids, to = _layout(src, dst), _ints("src_ids", src_ids), _ints("dst_ids", dst_ids)
+    if len(ids) != len(to):
+        raise ValueError(f"copy_pages: {len(ids)} pages to copy to {len(to)}")
+    a.n_copy, a.src_ids, a.dst_ids = len(ids), C.addressof(ids), C.addressof(to)
+    index = src[0].get_device()
+    _check(L.load().etxb_pages_update(index, C.byref(a), _BYTES, stream_handle(index, stream, (*src, *dst))))
 
 
 class PagePool:
@@ -76,7 +84,8 @@ class PagePool:
     A sequence is a row of `tables` (int32 [max_seqs][max_pages] on the device: the block table its attention reads), with a length in positions.
     Forked sequences share the full pages of what they have in common; a page that is shared is never written, since only full pages are.  Pages are
     given out lowest first.  Which pages are whose is kept on the host; a call changes the tables and copies pages in one launch on its stream, so the
-    steps that read them follow on the same stream (or wait for it).  A call that fails changes nothing."""
+    steps that read them follow on the same stream (or wait for it).  A call that fails changes nothing: ValueError for what cannot be asked,
+    EtxbError (E_FULL) where pages or rows run out."""
 
     def __init__(self, tensors, max_seqs: int, max_pages: int, tables=None, page_len: int = 16):
         self.tensors = _pool("tensors", tensors)
@@ -87,130 +96,85 @@ class PagePool:
             tables = torch.zeros((max_seqs, max_pages), dtype=torch.int32, device=dev)
         self.tables = cuda_tensor("tables", tables, (torch.int32,), (max_seqs, max_pages))
         same_device(dev, tables=tables)
-        self.page_len, self.n_pages = page_len, self.tensors[0].shape[1]
-        self._users = np.zeros(self.n_pages, np.int32)          # sequences that hold a page
-        self._pages = [None] * max_seqs                         # row -> its pages in order
-        self._length = [0] * max_seqs
+        self.page_len, self.n_pages, self._index = page_len, self.tensors[0].shape[1], self.tensors[0].get_device()
+        a = _layout(self.tensors, self.tensors)
+        a.tables, a.table_stride, a.table_rows, a.table_width = tables.data_ptr(), max(tables.stride(0), max_pages), max_seqs, max_pages
+        self._lib, self._h = L.load(), C.c_void_p()
+        _check(self._lib.etxb_pool_create(self._index, C.byref(a), _BYTES, page_len, self._carrier(), C.byref(self._h)))
+
+    def _carrier(self):
+        return None                                             # (the library's own etxb_pages_update)
+
+    def __del__(self):
+        if getattr(self, "_h", None):
+            self._lib.etxb_pool_destroy(self._h)
+            self._h = None
+
+    def _stream(self, stream):
+        return stream_handle(self._index, stream, (*self.tensors, self.tables))
 
     # ---- what is where
     @property
     def free_pages(self) -> int:
-        return int((self._users == 0).sum())
+        n = C.c_int32()
+        _check(self._lib.etxb_pool_free(self._h, C.byref(n)))
+        return n.value
 
     def rows(self) -> list:
-        return [r for r, p in enumerate(self._pages) if p is not None]
+        n = C.c_int32()
+        out = []
+        for r in range(self.tables.shape[0]):
+            _check(self._lib.etxb_pool_row(self._h, r, C.byref(n), None, 0, None))
+            if n.value >= 0:
+                out.append(r)
+        return out
 
     def pages_of(self, row: int) -> list:
-        return self._row(row).tolist()
+        n, buf = C.c_int32(), (C.c_int32 * self.tables.shape[1])()
+        self.length_of(row)
+        _check(self._lib.etxb_pool_row(self._h, row, None, buf, len(buf), C.byref(n)))
+        return buf[:n.value]
 
     def length_of(self, row: int) -> int:
-        self._row(row)
-        return self._length[row]
-
-    def _row(self, row):
-        if not 0 <= row < len(self._pages) or self._pages[row] is None:
+        n = C.c_int32()
+        _check(self._lib.etxb_pool_row(self._h, _int("row", row), C.byref(n), None, 0, None))
+        if n.value < 0:
             raise ValueError(f"row {row} holds no sequence")
-        return self._pages[row]
-
-    def _need(self, length: int) -> int:
-        if length < 0:
-            raise ValueError(f"a length of {length} positions")
-        n = -(-length // self.page_len)
-        if n > self.tables.shape[1]:
-            raise ValueError(f"{length} positions take {n} pages, a table has {self.tables.shape[1]}")
-        return n
-
-    def _take(self, n: int) -> np.ndarray:
-        free = np.flatnonzero(self._users == 0)[:n]
-        if free.size < n:
-            raise RuntimeError(f"the pool has {free.size} free pages, {n} are needed")
-        return free.astype(np.int32)
-
-    def _free_rows(self, n: int) -> list:
-        out = [r for r, p in enumerate(self._pages) if p is None][:n]
-        if len(out) < n:
-            raise RuntimeError(f"{len(out)} free rows in the tables, {n} are needed")
-        return out
+        return n.value
 
     # ---- calls
     def open(self, length: int, stream=None) -> int:
         """A new sequence with pages for `length` positions; returns its row."""
-        n = self._need(length)
-        row, pages = self._free_rows(1)[0], self._take(n)
-        if n:
-            _update(self.tensors, self.tensors, tables=self.tables, sets=(np.full(n, row), np.arange(n), pages), stream=stream)
-        self._users[pages] += 1
-        self._pages[row], self._length[row] = pages, length
-        return row
+        row = C.c_int32()
+        _check(self._lib.etxb_pool_open(self._h, _int("length", length), C.byref(row), self._stream(stream)))
+        return row.value
 
     def extend(self, rows, length, stream=None) -> None:
         """Pages up to `length` positions (a number, or one per row) for each of `rows`; a length is never reduced."""
-        rows = [int(rows)] if np.ndim(rows) == 0 else [int(r) for r in rows]
-        lengths = [int(length)] * len(rows) if np.ndim(length) == 0 else [int(n) for n in length]
-        if len(lengths) != len(rows) or len(set(rows)) != len(rows):
-            raise ValueError("extend: each row once, with one length")
-        for r, n in zip(rows, lengths):
-            self._row(r)
-            if n < self._length[r]:
-                raise ValueError(f"row {r} has {self._length[r]} positions, not {n}")
-        more = [self._need(n) - self._pages[r].size for r, n in zip(rows, lengths)]
-        new = self._take(sum(more))
-        if new.size:
-            cols = np.concatenate([np.arange(self._pages[r].size, self._pages[r].size + m) for r, m in zip(rows, more)])
-            _update(self.tensors, self.tensors, tables=self.tables, sets=(np.repeat(rows, more), cols, new), stream=stream)
-        self._users[new] += 1
-        at = 0
-        for r, m, n in zip(rows, more, lengths):
-            if m:
-                self._pages[r] = np.concatenate([self._pages[r], new[at:at + m]])
-                at += m
-            self._length[r] = n
+        rows = _ints("rows", rows)
+        lengths = _ints("length", [length] * len(rows) if isinstance(length, int) else length)
+        if len(lengths) != len(rows):
+            raise ValueError("extend: each row with one length")
+        _check(self._lib.etxb_pool_extend(self._h, rows, lengths, len(rows), self._stream(stream)))
 
     def fork(self, row: int, n: int, length: int | None = None, stream=None) -> list:
         """n new sequences that continue `row` from `length` positions on (None: all of it): the full pages are shared, the last, partly filled one is
         copied for each.  Returns their rows."""
-        pages = self._row(row)
-        length = self._length[row] if length is None else int(length)
-        if not 0 <= length <= self._length[row] or n < 0:
-            raise ValueError(f"fork: {n} sequences from {length} positions of {self._length[row]}")
-        full, part = divmod(length, self.page_len)
-        rows, new = self._free_rows(n), self._take(n if part else 0)
-        if n and (full or part):
-            sets = (rows, np.full(n, full), new) if part else ((), (), ())
-            _update(self.tensors, self.tensors, np.repeat(pages[full], n) if part else (), new, self.tables, sets, (rows, row, full), stream=stream)
-        self._users[pages[:full]] += n
-        self._users[new] += 1
-        for i, r in enumerate(rows):
-            self._pages[r] = np.concatenate([pages[:full], new[i:i + 1]]) if part else pages[:full].copy()
-            self._length[r] = length
-        return rows
+        if length is not None and length < 0:
+            raise ValueError(f"fork: from {length} positions")
+        row, n, length = _int("row", row), _int("n", n), -1 if length is None else _int("length", length)
+        rows = (C.c_int32 * max(n, 0))()
+        _check(self._lib.etxb_pool_fork(self._h, row, n, length, rows, self._stream(stream)))
+        return list(rows)
 
     def close(self, rows) -> None:
         """The sequences end: pages that nobody else holds are free again (their contents and the rows' entries stay as they are)."""
-        rows = [int(rows)] if np.ndim(rows) == 0 else [int(r) for r in rows]
-        if len(set(rows)) != len(rows):
-            raise ValueError("close: each row once")
-        for r in rows:
-            self._row(r)
-        for r in rows:
-            self._users[self._pages[r]] -= 1
-            self._pages[r], self._length[r] = None, 0
+        rows = _ints("rows", rows)
+        _check(self._lib.etxb_pool_close(self._h, rows, len(rows)))
 
     def compact(self, stream=None) -> int:
         """Moves pages until the ones in use are the lowest: the highest into the lowest hole, and so on.  Returns how many moved; the pool's pages from
         `n_pages - free_pages` on are then free."""
-        used = np.flatnonzero(self._users)
-        n = used.size
-        high = used[used >= n][::-1]
-        if high.size == 0:
-            return 0
-        low = np.flatnonzero(self._users[:n] == 0)
-        rows = [r for r in self.rows() if self._pages[r].size]
-        _update(self.tensors, self.tensors, high, low, self.tables, remap=(rows, [self._pages[r].size for r in rows]), stream=stream)
-        to = np.arange(self.n_pages, dtype=np.int32)
-        to[high] = low
-        self._users[low] = self._users[high]
-        self._users[high] = 0
-        for r in rows:
-            self._pages[r] = to[self._pages[r]]
-        return int(high.size)
+        moved = C.c_int32()
+        _check(self._lib.etxb_pool_compact(self._h, C.byref(moved), self._stream(stream)))
+        return moved.value

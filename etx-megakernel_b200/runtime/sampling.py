@@ -10,10 +10,11 @@ from typing import NamedTuple
 import torch
 
 from . import lib as L
-from ._call import cuda_tensor, same_device, stream_handle
+from ._call import cuda_tensor, stream_handle, vector
 
 _DT = {torch.bfloat16: L.DTYPES["bf16"], torch.float16: L.DTYPES["f16"], torch.float32: L.DTYPES["f32"]}
 MAX_V = 524288
+_BYTES = C.sizeof(L.SampleArgs)
 
 
 class Sampled(NamedTuple):
@@ -46,34 +47,36 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=Non
 
     temperature, top_k, top_p, min_p: numbers, or tensors [rows] (float32; top_k int32).  tokens / next_tokens: int32 tensors [rows] that take the tokens
     (the second one them once more: the next step's input).  stream: a raw handle or torch stream; None is the current one."""
-    cuda_tensor("logits", logits, tuple(_DT), (None, None))
+    cuda_tensor("logits", logits, _DT, (None, None))
     rows, V = logits.shape
     if not 1 <= V <= MAX_V:
         raise ValueError(f"logits: {V} tokens outside 1..{MAX_V}")
-    if rows > 1 and logits.stride(0) < V:
-        raise ValueError(f"logits: rows overlap (stride {logits.stride(0)} below {V})")
-    dev = logits.device
-    cuda_tensor("u", u, (torch.float32,), (rows,))
-    a = L.SampleArgs(logits=logits.data_ptr(), u=u.data_ptr(), row_stride=max(logits.stride(0), V) if rows > 1 else V, rows=rows, V=V, dtype=_DT[logits.dtype])
+    stride = logits.stride(0) if rows > 1 else V
+    if stride < V:
+        raise ValueError(f"logits: rows overlap (stride {stride} below {V})")
+    index = logits.get_device()
+    vector("u", u, torch.float32, rows, index)
+    a = L.SampleArgs()
+    a.logits, a.u, a.row_stride, a.rows, a.V, a.dtype = logits.data_ptr(), u.data_ptr(), stride, rows, V, _DT[logits.dtype]
     keep = [logits, u]
-    for name, v, dt, cast in (("temperature", temperature, torch.float32, float), ("top_k", top_k, torch.int32, int), ("top_p", top_p, torch.float32, float),
-                              ("min_p", min_p, torch.float32, float)):
+    for name, v in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("top_k", top_k)):
         if isinstance(v, torch.Tensor):
-            cuda_tensor(name, v, (dt,), (rows,))
-            setattr(a, name, v.data_ptr())
+            setattr(a, name, vector(name, v, torch.int32 if name == "top_k" else torch.float32, rows, index).data_ptr())
             keep.append(v)
         else:
-            setattr(a, name + "_all", min(cast(v), MAX_V) if cast is int else cast(v))
-    same_device(dev, u=u, **{f"setting {i}": t for i, t in enumerate(keep[2:])})
+            setattr(a, name + "_all", min(int(v), MAX_V) if name == "top_k" else float(v))
     for name, t in (("tokens", tokens), ("next_tokens", next_tokens)):
         if t is not None:
-            cuda_tensor(name, t, (torch.int32,), (rows,))
-            same_device(dev, **{name: t})
+            vector(name, t, torch.int32, rows, index)
+    dev = logits.device
     if tokens is None:
         tokens = torch.empty(rows, dtype=torch.int32, device=dev)
     logprobs, kept = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.int32, device=dev)
     a.tokens, a.logprobs, a.kept = tokens.data_ptr(), logprobs.data_ptr(), kept.data_ptr()
-    a.next = next_tokens.data_ptr() if next_tokens is not None else None
-    handle = stream_handle(dev, stream, keep + [tokens, next_tokens, logprobs, kept])
-    L.check(L.load().etxb_sample(dev.index, C.byref(a), C.sizeof(a), C.c_void_p(handle)))
+    if next_tokens is not None:
+        a.next = next_tokens.data_ptr()
+    handle = stream_handle(index, stream, (*keep, tokens, next_tokens, logprobs, kept))
+    rc = L.load().etxb_sample(index, C.byref(a), _BYTES, handle)
+    if rc:
+        L.check(rc)
     return Sampled(tokens, logprobs, kept)

@@ -40,7 +40,8 @@ enum {
   ETXB_E_RESIDENCY = 4,  /* the persistent grid cannot be co-resident on this device */
   ETXB_E_TIMEOUT = 5,    /* a device wait ran past its deadline; the kernel returned, the context is usable */
   ETXB_E_ABORTED = 6,    /* host abort requested */
-  ETXB_E_UNSUPPORTED = 7 /* shape outside what the tile supports (message says which) */
+  ETXB_E_UNSUPPORTED = 7,/* shape outside what the tile supports (message says which) */
+  ETXB_E_FULL = 8        /* a pool has no room: nothing was changed */
 };
 
 /* tile bodies (the `body` field of a plan's task type; the symbol names a graph links are mapped to these) */
@@ -259,6 +260,31 @@ typedef struct etxb_pages_args {
   int32_t n_copy, table_rows, table_width, n_set, n_share, share_from, shared, n_remap;
 } etxb_pages_args;
 int32_t etxb_pages_update(int device, const etxb_pages_args* args, size_t bytes, void* cuda_stream);
+
+/* A pool: which pages are whose.  A sequence is a row of the tables with a length in positions; its pages are given out lowest first.  Forked sequences
+ * share the full pages of what they have in common, and the last, partly filled one is copied for each; a shared page is never written, since only full
+ * pages are shared.  The books are the host's; what changes on the device (tables, copied pages) goes through one etxb_pages_update on the call's stream.
+ * A call that fails changes nothing (ETXB_E_ARG; ETXB_E_FULL: no free pages or rows).  Calls on one pool exclude one another.
+ *   create   `layout`: t[].dst and its strides, n_tensors, layers, dst_pages, tables, table_stride, table_rows, table_width (the rest is ignored).
+ *            update: what carries the changes out, null: etxb_pages_update (a host without the device gives its own)
+ *   open     a new sequence with pages for `length` positions
+ *   extend   pages up to lengths[i] positions for rows[i] (never fewer than it has; each row once)
+ *   fork     n sequences that continue `row` from `length` positions on (-1: all of them); rows: [n], theirs
+ *   close    the sequences end: pages that nobody else holds are free (contents and table entries stay as they are)
+ *   compact  moves pages until the ones in use are the lowest, the highest into the lowest hole first; moved: how many, may be null
+ *   row      *length = -1 for a row without a sequence; pages: [capacity], its first pages; n: how many it has.  Pointers may be null
+ *   free     free pages */
+typedef struct etxb_pool etxb_pool;
+typedef int32_t (*etxb_pages_fn)(int device, const etxb_pages_args* args, size_t bytes, void* cuda_stream);
+int32_t etxb_pool_create(int device, const etxb_pages_args* layout, size_t bytes, int32_t page_len, etxb_pages_fn update, etxb_pool** out);
+int32_t etxb_pool_destroy(etxb_pool* pool);
+int32_t etxb_pool_open(etxb_pool* pool, int32_t length, int32_t* row, void* cuda_stream);
+int32_t etxb_pool_extend(etxb_pool* pool, const int32_t* rows, const int32_t* lengths, int32_t n, void* cuda_stream);
+int32_t etxb_pool_fork(etxb_pool* pool, int32_t row, int32_t n, int32_t length, int32_t* rows, void* cuda_stream);
+int32_t etxb_pool_close(etxb_pool* pool, const int32_t* rows, int32_t n);
+int32_t etxb_pool_compact(etxb_pool* pool, int32_t* moved, void* cuda_stream);
+int32_t etxb_pool_row(etxb_pool* pool, int32_t row, int32_t* length, int32_t* pages, int32_t capacity, int32_t* n);
+int32_t etxb_pool_free(etxb_pool* pool, int32_t* pages);
 
 /* Decode attention of one layer for sequences that share prefixes: group g has a block table and a length of the positions its sequences have in
  * common, each sequence a table and a length of its own ones behind them (the new position's key and value are in the cache already, and counted).

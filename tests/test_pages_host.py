@@ -72,36 +72,57 @@ def test_nothing_to_do_is_no_work():
     call(remap_rows=[1], remap_entries=[4])
 
 
-class Device:
-    """What etxb_pages_update does, on CPU tensors."""
+class HostPool(PagePool):
+    """A pool over CPU tensors: numpy does what etxb_pages_update does, behind the library's checks of the lists."""
 
-    def __init__(self, monkeypatch):
-        monkeypatch.setattr(pages, "cuda_tensor", lambda name, t, dt, shape=None, inner=True: t)
-        monkeypatch.setattr(pages, "_update", self.update)
+    def _carrier(self):
+        def update(device, args, nbytes, stream):
+            a = args.contents
+            lst = lambda p, n: np.ctypeslib.as_array(C.cast(p, C.POINTER(C.c_int32)), (n,)).copy() if n else np.zeros(0, np.int32)  # noqa: E731
+            src, dst = lst(a.src_ids, a.n_copy), lst(a.dst_ids, a.n_copy)
+            assert len(set(dst)) == len(dst) and not set(dst) & set(src) and nbytes == C.sizeof(lib.PagesArgs)
+            for t in self.tensors:
+                for x, y in zip(src, dst):
+                    t[:, int(y)] = t[:, int(x)]
+            for r in lst(a.share_rows, a.n_share):
+                self.tables[int(r), :a.shared] = self.tables[a.share_from, :a.shared]
+            for r, c, p in zip(lst(a.set_rows, a.n_set), lst(a.set_cols, a.n_set), lst(a.set_pages, a.n_set)):
+                self.tables[int(r), int(c)] = int(p)
+            to = dict(zip(src.tolist(), dst.tolist()))
+            for r, n in zip(lst(a.remap_rows, a.n_remap), lst(a.remap_entries, a.n_remap)):
+                for c in range(n):
+                    self.tables[int(r), c] = to.get(int(self.tables[int(r), c]), int(self.tables[int(r), c]))
+            self.calls = getattr(self, "calls", 0) + 1
+            return getattr(self, "answer", 0)
+        self._fn = lib.PAGES_FN(update)
+        return C.cast(self._fn, C.c_void_p)
 
-    def update(self, src, dst, src_ids=(), dst_ids=(), tables=None, sets=((), (), ()), share=((), 0, 0), remap=((), ()), stream=None):
-        assert len(set(map(int, dst_ids))) == len(dst_ids) and not set(map(int, dst_ids)) & set(map(int, src_ids))
-        for s, d in zip(src, dst):
-            for a, b in zip(src_ids, dst_ids):
-                d[:, int(b)] = s[:, int(a)]
-        for r in share[0]:
-            tables[r, :share[2]] = tables[share[1], :share[2]]
-        for r, c, p in zip(*sets):
-            tables[int(r), int(c)] = int(p)
-        to = {int(a): int(b) for a, b in zip(src_ids, dst_ids)}
-        for r, n in zip(*remap):
-            for c in range(n):
-                tables[r, c] = to.get(int(tables[r, c]), int(tables[r, c]))
+    def _stream(self, stream):
+        return None
+
+
+@pytest.fixture
+def on_host(monkeypatch):
+    import __graft_entry__ as ge
+    ge.build()
+    monkeypatch.setattr(pages, "cuda_tensor", lambda name, t, dt, shape=None, inner=True: t)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+
+
+def users(pool):
+    held = np.zeros(pool.n_pages, int)
+    for r in pool.rows():
+        held[pool.pages_of(r)] += 1
+    return held
 
 
 @pytest.mark.parametrize("seed", range(6))
-def test_pool_over_random_lives(monkeypatch, seed):
+def test_pool_over_random_lives(on_host, seed):
     """Every sequence keeps reading its own positions through its table whatever else happens: positions are written as (sequence, position) marks."""
-    Device(monkeypatch)
     rng = random.Random(seed)
     P, N, ROWS, WIDTH = 4, 60, 9, 12
     t = torch.zeros((1, N, P), dtype=torch.int64)
-    pool = PagePool([t], ROWS, WIDTH, page_len=P)
+    pool = HostPool([t], ROWS, WIDTH, page_len=P)
     want, stamp = {}, 0
 
     def write(row, i0, i1):
@@ -109,12 +130,12 @@ def test_pool_over_random_lives(monkeypatch, seed):
         for i in range(i0, i1):
             stamp += 1
             page = int(pool.tables[row, i // P])
-            assert pool._users[page] == 1                          # a shared page is never written
+            assert users(pool)[page] == 1                          # a shared page is never written
             t[0, page, i % P] = stamp
             want[row].append(stamp)
     for _ in range(300):
         op, rows = rng.choice(["open", "fork", "extend", "extend", "close", "compact"]), pool.rows()
-        before = (pool._users.copy(), [None if p is None else p.copy() for p in pool._pages], list(pool._length), pool.tables.clone())
+        before = ([(r, pool.pages_of(r), pool.length_of(r)) for r in rows], pool.tables.clone(), t.clone())
         try:
             if op == "open":
                 r = pool.open(rng.randint(0, 20))
@@ -138,25 +159,22 @@ def test_pool_over_random_lives(monkeypatch, seed):
                     del want[r]
             elif op == "compact":
                 pool.compact()
-                assert pool._users[:N - pool.free_pages].all()
+                assert users(pool)[:N - pool.free_pages].all()
         except (RuntimeError, ValueError):                         # no room: nothing has changed
-            assert np.array_equal(before[0], pool._users) and before[2] == pool._length and torch.equal(before[3], pool.tables)
+            assert before[0] == [(r, pool.pages_of(r), pool.length_of(r)) for r in pool.rows()] and torch.equal(before[1], pool.tables) and torch.equal(before[2], t)
         for r in pool.rows():
             assert pool.pages_of(r) == pool.tables[r, :len(pool.pages_of(r))].tolist()
             assert [int(t[0, pool.tables[r, i // P], i % P]) for i in range(pool.length_of(r))] == want[r]
-        held = np.zeros(N, int)
-        for r in pool.rows():
-            held[pool.pages_of(r)] += 1
-        assert np.array_equal(held, pool._users)
+        assert int((users(pool) == 0).sum()) == pool.free_pages
 
 
-def test_pool_refusals(monkeypatch):
-    Device(monkeypatch)
-    pool = PagePool([torch.zeros((1, 6, 4))], 3, 4, page_len=4)
+def test_pool_refusals(on_host):
+    pool = HostPool([torch.zeros((1, 6, 4))], 3, 4, page_len=4)
     r = pool.open(7)
     for f, text in ((lambda: pool.open(17), "a table has 4"), (lambda: pool.open(-1), "length"), (lambda: pool.extend(r, 6), "not 6"), (lambda: pool.extend([r, r], 9), "once"),
                     (lambda: pool.extend(2, 9), "no sequence"), (lambda: pool.fork(r, 1, 8), "of 7"), (lambda: pool.fork(r, -1), "fork"), (lambda: pool.close([r, r]), "once"),
-                    (lambda: pool.close(1), "no sequence"), (lambda: pool.pages_of(-1), "no sequence"), (lambda: pool.extend([r], [8, 9]), "one length")):
+                    (lambda: pool.close(1), "no sequence"), (lambda: pool.pages_of(-1), "row -1 of 3"), (lambda: pool.open(2 ** 32 + 4), "32 bits"), (lambda: pool.fork(r, 2 ** 32), "32 bits"), (lambda: pool.extend([r], [8, 9]), "one length"), (lambda: pool.extend([r], 2 ** 40), "32 bits"),
+                    (lambda: pool.close(0.5), "whole"), (lambda: pool.length_of(3), "row 3 of 3"), (lambda: pool.fork(r, 1, -1), "from -1")):
         with pytest.raises(ValueError, match=text):
             f()
     with pytest.raises(RuntimeError, match="free rows"):
@@ -165,6 +183,39 @@ def test_pool_refusals(monkeypatch):
     with pytest.raises(RuntimeError, match="free pages"):
         pool.extend(r, 16)
     assert pool.length_of(r) == 7
+
+
+def test_what_cannot_be_carried_out_changes_nothing(on_host):
+    """The device refuses (a status that is not 0): the books stay as they were."""
+    pool = HostPool([torch.zeros((1, 9, 4))], 4, 4, page_len=4)
+    r = pool.open(7)
+    other = pool.open(3)
+    pool.close(r)
+    pool.answer = 3
+    state = (pool.rows(), pool.pages_of(other), pool.free_pages)
+    for f in (lambda: pool.open(5), lambda: pool.extend(other, 9), lambda: pool.fork(other, 2), lambda: pool.compact()):
+        with pytest.raises(lib.EtxbError):
+            f()
+        assert (pool.rows(), pool.pages_of(other), pool.free_pages) == state and pool.length_of(other) == 3
+    pool.answer = 0
+    assert pool.compact() == 1 and pool.pages_of(other) == [0]
+
+
+def test_pool_library_refusals():
+    import __graft_entry__ as ge
+    ge.build()
+    h, a = C.c_void_p(), lib.PagesArgs(dst_pages=4, table_rows=2, table_width=2)
+    fn = lib.load()
+    for args in ((0, None, 0, 16), (0, C.byref(a), 8, 16), (0, C.byref(a), C.sizeof(a), 0), (64, C.byref(a), C.sizeof(a), 16), (-1, C.byref(a), C.sizeof(a), 16)):
+        assert fn.etxb_pool_create(*args, None, C.byref(h)) == 1
+    assert fn.etxb_pool_create(0, C.byref(a), C.sizeof(a), 16, None, None) == 1
+    n = C.c_int32()
+    assert fn.etxb_pool_open(None, 1, C.byref(n), None) == 1 and fn.etxb_pool_free(None, C.byref(n)) == 1 and fn.etxb_pool_destroy(None) == 0
+    assert fn.etxb_pool_create(0, C.byref(a), C.sizeof(a), 16, None, C.byref(h)) == 0
+    assert fn.etxb_pool_open(h, 1, None, None) == 1 and fn.etxb_pool_extend(h, None, None, 1, None) == 1 and fn.etxb_pool_close(h, None, 1) == 1
+    assert fn.etxb_pool_fork(h, 0, 1, -1, None, None) == 1 and fn.etxb_pool_row(h, 0, None, None, -1, None) == 1 and fn.etxb_pool_free(h, None) == 1
+    assert fn.etxb_pool_open(h, 0, C.byref(n), None) == 0 and fn.etxb_pool_open(h, 2 ** 31 - 1, C.byref(n), None) == 1
+    assert fn.etxb_pool_destroy(h) == 0
 
 
 def test_host_tensors_are_refused():

@@ -192,6 +192,10 @@ static int32_t check_batch_block(int body, const unsigned char* blk, size_t byte
     if (bytes < sizeof(etxb::etxb_batch_args)) return fail(ETXB_E_ARG, "per-column prologue / argmax: the argument block is 32 bytes");
     etxb::etxb_batch_args a;
     memcpy(&a, blk, sizeof a);
+    if (body == ETXB_BODY_PROLOGUE_NB && (a.nb & ETXB_COLS_TABLES)) {
+      if (!a.tables || a.slot_span < 16 || a.slot_span % 16) return fail(ETXB_E_UNSUPPORTED, "per-column prologue over block tables: tables set, rows of slot_span / 16 entries");
+      a.nb &= ~ETXB_COLS_TABLES;
+    }
     if (a.nb < 1 || a.nb > 64 || a.slot_span < 0) return fail(ETXB_E_UNSUPPORTED, "per-column prologue / argmax: 1 <= nb <= 64 columns");
     return ETXB_OK;
   }

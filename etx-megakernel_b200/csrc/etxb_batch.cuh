@@ -253,17 +253,23 @@ __device__ __forceinline__ void tile_moe_down_g(const unsigned char* a, int blk,
 // ---------------------------------------------------------------------------------------------- per-column prologue
 // Columns of a batched step: token_in / token_out are [step][nb]; every column is at the step's position; column b owns
 // the cache slots [b * slot_span, (b + 1) * slot_span) of the shared block pool.
-// `zero`: not read (it named counters that the first column's task cleared; no tile counts arrivals any more).
-struct etxb_batch_args { int32_t nb, slot_span; int32_t* zero; uint32_t grid[3], nblocks; };
+// With ETXB_COLS_TABLES in nb the pages are the ones that block tables name, [nb][slot_span / 16], and the slots go to slot_mapping[1 + b]: the
+// attention tile takes a sequence whose slot address is the step's own slot_mapping for one whose slots are its positions.
+// (`tables` is read with that bit alone.)
+#define ETXB_COLS_TABLES 0x100
+struct etxb_batch_args { int32_t nb, slot_span; const int32_t* tables; uint32_t grid[3], nblocks; };
 __device__ __forceinline__ void tile_prologue_nb(const unsigned char* a, int b, const etxb_stepv& S) {
   const etxb_batch_args& d = *(const etxb_batch_args*)a;
-  if (b >= d.nb) return;
+  const int nb = d.nb & (ETXB_COLS_TABLES - 1);
+  if (b >= nb) return;
   const int t = S.tok;
   if (tidx() == 0) {
     if (S.token_time && b == 0) S.token_time[2 * t] = globaltimer();
-    S.positions[b] = S.pos; S.seq_lens[b] = S.pos + 1; S.slot_mapping[b] = (long long)b * d.slot_span + S.pos;
+    S.positions[b] = S.pos; S.seq_lens[b] = S.pos + 1;
+    if (d.nb & ETXB_COLS_TABLES) S.slot_mapping[1 + b] = (long long)__ldcg(d.tables + (size_t)b * (d.slot_span >> 4) + (S.pos >> 4)) * 16 + (S.pos & 15);
+    else S.slot_mapping[b] = (long long)b * d.slot_span + S.pos;
   }
-  const int id = __ldcg(S.token_in + (size_t)t * d.nb + b);
+  const int id = __ldcg(S.token_in + (size_t)t * nb + b);
   const uint4* src = (const uint4*)((const __nv_bfloat16*)S.embed + (size_t)id * S.H);
   uint4* dst = (uint4*)((__nv_bfloat16*)S.resid + (size_t)b * S.H);
   for (int i = tidx(); i < S.H / 8; i += ETXB_CONSUMERS) dst[i] = __ldg(src + i);

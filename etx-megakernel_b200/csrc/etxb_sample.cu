@@ -47,7 +47,7 @@ __device__ __forceinline__ Settings settings(const etxb_sample_args& a, int row)
 }
 __device__ __forceinline__ void store(const etxb_sample_args& a, int row, int token, float logp, int kept) {
   a.tokens[row] = token;
-  if (a.next) a.next[row] = token;
+  if (a.next) a.next[row] = max(token, 0);                        // (a token there is: the next step looks it up)
   if (a.logprobs) a.logprobs[row] = logp;
   if (a.kept) a.kept[row] = kept;
 }

@@ -131,6 +131,7 @@ ARGUMENTS.update({
     "route": [("ptr", "rlog"), ("ptr", "tw"), ("ptr", "ti"), ("ptr", "ecount"), ("ptr", "elist"), ("ptr", "active + layer"), ("i32", "E"), ("i32", "TOPK"),
               ("i32", "norm_topk | 0x100"), ("i32", "B"), ("i32", "B")],
     "cols": [("i32", "B"), ("i32", "nblk * BS")],
+    "cols_paged": [("i32", "B | 0x100"), ("i32", "nblk * BS"), ("ptr", "block_tables")],
 })
 
 
@@ -154,6 +155,7 @@ OPERATORS.update({
     "moe_down_tc": _batch_op("moe_down_tc", "tile_moe_down_tc", ("E*tpe", "1", "1"), "as gemv_tc", ("weights", "activation", "expert_lists", "routing_weights"),
                              ("expert_output",)),
     "cols": _batch_op("cols", "tile_prologue_nb / tile_argmax", ("B", "1", "1"), "B <= 64", ("token_in", "embedding", "logits"), ("residual", "positions", "token_out")),
+    "cols_paged": _batch_op("cols_paged", "tile_prologue_nb", ("B", "1", "1"), "B <= 64", ("token_in", "embedding", "block_tables"), ("residual", "positions")),
 })
 
 

@@ -17,6 +17,8 @@ then final norm (B tasks) -> lm_head (batched) -> argmax (B tasks).  All sequenc
 """
 from __future__ import annotations
 
+from dataclasses import replace
+
 import numpy as np
 import torch
 
@@ -28,7 +30,8 @@ from ..ops import attn as op_attn
 from ..ops import batch as op_batch
 from ..ops import gemv as op_gemv
 from ..passes import PassOptions, compile_graph
-from ..runtime import Session
+from ..runtime import PagePool, Session, copy_pages, sample
+from . import drawing
 from . import qwen as Q
 from .qwen import BS, SRC, X, ArgPool
 
@@ -36,10 +39,16 @@ _DT = {"bf16": torch.bfloat16, "f32": torch.float32, "i32": torch.int32, "i64": 
 UP_ROWS, DOWN_ROWS = 256, 512      # mma.sync engine: rows of one expert a gate+up / down task covers (blocks of 128 inside the tile)
 
 
-def buffer_shapes(d: Q.Dims, B: int, maxlen: int, steps: int, parts: int) -> dict:
+def buffer_shapes(d: Q.Dims, B: int, maxlen: int, steps: int, parts: int, pages: int | None = None) -> dict:
     """name -> (shape, dtype) of the activation / runtime buffers of B sequences (column b of every [B, ...] buffer
-    belongs to sequence b; the KV block pool gives sequence b the blocks [b * nblk, (b + 1) * nblk))."""
+    belongs to sequence b; the KV block pool gives sequence b the blocks [b * nblk, (b + 1) * nblk)).  pages: a pool of so many pages that the
+    sequences hold as their block tables say, and one more that columns without a sequence write to."""
     nblk = -(-maxlen // BS)
+    if pages is not None:
+        out = buffer_shapes(d, B, maxlen, steps, parts)
+        out["kc"], out["vc"] = [((d.L, pages + 1, *s[2:]), dt) for s, dt in (out["kc"], out["vc"])]
+        out["slot_mapping"] = ((B + 1,), "i64")
+        return out
     return {"resid": ((B, d.H), "bf16"), "resid2": ((B, d.H), "bf16"), "hn": ((B, d.H), "bf16"), "qkv": ((B, d.NQKV), "bf16"),
             "attn_out": ((B, d.NH * d.HD), "bf16"), "o": ((B, d.H), "bf16"), "o_norm": ((B, d.H), "bf16"), "logits": ((B, d.V), "bf16"),
             "positions": ((B,), "i64"), "seq_lens": ((B,), "i32"), "slot_mapping": ((B,), "i64"), "block_tables": ((B, nblk), "i32"),
@@ -52,13 +61,14 @@ def buffer_shapes(d: Q.Dims, B: int, maxlen: int, steps: int, parts: int) -> dic
             "skp": ((32,), "f32"), "skc": ((32,), "i32")}                       # named by the blocks of shared row blocks, not read (ops/batch.py)
 
 
-def build_graph(d: Q.Dims, ptr, B: int, maxlen: int = 1072, machine: MachineModel | str = "b200", engine: str = "tc"):
+def build_graph(d: Q.Dims, ptr, B: int, maxlen: int = 1072, machine: MachineModel | str = "b200", engine: str = "tc", pages: int | None = None):
     """The batched decode step of `d` for B sequences as a Graph plus its argument pool.  ptr(name) -> device address of
     a buffer (buffer_shapes) or packed weight (models.qwen.weight_shapes).  Returns (graph, pool, info).
 
     engine: what multiplies the batched grids (dense projections, expert gate+up / down) -- "tc": tcgen05.mma with TMA tensor
     copies and accumulators in tensor memory (needs every K a multiple of 64); "mma": the mma.sync tiles that read their
-    weights straight from global memory.  Same grids, same argument blocks, same results up to fp32 summation order."""
+    weights straight from global memory.  Same grids, same argument blocks, same results up to fp32 summation order.
+    pages: the positions lie in the pages that the block tables name (see buffer_shapes), not in blocks of each sequence's own."""
     if engine not in ("tc", "mma"):
         raise ValueError("engine is 'tc' or 'mma'")
     if engine == "tc" and any(k % 64 for k in (d.H, d.NH * d.HD, d.MI)):
@@ -68,6 +78,8 @@ def build_graph(d: Q.Dims, ptr, B: int, maxlen: int = 1072, machine: MachineMode
     if d.HD != 128 or d.G not in (1, 2, 4, 8):
         raise ValueError("the batched step uses the grouped attention tile: head_dim 128 and 1, 2, 4 or 8 q heads per kv head")
     op_batch.check_batch(B, max(d.H, d.NH * d.HD))
+    if B > 1 and d.V % 8:
+        raise ValueError(f"the batched step reads rows of logits by 16 bytes: vocab {d.V} is no multiple of 8")
     m = load_machine(machine) if isinstance(machine, str) else machine
     ent = {}
     for mod in (op_gemv, op_attn, op_batch):
@@ -78,7 +90,7 @@ def build_graph(d: Q.Dims, ptr, B: int, maxlen: int = 1072, machine: MachineMode
     pool = ArgPool()
     res = Resource(threads=op_gemv.THREADS, vgpr=128, lds_bytes=0)
     nblk = -(-maxlen // BS)
-    kv_layer_bytes = B * nblk * d.NKV * d.HD * BS * 2
+    kv_layer_bytes = (B * nblk if pages is None else pages + 1) * d.NKV * d.HD * BS * 2
     W = m.workers()
     gq, plen, gparts = d.G, op_attn.GQ_PART, -(-maxlen // op_attn.GQ_PART)      # one task per (128 positions, kv head): K / V read once
     # enough sequences to fill three tenths of the workers: one task per (sequence, kv head) walks the whole context; else one per partition.
@@ -129,7 +141,8 @@ def build_graph(d: Q.Dims, ptr, B: int, maxlen: int = 1072, machine: MachineMode
         add(name, "etx_tile_gemv_nb", gb("gemv_nb", t, W=Wp, x=ptr(x), out=ptr(out), M=M, K=K, rpt=rpt, tpe=1, nb=B, sx=K, sout=M, wts=bias, mode=mode), (t,), t)
 
     cols = argblock.pack_named(ent["cols"], (B, 1, 1), nb=B, slot_span=nblk * BS)
-    add("prologue", "vl_prologue_nb", cols, (B,), B)
+    first = cols if pages is None else argblock.pack_named(ent["cols_paged"], (B, 1, 1), nb=B | op_batch.COLS_TABLES, slot_span=nblk * BS, tables=ptr("block_tables"))
+    add("prologue", "vl_prologue_nb", first, (B,), B)
     for L in range(d.L):
         Wl = lambda n, L=L: ptr(f"{L}.{n}")                                  # noqa: E731
         if L == 0:
@@ -143,7 +156,7 @@ def build_graph(d: Q.Dims, ptr, B: int, maxlen: int = 1072, machine: MachineMode
                 ent["attn_fused"], (ntask, 1, 1), qkv=ptr("qkv") + b * d.NQKV * 2, qw=Wl("qn") if d.qk_norm else 0, kw=Wl("kn") if d.qk_norm else 0,
                 cos_sin=ptr("cos_sin"), kc=ptr("kc") + L * kv_layer_bytes, vc=ptr("vc") + L * kv_layer_bytes,
                 block_tables=ptr("block_tables") + b * nblk * 4, seq_lens=ptr("seq_lens") + 4 * b, positions=ptr("positions") + 8 * b,
-                slot_mapping=ptr("slot_mapping") + 8 * b, exp_sums=ptr("exp_sums") + b * d.NH * gparts * 4, max_logits=ptr("max_logits") + b * d.NH * gparts * 4,
+                slot_mapping=ptr("slot_mapping") + 8 * (b + (pages is not None)), exp_sums=ptr("exp_sums") + b * d.NH * gparts * 4, max_logits=ptr("max_logits") + b * d.NH * gparts * 4,
                 tmp_out=ptr("tmp_out") + b * d.NH * gparts * op_attn.GQ_PARTIAL_FLOATS * 4, out=ptr("attn_out") + b * d.NH * d.HD * 2,
                 counters=ptr("attn_counters") + 4 * (L * B + b) * d.NH, scale=scale, eps=d.eps, NH=d.NH, NKV=d.NKV, HD=d.HD, BS=BS, X=X,
                 max_parts=gparts, gq=gq, part_len=op_attn.tagged_part_len(L, whole, lim=int(precise) if whole else op_attn.GQ_LIM))
@@ -180,11 +193,17 @@ def build_graph(d: Q.Dims, ptr, B: int, maxlen: int = 1072, machine: MachineMode
 
 
 class BatchProgram:
-    """B sequences decoded in lock step on one GPU: weights, per-sequence buffers and KV blocks, plan, session."""
+    """B sequences decoded in lock step on one GPU: weights, per-sequence buffers and KV blocks, plan, session.
+
+    pages: the KV cache is a pool of so many pages (`self.cache`, a runtime.PagePool whose rows are the columns) in place of maxlen positions for every
+    sequence: sequences hold what they need, and forked ones share the pages of what they have in common.  A column without a sequence runs along and
+    writes to a page of its own."""
 
     def __init__(self, dims: Q.Dims, weights: dict, batch: int, device: int = 0, maxlen: int = 1072, steps: int | None = None, machine="b200",
-                 engine: str = "tc"):
-        self.d, self.B, self.maxlen = dims, int(batch), maxlen
+                 engine: str = "tc", pages: int | None = None):
+        self.d, self.B, self.maxlen, self.pages = dims, int(batch), maxlen, pages
+        if pages is not None and pages < 1:
+            raise ValueError("pages: at least one")
         self.dev = torch.device("cuda", device)
         self.machine = load_machine(machine) if isinstance(machine, str) else machine
         self.steps = steps or maxlen
@@ -193,16 +212,21 @@ class BatchProgram:
             if k not in weights or tuple(weights[k].shape) != tuple(shp):
                 raise ValueError(f"weight {k}: expected shape {shp}, got {tuple(weights[k].shape) if k in weights else None}")
         parts = -(-maxlen // op_attn.GQ_PART)
-        self.buf = {n: torch.zeros(shape, dtype=_DT[dt], device=self.dev) for n, (shape, dt) in buffer_shapes(dims, self.B, maxlen, self.steps, parts).items()}
+        self.buf = {n: torch.zeros(shape, dtype=_DT[dt], device=self.dev) for n, (shape, dt) in buffer_shapes(dims, self.B, maxlen, self.steps, parts, pages).items()}
         nblk = self.buf["block_tables"].shape[1]
-        self.buf["block_tables"].copy_(torch.arange(self.B * nblk, dtype=torch.int32).view(self.B, nblk))
+        self.cache = None
+        if pages is None:
+            self.buf["block_tables"].copy_(torch.arange(self.B * nblk, dtype=torch.int32).view(self.B, nblk))
+        else:
+            self.buf["block_tables"].fill_(pages)
+            self.cache = PagePool([self.buf["kc"][:, :pages], self.buf["vc"][:, :pages]], self.B, nblk, tables=self.buf["block_tables"], page_len=BS)
 
         def ptr(name):
             t = self.buf.get(name)
             if t is None:
                 t = self.w[name]
             return t.data_ptr()
-        self.graph, self.pool, self.info = build_graph(dims, ptr, self.B, maxlen, self.machine, engine=engine)
+        self.graph, self.pool, self.info = build_graph(dims, ptr, self.B, maxlen, self.machine, engine=engine, pages=pages)
         pool = self.pool.bytes()
         self.plan = compile_graph(self.graph, self.machine, {"POOL": len(pool)}, options=PassOptions())
         self.session = Session(self.plan, {}, pool, device)
@@ -218,9 +242,11 @@ class BatchProgram:
         else:
             self.session.launch()
 
-    def generate(self, prompts, n_gen: int, sync_every: int = 32):
-        """prompts: [B][P] token ids (one length).  Feeds them position by position, then n_gen greedy tokens per sequence
-        (the next tokens never leave the device).  Returns [B][n_gen]."""
+    def generate(self, prompts, n_gen: int, sync_every: int = 32, sampling=None):
+        """prompts: [B][P] token ids (one length).  Feeds them position by position, then n_gen tokens per sequence
+        (the next tokens never leave the device).  Returns [B][n_gen].  sampling: None for greedy tokens, or a runtime.Sampling (numbers, or tensors
+        of one value per sequence) whose tokens are drawn on the device; their log-probabilities are left in self.logprobs, [n_gen][B].
+        A program over pages ends its sequences first and opens new ones."""
         prompts = np.asarray(prompts, np.int64)
         if prompts.shape[0] != self.B:
             raise ValueError(f"{prompts.shape[0]} prompts for a batch of {self.B}")
@@ -228,17 +254,108 @@ class BatchProgram:
         n = P + n_gen - 1
         if n + 2 > self.buf["token_in"].shape[0] or n > self.maxlen:
             raise ValueError("sequence longer than the session was sized for")
+        if self.cache is not None:
+            if self.B * -(-n // BS) > self.pages:
+                raise ValueError(f"{self.B} sequences of {n} positions in {self.pages} pages")
+            self.release(self.cache.rows())
+            for _ in range(self.B):
+                self.cache.open(n)
+        return self._run(prompts.T, 0, n_gen, sync_every, sampling)
+
+    def _run(self, fed, pos: int, n_gen: int, sync_every: int, sampling):
+        """fed: [P][B] tokens from position `pos` on, then n_gen tokens; [B][n_gen]."""
+        P = fed.shape[0]
+        n = P + n_gen - 1
         tin = torch.zeros_like(self.buf["token_in"])
-        tin[:P] = torch.from_numpy(prompts.T.copy()).to(torch.int32)
+        tin[:P] = torch.from_numpy(fed.copy()).to(torch.int32)
         self.buf["token_in"].copy_(tin)
         torch.cuda.synchronize(self.dev)
-        for t in range(n):
-            self.step(t, t, write_next=t + 1 >= P, wait=(t % sync_every == sync_every - 1) or t == n - 1)
+        if sampling is not None:
+            drawing.run(self, n, P - 1, pos, self.B, sampling, sync_every)
+        else:
+            for t in range(n):
+                self.step(t, pos + t, write_next=t + 1 >= P, wait=(t % sync_every == sync_every - 1) or t == n - 1)
         return self.buf["token_out"][P - 1:n].cpu().numpy().T
+
+    def _tokens(self, tokens, shape):
+        tokens = np.asarray(tokens, np.int64).reshape(shape)
+        if tokens.size and not 0 <= tokens.min() <= tokens.max() < self.d.V:
+            raise ValueError(f"tokens outside the vocabulary of {self.d.V}")
+        return tokens
+
+    # ---- sequences over pages
+    def _paged(self):
+        if self.cache is None:
+            raise ValueError("the program was built without pages")
+        return self.cache
+
+    def release(self, columns) -> None:
+        """The columns' sequences end; the columns write to a page of nobody's until new ones begin there."""
+        columns = [int(c) for c in columns]
+        self._paged().close(columns)
+        self._idle()
+
+    def _idle(self):
+        """Columns without a sequence name the page of nobody's (a closed row's entries stay as they were, and others may hold those pages by now)."""
+        idle = sorted(set(range(self.B)) - set(self.cache.rows()))
+        if idle:
+            self.buf["block_tables"][idle] = self.pages
+
+    def adopt(self, one, length: int) -> int:
+        """A new sequence with the first `length` positions of a one-sequence program's cache (models.decode.DecodeProgram of the same model on the same
+        GPU); returns its column."""
+        pool, d = self._paged(), one.d
+        if (d.L, d.NKV, d.HD) != (self.d.L, self.d.NKV, self.d.HD) or not 0 <= length <= one.maxlen or one.dev != self.dev:
+            raise ValueError(f"adopt: {length} positions of a cache of {d.L} layers, {d.NKV} kv heads of {d.HD}, {one.maxlen} positions on {one.dev}")
+        column = pool.open(length)
+        ids = pool.pages_of(column)
+        if ids:
+            copy_pages([one.buf["kc"], one.buf["vc"]], pool.tensors, list(range(len(ids))), ids)
+        return column
+
+    def fork(self, column: int, n: int) -> list:
+        """n new sequences that continue the column's: its full pages are shared, the last one is copied.  Returns their columns."""
+        return self._paged().fork(column, n)
+
+    def decode(self, tokens, pos: int, n_gen: int, sync_every: int = 32, sampling=None):
+        """Every column takes its token of `tokens` [B] at position `pos`, then n_gen tokens per column; [B][n_gen].  Sequences grow as far as the steps
+        reach; all have `pos` positions behind them (columns without a sequence run along)."""
+        pool, n = self._paged(), n_gen
+        if n + 2 > self.buf["token_in"].shape[0] or pos + n > self.maxlen or n_gen < 1:
+            raise ValueError("sequence longer than the session was sized for")
+        rows = pool.rows()
+        if any(pool.length_of(r) != pos for r in rows):
+            raise ValueError(f"decode: sequences of {[pool.length_of(r) for r in rows]} positions at position {pos}")
+        tokens = self._tokens(tokens, (1, self.B))
+        if sampling is not None:
+            drawing.check(self, n, self.B, sampling)                         # (before the sequences grow)
+        pool.extend(rows, pos + n)
+        self._idle()
+        return self._run(tokens, pos, n_gen, sync_every, sampling)
+
+    def answers(self, one, prompt, n_gen: int, sampling, sync_every: int = 32):
+        """B answers to one prompt: `one` (a DecodeProgram of the same weights) reads it, its cache is adopted and forked, and every column draws its own
+        tokens.  Returns [B][n_gen]; log-probabilities in self.logprobs, [n_gen][B]."""
+        one.generate(prompt, 1)
+        P = len(prompt)
+        self.release(self._paged().rows())
+        self.fork(self.adopt(one, P), self.B - 1)
+        u = sampling.numbers(n_gen, self.B, self.dev)
+        logits = one.buf["logits"].view(1, -1).expand(self.B, -1).contiguous()
+        first = sample(logits, u[0], sampling.temperature, sampling.top_k, sampling.top_p, sampling.min_p)
+        tokens = first.tokens.cpu().numpy()
+        if n_gen == 1:
+            self.logprobs = first.logprobs[None]
+            return tokens[:, None]
+        rest = self.decode(tokens, P, n_gen - 1, sync_every, replace(sampling, given=u[1:]))
+        self.logprobs = torch.cat([first.logprobs[None], self.logprobs])
+        return np.concatenate([tokens[:, None], rest], axis=1)
 
     def load_kv(self, layer: int, seq: int, K: np.ndarray, V: np.ndarray):
         """Pre-fill positions 0..ctx-1 of one layer of sequence `seq` from contiguous float32 (bf16-exact) [ctx][NKV][HD] arrays."""
         ctx, nkv, hd = K.shape
+        if self.cache is not None:
+            raise ValueError("load_kv: a program over pages takes its contexts from another one (adopt)")
         nblk = self.buf["block_tables"].shape[1]
         kc, vc = self.buf["kc"][layer], self.buf["vc"][layer]
         Kt = torch.from_numpy(np.ascontiguousarray(K)).to(self.dev).to(torch.bfloat16)

@@ -12,6 +12,7 @@ import torch
 from ..machine import load_machine
 from ..passes import PassOptions, compile_graph
 from ..runtime import ExchangeRegion, Session
+from . import drawing
 from . import qwen as Q
 
 _DT = {"bf16": torch.bfloat16, "f32": torch.float32, "i32": torch.int32, "i64": torch.int64}
@@ -136,9 +137,12 @@ class DecodeProgram:
         else:
             self.session.launch()
 
-    def generate(self, prompt, n_gen: int, start_pos: int = 0, sync_every: int = 64, unfused: bool = False):
-        """Feed `prompt` token by token (positions start_pos ...), then n_gen greedy tokens; the next token never leaves
-        the device.  Returns the n_gen generated ids (the argmax after the last prompt token is the first)."""
+    def generate(self, prompt, n_gen: int, start_pos: int = 0, sync_every: int = 64, unfused: bool = False, sampling=None):
+        """Feed `prompt` token by token (positions start_pos ...), then n_gen tokens; the next token never leaves the device.  Returns the n_gen
+        generated ids (the one after the last prompt token is the first).  sampling: None for greedy tokens, or a runtime.Sampling whose tokens are
+        drawn on the device (equal seeds give equal tokens; their log-probabilities are left in self.logprobs, [n_gen][1])."""
+        if sampling is not None and (unfused or self.ranks > 1):
+            raise ValueError("generate: tokens are drawn behind single launches of a model whose logits lie on one GPU")
         prompt = [int(x) for x in prompt]
         n = len(prompt) + n_gen - 1
         if n + 2 > self.buf["token_in"].numel() or start_pos + n > self.maxlen:
@@ -147,6 +151,9 @@ class DecodeProgram:
         tin[:len(prompt)] = torch.tensor(prompt, dtype=torch.int32)
         self.buf["token_in"].copy_(tin)
         torch.cuda.synchronize(self.dev)
+        if sampling is not None:
+            drawing.run(self, n, len(prompt) - 1, start_pos, 1, sampling, sync_every)
+            return self.buf["token_out"][len(prompt) - 1:n].cpu().numpy()
         for t in range(n):
             self.step(t, start_pos + t, write_next=t + 1 >= len(prompt), wait=(t % sync_every == sync_every - 1) or t == n - 1, unfused=unfused)
         return self.buf["token_out"][len(prompt) - 1:n].cpu().numpy()

@@ -40,6 +40,7 @@ from ..ops import gemv as op_gemv
 from ..ops import mla as op_mla
 from ..passes import PassOptions, compile_graph
 from ..runtime import Session
+from . import drawing
 from . import qwen as Q
 from .qwen import SRC, ArgPool
 
@@ -405,8 +406,9 @@ class MlaProgram:
         else:
             self.session.launch()
 
-    def generate(self, prompt, n_gen: int, start_pos: int = 0, sync_every: int = 64):
-        """Feed `prompt` token by token, then n_gen greedy tokens (the next token never leaves the device)."""
+    def generate(self, prompt, n_gen: int, start_pos: int = 0, sync_every: int = 64, sampling=None):
+        """Feed `prompt` token by token, then n_gen tokens (the next token never leaves the device).  sampling: None for greedy tokens, or a
+        runtime.Sampling whose tokens are drawn on the device (their log-probabilities are left in self.logprobs, [n_gen][1])."""
         prompt = [int(x) for x in prompt]
         n = len(prompt) + n_gen - 1
         if n + 2 > self.buf["token_in"].numel() or start_pos + n > self.maxlen:
@@ -415,6 +417,9 @@ class MlaProgram:
         tin[:len(prompt)] = torch.tensor(prompt, dtype=torch.int32)
         self.buf["token_in"].copy_(tin)
         torch.cuda.synchronize(self.dev)
+        if sampling is not None:
+            drawing.run(self, n, len(prompt) - 1, start_pos, 1, sampling, sync_every)
+            return self.buf["token_out"][len(prompt) - 1:n].cpu().numpy()
         for t in range(n):
             self.step(t, start_pos + t, write_next=t + 1 >= len(prompt), wait=(t % sync_every == sync_every - 1) or t == n - 1)
         return self.buf["token_out"][len(prompt) - 1:n].cpu().numpy()

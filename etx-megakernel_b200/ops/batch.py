@@ -35,6 +35,10 @@ ROUTE_PARAMS = [("logits", "ptr addrspace(1)", 0, 8), ("wts", "ptr addrspace(1)"
                 ("E", "i32", 48, 4), ("K", "i32", 52, 4), ("mode", "i32", 56, 4), ("nb", "i32", 60, 4), ("cap", "i32", 64, 4)]
 COLS_BYTES, COLS_GRID = 32, 16
 COLS_PARAMS = [("nb", "i32", 0, 4), ("slot_span", "i32", 4, 4), ("zero", "ptr addrspace(1)", 8, 8)]
+# the prologue over block tables: column b's position lies in page tables[b][pos / 16] (rows of slot_span / 16 entries), and its slot goes to
+# slot_mapping[1 + b]; nb carries COLS_TABLES
+COLS_TABLES = 0x100
+COLS_PAGED_PARAMS = [("nb", "i32", 0, 4), ("slot_span", "i32", 4, 4), ("tables", "ptr addrspace(1)", 8, 8)]
 TC_ROWS = 256               # weight rows one tcgen05 instruction takes (four TMA boxes of 64)
 XBYTES = 40960              # shared memory for the token vectors of a pass: min(8, XBYTES // (2 K + 64)) columns per pass
 GROUP_ROWS = 128            # weight rows a block of the tensor-core loop covers
@@ -48,6 +52,7 @@ def import_entries(threads: int = 544) -> dict:
                            ("gemv_tc", "bf16 GEMV, up to 32 columns per weight read (tcgen05.mma, TMA, tensor memory)"),
                            ("moe_up_tc", "expert-grouped gate+up on tcgen05"), ("moe_down_tc", "expert-grouped down on tcgen05"))}
     out["route"] = entry("route", "route", ROUTE_PARAMS, ROUTE_BYTES, ROUTE_GRID, threads, "softmax top-k per column + per-expert token lists")
+    out["cols_paged"] = entry("cols_paged", "cols_paged", COLS_PAGED_PARAMS, COLS_BYTES, COLS_GRID, threads, "per-column prologue of a batched step over block tables")
     out["cols"] = entry("cols", "cols", COLS_PARAMS, COLS_BYTES, COLS_GRID, threads, "per-column prologue / argmax of a batched step")
     return out
 

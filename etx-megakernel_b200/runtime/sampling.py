@@ -31,9 +31,14 @@ class Sampling:
     top_p: object = 1.0
     min_p: object = 0.0
     seed: int = 0
+    given: torch.Tensor | None = None      # the random numbers themselves, float32 [steps][rows], in place of the seed's
 
     def numbers(self, steps: int, rows: int, device) -> torch.Tensor:
         """The random numbers of a run: [steps][rows] in [0, 1)."""
+        if self.given is not None:
+            if tuple(self.given.shape) != (steps, rows):
+                raise ValueError(f"given random numbers {tuple(self.given.shape)}, the run takes {(steps, rows)}")
+            return self.given
         return torch.rand((steps, rows), device=device, generator=torch.Generator(device=device).manual_seed(self.seed))
 
 
@@ -46,7 +51,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=Non
     with itself exceeds u times the sum of the kept ones.  temperature 0: the largest logit.  Equal inputs give equal tokens, whatever else runs.
 
     temperature, top_k, top_p, min_p: numbers, or tensors [rows] (float32; top_k int32).  tokens / next_tokens: int32 tensors [rows] that take the tokens
-    (the second one them once more: the next step's input).  stream: a raw handle or torch stream; None is the current one."""
+    (the second one them once more, 0 where there is none: the next step's input).  stream: a raw handle or torch stream; None is the current one."""
     cuda_tensor("logits", logits, _DT, (None, None))
     rows, V = logits.shape
     if not 1 <= V <= MAX_V:

@@ -225,7 +225,7 @@ typedef struct etxb_sample_args {
   const float* top_p;
   const float* min_p;
   int32_t* tokens;             /* [rows] */
-  int32_t* next;               /* [rows], the tokens once more (the next step's input), may be null */
+  int32_t* next;               /* [rows], the tokens once more, 0 for -1 (the next step's input), may be null */
   float* logprobs;             /* [rows] log-probability of the token among the kept ones, may be null */
   int32_t* kept;               /* [rows] number of tokens kept, may be null */
   int64_t row_stride;

@@ -158,6 +158,17 @@ def test_strides_offsets_and_streams(dtype):
         assert tok[[0, 8]].tolist() == [77, 77] and nxt[[0, 8]].tolist() == [78, 78]      # nothing behind the rows is touched
 
 
+@pytest.mark.parametrize("dtype", ALL)
+def test_the_next_input_is_a_token(dtype):
+    """A row without an allowed token gives -1; what goes to the next step, which looks it up, is 0."""
+    l = rows(3, 700, dtype, 21)
+    l[1] = float("nan")
+    nxt = torch.full((3,), 78, dtype=torch.int32, device=DEV)
+    r = sample(l, torch.full((3,), 0.5, device=DEV), next_tokens=nxt)
+    t = r.tokens.tolist()
+    assert t[1] == -1 and nxt.tolist() == [t[0], 0, t[2]]
+
+
 def test_captured_replayed_and_repeated():
     l = rows(5, 151936, torch.bfloat16, 8)
     u = torch.rand(5, device=DEV)

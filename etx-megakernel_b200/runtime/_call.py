@@ -4,7 +4,7 @@ from __future__ import annotations
 import torch
 
 _Tensor = torch.Tensor
-_raw_stream = torch._C._cuda_getCurrentRawStream
+raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def cuda_tensor(name: str, t, dtypes, shape=None, inner: bool = True):
@@ -37,7 +37,7 @@ def same_device(device, **tensors):
 def stream_handle(index: int, stream, tensors) -> int:
     """The raw handle of the call's stream on device `index`: the current one, or `stream` (a raw handle or a torch stream), which the tensors' memory is
     then kept for until it has passed the call."""
-    current = _raw_stream(index)
+    current = raw_stream(index)
     if stream is None:
         return current
     handle = int(getattr(stream, "cuda_stream", stream))

@@ -4,17 +4,45 @@ Beside the tiles of the step (ops/attn.py), which read every sequence's whole co
 from __future__ import annotations
 
 import ctypes as C
+import struct
+from array import array
 from itertools import accumulate
 
 import torch
 
 from . import lib as L
-from ._call import cuda_tensor, same_device, stream_handle, vector
+from ._call import cuda_tensor, raw_stream, same_device, stream_handle
 
 MAX_SEQS = 1024
 _BF16, _I32 = (torch.bfloat16,), (torch.int32,)
-_BYTES = C.sizeof(L.AttnSharedArgs)
+_T, _BYTES = torch.Tensor, C.sizeof(L.AttnSharedArgs)
+_pack, _WORK = struct.Struct("11PN6q8ifi").pack, 10                # (the structure's fields in order, quicker than through ctypes; where `work` stands)
 _BAD = {1: "a table names a page outside the cache", 2: "a length lies outside its table", 4: "a wait inside the kernel ran past two seconds"}
+
+
+def _check(q, kc, vc, tables, lens, prefix_tables, prefix_lens, out, status):
+    """Raises what is wrong with the tensors."""
+    cuda_tensor("kc", kc, _BF16, (None, None, None, 16, 8), inner=False)
+    pages, NKV, hd8 = kc.shape[:3]
+    HD = 8 * hd8
+    cuda_tensor("vc", vc, _BF16, (pages, NKV, HD, 16), inner=False)
+    if kc.stride()[1:] != (hd8 * 128, 128, 8, 1) or vc.stride()[1:] != (HD * 16, 16, 1):
+        raise ValueError("kc, vc: a page has no gaps")
+    cuda_tensor("q", q, _BF16)
+    shape = q.shape
+    if len(shape) == 3 and (shape[2] != HD or (shape[1] > 1 and q.stride(1) != HD)) or len(shape) not in (2, 3) or (len(shape) == 2 and shape[1] % HD):
+        raise ValueError(f"q: shape {tuple(shape)} with strides {q.stride()}, expected [sequences][heads][{HD}] with adjoining heads")
+    if out is not None:
+        cuda_tensor("out", out, _BF16, shape)
+        if len(shape) == 3 and shape[1] > 1 and out.stride(1) != HD:
+            raise ValueError("out: the heads of a row adjoin")
+    cuda_tensor("tables", tables, _I32, (shape[0], None))
+    cuda_tensor("lens", lens, _I32, (shape[0],))
+    cuda_tensor("prefix_tables", prefix_tables, _I32, (None, None))
+    cuda_tensor("prefix_lens", prefix_lens, _I32, (prefix_tables.shape[0],))
+    if status is not None:
+        cuda_tensor("status", status, _I32, (1,))
+    same_device(q.device, kc=kc, vc=vc, out=out, tables=tables, lens=lens, prefix_tables=prefix_tables, prefix_lens=prefix_lens, status=status)
 
 
 def attn_shared(q, kc, vc, tables, lens, prefix_tables, prefix_lens, groups=None, scale=None, out=None, status=None, stream=None):
@@ -32,52 +60,44 @@ def attn_shared(q, kc, vc, tables, lens, prefix_tables, prefix_lens, groups=None
     stream       a raw handle or torch stream; None is the current one
 
     Scores, statistics and sums are fp32.  A sequence without any position has the output 0.  Equal inputs give equal outputs."""
-    cuda_tensor("kc", kc, _BF16, (None, None, None, 16, 8), inner=False)
-    pages, NKV, hd8 = kc.shape[:3]
-    HD, page = 8 * hd8, NKV * hd8 * 128
-    cuda_tensor("vc", vc, _BF16, (pages, NKV, HD, 16), inner=False)
-    if kc.stride()[1:] != (hd8 * 128, 128, 8, 1) or vc.stride()[1:] != (HD * 16, 16, 1):
-        raise ValueError("kc, vc: a page has no gaps")
-    cuda_tensor("q", q, _BF16)
-    shape = q.shape
-    if len(shape) == 3 and (shape[2] != HD or (shape[1] > 1 and q.stride(1) != HD)) or len(shape) not in (2, 3) or (len(shape) == 2 and shape[1] % HD):
-        raise ValueError(f"q: shape {tuple(shape)} with strides {q.stride()}, expected [sequences][heads][{HD}] with adjoining heads")
-    seqs, NH, index = shape[0], shape[1] if len(shape) == 3 else shape[1] // HD, q.get_device()
+    # What usually comes passes here in a few microseconds, which is what small calls take; all else goes through _check, which says what is wrong.
+    plain = out is None and status is None and isinstance(q, _T) and isinstance(kc, _T) and isinstance(vc, _T) and isinstance(tables, _T) and \
+        isinstance(lens, _T) and isinstance(prefix_tables, _T) and isinstance(prefix_lens, _T)
+    if plain:
+        shape, k, v, t, p, index = q.shape, kc.shape, vc.shape, tables.shape, prefix_tables.shape, q.get_device()
+        plain = len(shape) == 3 and len(k) == 5 and len(t) == 2 and len(p) == 2 and index >= 0 and \
+            q.dtype is kc.dtype is vc.dtype is torch.bfloat16 and tables.dtype is lens.dtype is prefix_tables.dtype is prefix_lens.dtype is torch.int32 and \
+            kc.get_device() == vc.get_device() == tables.get_device() == lens.get_device() == prefix_tables.get_device() == prefix_lens.get_device() == index and \
+            q.is_contiguous() and kc.is_contiguous() and vc.is_contiguous() and tables.is_contiguous() and prefix_tables.is_contiguous() and lens.is_contiguous() and \
+            prefix_lens.is_contiguous() and k[3] == 16 and k[4] == 8 and shape[2] == 8 * k[2] and v == (k[0], k[1], shape[2], 16) and t[0] == shape[0] and \
+            lens.shape == (shape[0],) and prefix_lens.shape == (p[0],)
+    if not plain:
+        _check(q, kc, vc, tables, lens, prefix_tables, prefix_lens, out, status)
+        shape, k, t, p, index = q.shape, kc.shape, tables.shape, prefix_tables.shape, q.get_device()
+    seqs, pages, NKV, HD, n_groups = shape[0], k[0], k[1], 8 * k[2], p[0]
+    NH = shape[1] if len(shape) == 3 else shape[1] // HD
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
-    else:
-        cuda_tensor("out", out, _BF16, shape)
-        if len(shape) == 3 and NH > 1 and out.stride(1) != HD:
-            raise ValueError("out: the heads of a row adjoin")
-    cuda_tensor("tables", tables, _I32, (seqs, None))
-    vector("lens", lens, torch.int32, seqs, index)
-    cuda_tensor("prefix_tables", prefix_tables, _I32, (None, None))
-    n_groups = prefix_tables.shape[0]
-    vector("prefix_lens", prefix_lens, torch.int32, n_groups, index)
-    if status is not None:
-        vector("status", status, torch.int32, 1, index)
+        out = torch.empty_like(q) if plain else torch.empty(shape, dtype=torch.bfloat16, device=q.device)
     sizes = (seqs,) if groups is None else [int(n) for n in groups]
     if len(sizes) != n_groups or min(sizes, default=0) < 0 or sum(sizes) != seqs:
         raise ValueError(f"groups: {n_groups} sizes of {seqs} sequences altogether, got {list(sizes)}")
     if seqs > MAX_SEQS or n_groups > MAX_SEQS:
         raise ValueError(f"attn_shared: at most {MAX_SEQS} sequences and groups")
-    if not kc.get_device() == vc.get_device() == out.get_device() == tables.get_device() == prefix_tables.get_device() == index:
-        same_device(q.device, kc=kc, vc=vc, out=out, tables=tables, prefix_tables=prefix_tables)
-    first = (C.c_int32 * (n_groups + 1))(0, *accumulate(sizes))
-    a = L.AttnSharedArgs(q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), tables.data_ptr(), lens.data_ptr(), prefix_tables.data_ptr(), prefix_lens.data_ptr(),
-                         C.addressof(first), status.data_ptr() if status is not None else None, None, 0,
-                         q.stride(0) if seqs > 1 else NH * HD, out.stride(0) if seqs > 1 else NH * HD, kc.stride(0) if pages > 1 else page, vc.stride(0) if pages > 1 else page,
-                         tables.stride(0), prefix_tables.stride(0), seqs, n_groups, NH, NKV, HD, pages, tables.shape[1], prefix_tables.shape[1],
-                         HD ** -0.5 if scale is None else float(scale), 0)
+    first = array("i", (0, *accumulate(sizes)))
+    page = HD * NKV * 16
+    a = [q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), tables.data_ptr(), lens.data_ptr(), prefix_tables.data_ptr(), prefix_lens.data_ptr(),
+         first.buffer_info()[0], 0 if status is None else status.data_ptr(), 0, 0,
+         q.stride(0) if seqs > 1 else NH * HD, out.stride(0) if seqs > 1 else NH * HD, kc.stride(0) if pages > 1 else page, vc.stride(0) if pages > 1 else page,
+         tables.stride(0), prefix_tables.stride(0), seqs, n_groups, NH, NKV, HD, pages, t[1], p[1], HD ** -0.5 if scale is None else float(scale), 0]
     lib, n, work = L.load(), C.c_size_t(), None
-    rc = lib.etxb_attn_shared_work(index, C.byref(a), _BYTES, C.byref(n))
+    rc = lib.etxb_attn_shared_work(index, _pack(*a), _BYTES, C.byref(n))
     if rc:
         L.check(rc)
     if n.value:                                                  # of this call alone: torch keeps it from others until the stream has passed
         work = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        a.work, a.work_bytes = work.data_ptr(), n.value
-    handle = stream_handle(index, stream, (q, out, kc, vc, tables, lens, prefix_tables, prefix_lens, status, work))
-    rc = lib.etxb_attn_shared(index, C.byref(a), _BYTES, handle)
+        a[_WORK:_WORK + 2] = work.data_ptr(), n.value
+    handle = raw_stream(index) if stream is None else stream_handle(index, stream, (q, out, kc, vc, tables, lens, prefix_tables, prefix_lens, status, work))
+    rc = lib.etxb_attn_shared(index, _pack(*a), _BYTES, handle)
     if rc:
         L.check(rc)
     return out

@@ -151,11 +151,11 @@ def load():
         "etxb_exchange_alloc": [C.c_int, sz, C.POINTER(vp), vp], "etxb_exchange_free": [C.c_int, vp],
         "etxb_exchange_open": [C.c_int, vp, C.POINTER(vp)], "etxb_exchange_close": [C.c_int, vp],
         "etxb_set_exchange": [vp, i32, i32, vp, sz, C.POINTER(vp)],
-        "etxb_sample": [C.c_int, C.POINTER(SampleArgs), sz, vp], "etxb_pages_update": [C.c_int, C.POINTER(PagesArgs), sz, vp],
+        "etxb_sample": [C.c_int, vp, sz, vp], "etxb_pages_update": [C.c_int, C.POINTER(PagesArgs), sz, vp],
         "etxb_pool_create": [C.c_int, C.POINTER(PagesArgs), sz, i32, vp, C.POINTER(vp)], "etxb_pool_destroy": [vp], "etxb_pool_open": [vp, i32, C.POINTER(i32), vp],
         "etxb_pool_extend": [vp, vp, vp, i32, vp], "etxb_pool_fork": [vp, i32, i32, i32, vp, vp], "etxb_pool_close": [vp, vp, i32],
         "etxb_pool_compact": [vp, C.POINTER(i32), vp], "etxb_pool_row": [vp, i32, C.POINTER(i32), vp, i32, C.POINTER(i32)], "etxb_pool_free": [vp, C.POINTER(i32)],
-        "etxb_attn_shared": [C.c_int, C.POINTER(AttnSharedArgs), sz, vp], "etxb_attn_shared_work": [C.c_int, C.POINTER(AttnSharedArgs), sz, C.POINTER(sz)],
+        "etxb_attn_shared": [C.c_int, vp, sz, vp], "etxb_attn_shared_work": [C.c_int, vp, sz, C.POINTER(sz)],
     }
     for name, args in proto.items():
         fn = getattr(lib, name)

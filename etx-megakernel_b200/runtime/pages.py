@@ -11,7 +11,7 @@ from array import array
 import torch
 
 from . import lib as L
-from ._call import cuda_tensor, same_device, stream_handle
+from ._call import cuda_tensor, raw_stream, same_device, stream_handle
 
 _BYTES = C.sizeof(L.PagesArgs)
 
@@ -39,9 +39,11 @@ def _layout(src, dst):
 
 def _ints(name, v):
     """`v` as a C array of 32-bit numbers (a number is one of them)."""
-    v = v.tolist() if hasattr(v, "tolist") else v
+    if type(v) is not list:
+        v = v.tolist() if hasattr(v, "tolist") else v
+        v = v if isinstance(v, (list, tuple, range)) else (v,)
     try:
-        out = array("i", v if isinstance(v, (list, tuple, range)) else (v,))
+        out = array("i", v)
     except (TypeError, OverflowError) as e:
         raise ValueError(f"{name}: whole numbers of 32 bits") from e
     return (C.c_int32 * len(out)).from_buffer(out)
@@ -49,6 +51,8 @@ def _ints(name, v):
 
 def _int(name, v):
     """`v` as a 32-bit number (ctypes would cut a larger one)."""
+    if type(v) is int and -2 ** 31 <= v < 2 ** 31:
+        return v
     return _ints(name, [v])[0]
 
 
@@ -111,6 +115,8 @@ class PagePool:
             self._h = None
 
     def _stream(self, stream):
+        if stream is None:
+            return raw_stream(self._index)
         return stream_handle(self._index, stream, (*self.tensors, self.tables))
 
     # ---- what is where
@@ -165,7 +171,7 @@ class PagePool:
         row, n, length = _int("row", row), _int("n", n), -1 if length is None else _int("length", length)
         rows = (C.c_int32 * max(n, 0))()
         _check(self._lib.etxb_pool_fork(self._h, row, n, length, rows, self._stream(stream)))
-        return list(rows)
+        return rows[:]
 
     def close(self, rows) -> None:
         """The sequences end: pages that nobody else holds are free again (their contents and the rows' entries stay as they are)."""

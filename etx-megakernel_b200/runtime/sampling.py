@@ -4,17 +4,19 @@ No counterpart in the reference, whose host loop is greedy (examples/vllm_llm/vl
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
 
 from . import lib as L
-from ._call import cuda_tensor, stream_handle, vector
+from ._call import cuda_tensor, raw_stream, stream_handle, vector
 
 _DT = {torch.bfloat16: L.DTYPES["bf16"], torch.float16: L.DTYPES["f16"], torch.float32: L.DTYPES["f32"]}
 MAX_V = 524288
-_BYTES = C.sizeof(L.SampleArgs)
+_T, _BYTES = torch.Tensor, C.sizeof(L.SampleArgs)
+_pack = struct.Struct("10Pq4i3fi").pack                            # (the structure's fields in order, quicker than through ctypes)
 
 
 class Sampled(NamedTuple):
@@ -52,7 +54,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=Non
 
     temperature, top_k, top_p, min_p: numbers, or tensors [rows] (float32; top_k int32).  tokens / next_tokens: int32 tensors [rows] that take the tokens
     (the second one them once more, 0 where there is none: the next step's input).  stream: a raw handle or torch stream; None is the current one."""
-    cuda_tensor("logits", logits, _DT, (None, None))
+    if not (isinstance(logits, _T) and logits.is_cuda and logits.dtype in _DT and len(logits.shape) == 2 and (logits.shape[1] == 1 or logits.stride(1) == 1)):
+        cuda_tensor("logits", logits, _DT, (None, None))          # (says what is wrong)
     rows, V = logits.shape
     if not 1 <= V <= MAX_V:
         raise ValueError(f"logits: {V} tokens outside 1..{MAX_V}")
@@ -61,27 +64,30 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=Non
         raise ValueError(f"logits: rows overlap (stride {stride} below {V})")
     index = logits.get_device()
     vector("u", u, torch.float32, rows, index)
-    a = L.SampleArgs()
-    a.logits, a.u, a.row_stride, a.rows, a.V, a.dtype = logits.data_ptr(), u.data_ptr(), stride, rows, V, _DT[logits.dtype]
     keep = [logits, u]
-    for name, v in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("top_k", top_k)):
-        if isinstance(v, torch.Tensor):
-            setattr(a, name, vector(name, v, torch.int32 if name == "top_k" else torch.float32, rows, index).data_ptr())
-            keep.append(v)
-        else:
-            setattr(a, name + "_all", min(int(v), MAX_V) if name == "top_k" else float(v))
-    for name, t in (("tokens", tokens), ("next_tokens", next_tokens)):
-        if t is not None:
-            vector(name, t, torch.int32, rows, index)
-    dev = logits.device
-    if tokens is None:
-        tokens = torch.empty(rows, dtype=torch.int32, device=dev)
-    logprobs, kept = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.int32, device=dev)
-    a.tokens, a.logprobs, a.kept = tokens.data_ptr(), logprobs.data_ptr(), kept.data_ptr()
+
+    def setting(name, v, dtype):
+        """The setting as (address of one value per row, value for all)."""
+        if not isinstance(v, _T):
+            return 0, max(min(int(v), MAX_V), 0) if dtype is torch.int32 else C.c_float(v).value
+        keep.append(vector(name, v, dtype, rows, index))
+        return v.data_ptr(), 0
+    temperatures, temperature = setting("temperature", temperature, torch.float32)
+    ks, k = setting("top_k", top_k, torch.int32)
+    ps, p = setting("top_p", top_p, torch.float32)
+    mins, least = setting("min_p", min_p, torch.float32)
     if next_tokens is not None:
-        a.next = next_tokens.data_ptr()
-    handle = stream_handle(index, stream, (*keep, tokens, next_tokens, logprobs, kept))
-    rc = L.load().etxb_sample(index, C.byref(a), _BYTES, handle)
+        keep.append(vector("next_tokens", next_tokens, torch.int32, rows, index))
+    logprobs = torch.empty_like(u)
+    kept = torch.empty_like(u, dtype=torch.int32)
+    if tokens is None:
+        tokens = torch.empty_like(kept)
+    else:
+        vector("tokens", tokens, torch.int32, rows, index)
+    handle = raw_stream(index) if stream is None else stream_handle(index, stream, (*keep, tokens, logprobs, kept))
+    a = _pack(logits.data_ptr(), u.data_ptr(), temperatures, ks, ps, mins, tokens.data_ptr(), 0 if next_tokens is None else next_tokens.data_ptr(), logprobs.data_ptr(),
+              kept.data_ptr(), stride, rows, V, _DT[logits.dtype], k, temperature, p, least, 0)
+    rc = L.load().etxb_sample(index, a, _BYTES, handle)
     if rc:
         L.check(rc)
     return Sampled(tokens, logprobs, kept)

@@ -43,3 +43,11 @@ def test_host_tensors_are_refused():
     z = torch.zeros(2, 2, 16, 16, 8, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA tensor"):
         attn_shared(z, z, z, z, z, z, z)
+
+
+def test_packed_arguments_are_the_structure():
+    import importlib
+    mod = importlib.import_module("etx_megakernel_b200.runtime.attn_shared")
+    values = list(range(1, 27)) + [0.5, 28]
+    packed = lib.AttnSharedArgs.from_buffer_copy(mod._pack(*values))
+    assert C.sizeof(packed) == len(mod._pack(*values)) and [getattr(packed, n) for n, _ in packed._fields_] == values

@@ -39,3 +39,11 @@ def test_host_tensors_are_refused():
         sample(l, u)
     with pytest.raises(ValueError, match="CUDA tensor"):
         sample([1.0], u)
+
+
+def test_packed_arguments_are_the_structure():
+    import importlib
+    mod = importlib.import_module("etx_megakernel_b200.runtime.sampling")
+    values = list(range(1, 16)) + [0.5, 0.25, 0.125, 19]
+    packed = lib.SampleArgs.from_buffer_copy(mod._pack(*values))
+    assert C.sizeof(packed) == len(mod._pack(*values)) and [getattr(packed, n) for n, _ in packed._fields_] == values

@@ -62,15 +62,17 @@ __device__ __forceinline__ bool falls(int how, uint32_t rank, double x, uint32_t
 }
 
 // ================================================================================================ logits of 16 bits
-// Keys: values as unsigned numbers in the values' order; 0 for -inf and NaN; -0 is +0.  INF: the key of +inf (bf16 0x7f80, fp16 0x7c00).
+// Keys: values as unsigned numbers in the values' order, two a word.  Numbers have the keys LOWEST .. HIGHEST; below them stand -inf (LOWEST - 1) and the
+// NaN with a sign, above them the other NaN.  -0 has the key before +0's: counts of it become +0's.  INF: the bits of +inf (bf16 0x7f80, fp16 0x7c00).
+constexpr uint32_t MINUS_ZERO = 0x7fffu, ZERO = 0x8000u;
 template <uint32_t INF>
 struct Key16 {
-  static constexpr uint32_t LOWEST = (uint32_t)(0xffffu - (INF - 1u + 0x8000u)) & 0xffffu;         // the key of the type's lowest number
-  static __device__ __forceinline__ uint32_t of(uint32_t u) {                                       // u: 16 bits
-    uint32_t k = (u & 0x8000u) ? (~u & 0xffffu) : (u | 0x8000u);
-    if (k == 0x7fffu) k = 0x8000u;
-    return k - LOWEST <= INF + 0x8000u - LOWEST ? k : 0u;
+  static constexpr uint32_t LOWEST = 0x8000u - INF, HIGHEST = 0x8000u + INF, NOTHING = (0x8000u | INF) * 0x10001u;   // (two times -inf)
+  static __device__ __forceinline__ uint32_t of_two(uint32_t u) {
+    const uint32_t m = u & 0x80008000u;
+    return u ^ 0x80008000u ^ (m - (m >> 15));
   }
+  static __device__ __forceinline__ bool is(uint32_t k) { return k - LOWEST <= HIGHEST - LOWEST; }
 };
 template <typename T> __device__ __forceinline__ float value16(uint32_t key);
 template <> __device__ __forceinline__ float value16<__nv_bfloat16>(uint32_t key) {
@@ -81,6 +83,7 @@ template <> __device__ __forceinline__ float value16<__half>(uint32_t key) {
 }
 
 constexpr int GROUPS = 2048, CHUNK = 8191;                          // groups of 32 values; vectors of 8 logits a block counts (16 bits hold their number)
+constexpr int PIECE = 4095, PART = 32767, PARTS = 32;               // of a whole row (see counts_kernel)
 struct Group {
   double mass, mass_min;                                            // sum of the weights of its tokens, and of those that min-p keeps
   uint32_t count, count_min;
@@ -91,7 +94,8 @@ struct Counts {
   double before_mass[GROUPS + 1];                                   // of the groups above (index: from the largest value down)
   uint32_t before_count[GROUPS + 1];
   uint16_t list[GROUPS];                                            // of the groups this block joins, the ones that occur
-  uint32_t bits[GROUPS / 32];                                       // the groups that occur in this block's part
+  uint32_t bits[GROUPS / 32], row_bits[GROUPS / 32];                // the groups that occur in this block's part; those of the row that this block joins
+  uint32_t part_key[PARTS], part_count[PARTS], n_parts, low;        // (a whole row) counts that 16 bits do not hold
   uint32_t wc[WARPS], wcm[WARPS];
   double wm[WARPS], wmm[WARPS];
   uint32_t maxkey, n_list;
@@ -102,13 +106,18 @@ struct Counts {
 };
 static_assert(sizeof(Counts) <= 231424, "a block's shared memory");
 
+// NV > 0: a block has NV vectors a thread, which stay in registers.  NV = 0: one block counts a whole row, whatever its length, in pieces of PIECE vectors;
+// before a counter could pass its 16 bits, what stands above 32767 in any of them goes to a list.  (A row of 151936 in 4 blocks that wait for each other, 256
+// rows: 194 us; in one: see the launch.)
 template <typename T, int NV>
 __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_args a) {
   using K = Key16<sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u>;
+  constexpr bool WHOLE = NV == 0;
+  constexpr int N = WHOLE ? 4 : NV;
   extern __shared__ __align__(16) unsigned char smem[];
   Counts& s = *(Counts*)smem;
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), r = (int)cluster.block_rank(), row = blockIdx.x / C;
+  const int C = WHOLE ? 1 : (int)cluster.num_blocks(), r = WHOLE ? 0 : (int)cluster.block_rank(), row = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const Settings st = settings(a, row);
   const bool greedy = !(st.T > 0.f);
@@ -117,54 +126,113 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
   const T* l = (const T*)a.logits + (long long)row * a.row_stride;
   const int shift = (int)((uintptr_t)l & 15) / 2, nvec = (shift + V + 7) / 8;
   const int v0 = (int)((long long)nvec * r / C), v1 = (int)((long long)nvec * (r + 1) / C);
-  uint4 key[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = v0 + i * THREADS + tid;
-    key[i] = make_uint4(0u, 0u, 0u, 0u);
+  auto keys_of = [&](int v, int end) {
+    uint4 q = make_uint4(K::NOTHING, K::NOTHING, K::NOTHING, K::NOTHING);
     const int e = v * 8 - shift;
-    if (v < v1 && e >= 0 && e + 8 <= V) key[i] = __ldg((const uint4*)(l + e));
-    else if (v < v1) {                                              // the row's ends, one by one (0xffff is no number)
+    if (v < end && e >= 0 && e + 8 <= V) q = __ldg((const uint4*)(l + e));
+    else if (v < end) {                                             // the row's ends, one by one
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int x = e + 2 * j;
-        const uint32_t lo = x >= 0 && x < V ? ((const unsigned short*)l)[x] : 0xffffu, hi = x + 1 >= 0 && x + 1 < V ? ((const unsigned short*)l)[x + 1] : 0xffffu;
+        const uint32_t lo = x >= 0 && x < V ? ((const unsigned short*)l)[x] : K::NOTHING & 0xffffu, hi = x + 1 >= 0 && x + 1 < V ? ((const unsigned short*)l)[x + 1] : K::NOTHING & 0xffffu;
         w[j] = lo | (hi << 16);
       }
-      key[i] = make_uint4(w[0], w[1], w[2], w[3]);
-    } else key[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
-  }
-  if (!greedy)
-    for (int i = tid; i < 32768 / 4; i += THREADS) ((uint4*)s.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
-  if (!greedy)
-    for (int i = tid; i < (int)(sizeof s.group / 16); i += THREADS) ((uint4*)s.group)[i] = make_uint4(0u, 0u, 0u, 0u);
-  if (tid == 0) { s.maxkey = 0u; s.n_list = 0u; }
-  __syncthreads();
+      q = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return make_uint4(K::of_two(q.x), K::of_two(q.y), K::of_two(q.z), K::of_two(q.w));
+  };
+  uint4 key[N];
   uint32_t mx = 0u, low = 0u;
+  auto fetch = [&](int v, int end) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    uint32_t* w = (uint32_t*)&key[i];
+    for (int i = 0; i < N; ++i) key[i] = keys_of(v + i * THREADS + tid, end);
+  };
+  auto largest = [&]() {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t k0 = K::of(w[j] & 0xffffu), k1 = K::of(w[j] >> 16);
-      w[j] = k0 | (k1 << 16);
-      mx = max(mx, max(k0, k1));
-      if (!greedy) {
-        // (a mask of the type's lowest number makes most of a row equal: those are counted without memory)
-        if (k0 == K::LOWEST) ++low; else if (k0) atomicAdd(&s.hist[k0 >> 1], 1u << ((k0 & 1u) * 16u));
-        if (k1 == K::LOWEST) ++low; else if (k1) atomicAdd(&s.hist[k1 >> 1], 1u << ((k1 & 1u) * 16u));
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t k = ((const uint32_t*)&key[i])[j >> 1] >> (16 * (j & 1)) & 0xffffu;
+        if (K::is(k)) mx = max(mx, k == MINUS_ZERO ? ZERO : k);
+      }
+  };
+  // No branch for a logit (with one for "-inf" and one for the lowest number 0.46 clocks each, so 0.2; the atomics alone are 0.14).  Masked ones, -inf or the type's lowest
+  // number, are most of some rows and would wait for each other: the first are not counted, the others without memory.
+  const uint32_t hist = (uint32_t)__cvta_generic_to_shared(s.hist);
+  auto count = [&]() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t w = ((const uint32_t*)&key[i])[j >> 1], k = j & 1 ? w >> 16 : w & 0xffffu;
+        asm volatile("{\n .reg .pred p;\n setp.gt.u32 p, %0, 1;\n @p red.shared.add.u32 [%1], %2;\n}" ::
+                         "r"(k - (K::LOWEST - 1u)), "r"(hist + ((k << 1) & 0x1fffcu)), "r"(k & 1u ? 0x10000u : 1u) : "memory");
+        low += k == K::LOWEST ? 1u : 0u;
       }
     }
-  }
-  mx = __reduce_max_sync(~0u, mx); low = __reduce_add_sync(~0u, low);
-  if (lane == 0) { atomicMax(&s.maxkey, mx); if (low) atomicAdd(&s.hist[K::LOWEST >> 1], low << ((K::LOWEST & 1u) * 16u)); }
-  __syncthreads();
+  };
+  if constexpr (!WHOLE) fetch(v0, v1);
   if (!greedy) {
-    // groups that occur: four lanes look at the 64 bytes of one
+    for (int i = tid; i < 32768 / 4; i += THREADS) ((uint4*)s.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = tid; i < (int)(sizeof s.group / 16); i += THREADS) ((uint4*)s.group)[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  if (tid == 0) { s.maxkey = 0u; s.n_list = 0u; s.n_parts = 0u; s.low = 0u; }
+  __syncthreads();
+  if constexpr (!WHOLE) {
+    if (greedy) largest(); else count();
+  } else {
+    for (int v = 0, piece = 0; v < nvec; v += PIECE, ++piece) {
+      fetch(v, min(v + PIECE, nvec));
+      if (greedy) { largest(); continue; }
+      if (piece >= 2) {                                             // two pieces are 65520 logits; behind this, 32768 and one piece fit
+        __syncthreads();
+        for (int i = tid; i < 32768 / 4; i += THREADS) {
+          const uint4 q = ((const uint4*)s.hist)[i];
+          if (((q.x | q.y | q.z | q.w) & 0x80008000u) == 0u) continue;
+          for (int k = 8 * i; k < 8 * i + 8; ++k) {
+            uint16_t& c = ((uint16_t*)s.hist)[k];
+            if (c < PART + 1) continue;
+            c -= PART;
+            if (K::is((uint32_t)k)) { const uint32_t n = atomicAdd(&s.n_parts, 1u); s.part_key[n] = k == MINUS_ZERO ? ZERO : k; s.part_count[n] = PART; }      // (16 of them at most)
+          }
+        }
+        __syncthreads();
+      }
+      count();
+    }
+  }
+  if (greedy) {
+    mx = __reduce_max_sync(~0u, mx);
+    if (lane == 0) atomicMax(&s.maxkey, mx);
+    __syncthreads();
+  } else {
+    low = __reduce_add_sync(~0u, low);
+    if (lane == 0 && low) atomicAdd(&s.low, low);
+    __syncthreads();
+    // what is no number goes, -0 becomes +0, the lowest ones come in
+    if (tid < (int)K::LOWEST / 2) s.hist[tid] = 0u;
+    if (tid < (0x10000 - (int)K::HIGHEST) / 2) s.hist[K::HIGHEST / 2 + tid] &= tid ? 0u : 0xffffu;
+    static_assert(K::LOWEST / 2 <= THREADS && (0x10000 - K::HIGHEST) / 2 <= THREADS && K::HIGHEST % 2 == 0 && K::LOWEST % 2 == 0, "a thread a word");
+    if (tid == THREADS - 1) {
+      auto put = [&](uint32_t k, uint32_t n) {
+        uint16_t& c = ((uint16_t*)s.hist)[k];
+        if (c + n > 65535u) { const uint32_t i = s.n_parts++; s.part_key[i] = k; s.part_count[i] = n - 1u; n = 1u; if (c) { s.part_count[i] += 1u; n = 0u; } }
+        c += (uint16_t)n;
+      };
+      const uint32_t minus = s.hist[MINUS_ZERO / 2] >> 16;
+      if (minus) { s.hist[MINUS_ZERO / 2] &= 0xffffu; put(ZERO, minus); }
+      if (s.low) put(K::LOWEST, s.low);
+    }
+    __syncthreads();
+    // groups that occur: four lanes look at the 64 bytes of one; the largest value
     for (int i = 0; i < GROUPS * 4 / THREADS; ++i) {
       const uint4 q = ((const uint4*)s.hist)[i * THREADS + tid];
       uint32_t any = q.x | q.y | q.z | q.w;
+      if (any) {
+        const int top = q.w ? 6 : q.z ? 4 : q.y ? 2 : 0;
+        mx = (uint32_t)((i * THREADS + tid) * 8 + top) + ((q.w ? q.w : q.z ? q.z : q.y ? q.y : q.x) >> 16 ? 1u : 0u);         // (i rises)
+      }
       any |= __shfl_xor_sync(~0u, any, 1); any |= __shfl_xor_sync(~0u, any, 2);
       uint32_t b = __ballot_sync(~0u, any != 0u);                   // 8 groups, a nibble each
       if (lane == 0) {
@@ -173,6 +241,8 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
         ((unsigned char*)s.bits)[i * (THREADS / 32) + warp] = (unsigned char)b;
       }
     }
+    mx = __reduce_max_sync(~0u, mx);
+    if (lane == 0) atomicMax(&s.maxkey, mx);
   }
   cluster.sync();
   // one word from every block of the cluster, all on their way at once
@@ -197,6 +267,7 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
   // tokens of value k in the whole row
   auto tokens_of = [&](uint32_t k) {
     uint32_t n = 0u;
+    for (uint32_t i = 0; i < s.n_parts; ++i) n += s.part_key[i] == k ? s.part_count[i] : 0u;      // (of this block: it is the only one, or there are none)
     from_all((const uint16_t*)s.hist + k, uint16_t(), [&](int, uint16_t x) { n += x; });
     return n;
   };
@@ -208,9 +279,16 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
     if (tid < GROUPS / 32) {
       uint32_t b = 0u;
       from_all(&s.bits[tid], uint32_t(), [&](int, uint32_t x) { b |= x; });
-      b &= (C == 1 ? ~0u : C == 2 ? 0x55555555u : C == 4 ? 0x11111111u : 0x01010101u) << r;
-      uint32_t n = b ? atomicAdd(&s.n_list, (uint32_t)__popc(b)) : 0u;
-      for (; b; b &= b - 1u) s.list[n++] = (uint16_t)(tid * 32 + __ffs(b) - 1);
+      s.row_bits[tid] = b & (C == 1 ? ~0u : C == 2 ? 0x55555555u : C == 4 ? 0x11111111u : 0x01010101u) << r;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < GROUPS / THREADS; ++i) {
+      const uint32_t b = s.row_bits[i * WARPS + warp];
+      uint32_t n = 0u;
+      if (lane == 0 && b) n = atomicAdd(&s.n_list, (uint32_t)__popc(b));
+      n = __shfl_sync(~0u, n, 0) + (uint32_t)__popc(b & ((1u << lane) - 1u));
+      if (b >> lane & 1u) s.list[n] = (uint16_t)(i * THREADS + tid);
     }
     __syncthreads();
     for (uint32_t i = warp; i < s.n_list; i += WARPS) {
@@ -334,7 +412,8 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
       }
       // which block has it: the tokens of that value in the blocks before
       uint32_t ahead = 0u, here = 0u;
-      from_all((const uint16_t*)s.hist + place_key, uint16_t(), [&](int c, uint16_t z) { if (c < r) ahead += z; if (c == r) here = z; });
+      if constexpr (WHOLE) here = place_count;
+      else from_all((const uint16_t*)s.hist + place_key, uint16_t(), [&](int c, uint16_t z) { if (c < r) ahead += z; if (c == r) here = z; });
       if (lane == 0) {
         s.at = place_key; s.nth = nth - ahead; s.mine = ahead <= nth && nth < ahead + here;
         s.kept = (int)n; s.logp = (float)(log_weight(place_key) - log(Wn));
@@ -348,15 +427,46 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
   const float logp = s.logp;
   const int kept = s.kept;
   const bool mine = s.mine != 0;
-  if (mine) {
+  const uint32_t at_too = at == ZERO ? MINUS_ZERO : at;
+  auto matches = [&](const uint4& q) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { const uint32_t k = (&q.x)[j >> 1] >> (16 * (j & 1)) & 0xffffu; m |= (k == at || k == at_too ? 1u : 0u) << j; }
+    return m;
+  };
+  if constexpr (WHOLE) {
+    // a warp has a 32nd of the row, in the order of the indices
+    uint32_t* cnt = (uint32_t*)s.list;
+    const int per = (nvec + WARPS - 1) / WARPS, w0 = min(warp * per, nvec), w1 = min(w0 + per, nvec);
+    uint32_t c = 0u;
+#pragma unroll 4
+    for (int v = w0; v < w1; v += 32) c += (uint32_t)__popc(matches(keys_of(v + lane, w1)));
+    c = __reduce_add_sync(~0u, c);
+    if (lane == 0) cnt[warp] = c;
+    __syncthreads();
+    uint32_t before = 0u;
+    for (int w = 0; w < warp; ++w) before += cnt[w];
+    if (before <= nth && nth < before + c)
+      for (int v = w0; v < w1; v += 32) {
+        uint32_t m = matches(keys_of(v + lane, w1));
+        const uint32_t n = (uint32_t)__popc(m);
+        uint32_t upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(~0u, upto, o); if (lane >= o) upto += x; }
+        const uint32_t mine_before = before + upto - n;
+        if (mine_before <= nth && nth < mine_before + n) {
+          for (uint32_t q = mine_before; q < nth; ++q) m &= m - 1u;
+          store(a, row, (v + lane) * 8 - shift + __ffs(m) - 1, logp, kept);
+        }
+        before += __shfl_sync(~0u, upto, 31);
+        if (before > nth) break;
+      }
+  } else if (mine) {
     uint32_t* cnt = (uint32_t*)s.list;                              // matches by vector number and warp: the order of the indices
     uint32_t match[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t* w = (const uint32_t*)&key[i];
-      match[i] = 0u;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) match[i] |= ((w[j] & 0xffffu) == at ? 1u << (2 * j) : 0u) | ((w[j] >> 16) == at ? 2u << (2 * j) : 0u);
+      match[i] = matches(key[i]);
       const uint32_t c = __reduce_add_sync(~0u, (uint32_t)__popc(match[i]));
       if (lane == 0) cnt[i * WARPS + warp] = c;
     }
@@ -396,7 +506,6 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
 }
 
 // ================================================================================================ logits of 32 bits
-// (also 16-bit ones of a vocabulary that the counters of a cluster do not hold)
 // Logits as keys whose order as unsigned numbers is the order of the values; 0: not live (-inf, NaN).  -0 counts as +0.
 __device__ __forceinline__ uint32_t key_of(float l) {
   uint32_t u = __float_as_uint(l);
@@ -406,11 +515,7 @@ __device__ __forceinline__ uint32_t key_of(float l) {
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key); }
 
-__device__ __forceinline__ float load(const float* p, int i) { return p[i]; }
-__device__ __forceinline__ float load(const __nv_bfloat16* p, int i) { return __bfloat162float(p[i]); }
-__device__ __forceinline__ float load(const __half* p, int i) { return __half2float(p[i]); }
-
-constexpr int BINS = 2048;
+constexpr int BINS = 2048, LIST = 2048;
 struct Sums {
   uint32_t count[BINS], lo[BINS], hi[BINS];                         // of this block's part
   uint32_t all_count[2][BINS];                                      // of the row: by the first 11 bits of the key; by the next ones of one of those bins
@@ -421,6 +526,7 @@ struct Sums {
   unsigned long long mass_min;
   uint32_t bin, before_count, n;
   unsigned long long before_mass;
+  uint32_t part[2][LIST], n_part[2], list[LIST];                    // the values of one of the first bins: this block's, and the row's
 };
 struct Row {
   double max, inv_t;
@@ -436,8 +542,9 @@ __device__ __forceinline__ double real_weight(const Row& r, uint32_t key) {
 }
 __device__ __forceinline__ unsigned long long weight(const Row& r, uint32_t key) { return __double2ull_rn(real_weight(r, key) * r.scale); }
 
-// C blocks have a row together; each goes over its part of it once for the first bins and once for every refinement (the part stays in its L1).
-template <typename T>
+// C blocks have a row together.  Each goes over its part of it twice for the first bins.  A border falls into one of them, which rarely has more than LIST tokens: they are
+// told to all blocks, and each refines them by itself.  (Refined over the row, with the blocks' bins joined for each level: 13 rows of 50257 67 us.)  A bin of more tokens
+// is refined over the row.
 __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a) {
   extern __shared__ __align__(16) unsigned char smem[];
   Sums& s = *(Sums*)smem;
@@ -445,7 +552,7 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
   const int C = (int)cluster.num_blocks(), r = (int)cluster.block_rank(), row = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int i0 = (int)((long long)a.V * r / C), i1 = (int)((long long)a.V * (r + 1) / C);
-  const T* l = (const T*)a.logits + (long long)row * a.row_stride;
+  const float* l = (const float*)a.logits + (long long)row * a.row_stride;
   const Settings st = settings(a, row);
 
   if (tid == 0) { s.maxkey = 0u; s.live = 0u; s.kept_min = 0u; s.mass_min = 0ull; }
@@ -453,7 +560,17 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
   clear();
   __syncthreads();
   uint32_t mx = 0u, live = 0u;
-  for (int i = i0 + tid; i < i1; i += THREADS) { const uint32_t key = key_of(load(l, i)); mx = max(mx, key); live += key ? 1u : 0u; }
+  // 8 logits a thread at once: their loads are on the way together
+  auto for_all = [&](auto use) {
+    for (int i = i0 + tid; i < i1; i += 8 * THREADS) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i + j * THREADS < i1 ? l[i + j * THREADS] : -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) use(key_of(v[j]));
+    }
+  };
+  for_all([&](uint32_t key) { mx = max(mx, key); live += key ? 1u : 0u; });
   mx = __reduce_max_sync(~0u, mx); live = __reduce_add_sync(~0u, live);
   if (lane == 0) { atomicMax(&s.maxkey, mx); atomicAdd(&s.live, live); }
   cluster.sync();
@@ -493,14 +610,13 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
     };
     uint32_t cm = 0u;
     unsigned long long mm = 0ull;
-    for (int i = i0 + tid; i < i1; i += THREADS) {
-      const uint32_t key = key_of(load(l, i));
-      if (!key) continue;
+    for_all([&](uint32_t key) {
+      if (!key) return;
       const double e = real_weight(w, key);
       const unsigned long long x = __double2ull_rn(e * w.scale);
       add(key >> 21, x);
       if (e >= (double)st.min_p) { ++cm; mm += x; }
-    }
+    });
     cm = __reduce_add_sync(~0u, cm);
 #pragma unroll
     for (int o = 16; o; o >>= 1) mm += __shfl_xor_sync(~0u, mm, o);
@@ -551,20 +667,47 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
     };
     uint32_t place_key = 0u, place_before = 0u, place_count = 0u;
     unsigned long long place_mass = 0ull;
+    uint32_t held = ~0u;                      // the bin whose tokens s.list has
+    int buf = 0;
     auto lookup = [&](int how, uint32_t rank, double x) {
       find_bin(0, BINS, how, rank, x, 0u, 0ull);
       if (s.bin == ~0u) return false;
       uint32_t prefix = s.bin, cb = s.before_count;
       unsigned long long mb = s.before_mass;
+      const uint32_t in_bin = s.n;
+      const bool few = in_bin <= LIST;        // (of the whole row: every block decides alike)
+      if (few && prefix != held) {
+        if (tid == 0) s.n_part[buf] = 0u;
+        __syncthreads();
+        for_all([&](uint32_t k) { if (k && k >> 21 == prefix) s.part[buf][atomicAdd(&s.n_part[buf], 1u)] = k; });
+        cluster.sync();                       // (a block reads another one's part until the next such sync: the parts alternate)
+        uint32_t off = 0u, n[MAX_CLUSTER];
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; ++c) n[c] = c < C ? *cluster.map_shared_rank(&s.n_part[buf], c) : 0u;
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; ++c) {
+          if (c >= C) break;
+          const uint32_t* from = cluster.map_shared_rank(s.part[buf], c);
+          for (uint32_t i = tid; i < n[c]; i += THREADS) s.list[off + i] = from[i];
+          off += n[c];
+        }
+        held = prefix; buf ^= 1;
+        __syncthreads();
+      }
       for (int level = 1; level < 3; ++level) {
         const int bits = level == 1 ? 11 : 10, shift = level == 1 ? 10 : 0, nb = 1 << bits;
         clear();
         __syncthreads();
-        for (int i = i0 + tid; i < i1; i += THREADS) {
-          const uint32_t k = key_of(load(l, i));
-          if (k && (k >> (shift + bits)) == prefix) add((k >> shift) & (nb - 1), weight(w, k));
+        auto take = [&](uint32_t k) { if (k && (k >> (shift + bits)) == prefix) add((k >> shift) & (nb - 1), weight(w, k)); };
+        if (few) {
+          for (uint32_t i = tid; i < in_bin; i += THREADS) take(s.list[i]);
+          __syncthreads();
+          for (int i = tid; i < BINS; i += THREADS) { s.all_count[1][i] = s.count[i]; s.all_mass[1][i] = ((unsigned long long)s.hi[i] << 32) + s.lo[i]; }
+          __syncthreads();
+        } else {
+          for_all(take);
+          join(1);
         }
-        join(1);
         find_bin(1, nb, how, rank, x, cb, mb);
         if (s.bin == ~0u) return false;       // (cannot be: the sums of a bin are the bin's)
         prefix = (prefix << bits) | s.bin; cb = s.before_count; mb = s.before_mass;
@@ -614,7 +757,8 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
   // its nth token, by index: a warp has 32nd parts of the block's part
   const int per = (i1 - i0 + WARPS - 1) / WARPS, w0 = i0 + warp * per, w1 = min(i1, w0 + per);
   uint32_t c = 0u;
-  for (int i = w0 + lane; i < w1; i += 32) c += key_of(load(l, i)) == at ? 1u : 0u;
+#pragma unroll 8
+  for (int i = w0 + lane; i < w1; i += 32) c += key_of(l[i]) == at ? 1u : 0u;
   c = __reduce_add_sync(~0u, c);
   if (tid == 0) s.here = 0u;
   __syncthreads();
@@ -625,7 +769,7 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
   for (int b = 0; b < warp; ++b) before += s.wcm[b];
   if (before <= nth && nth < before + c)
     for (int i = w0; i < w1; i += 32) {
-      const bool is = i + lane < w1 && key_of(load(l, i + lane)) == at;
+      const bool is = i + lane < w1 && key_of(l[i + lane]) == at;
       uint32_t hits = __ballot_sync(~0u, is);
       const uint32_t some = (uint32_t)__popc(hits);
       if (nth < before + some) {
@@ -664,26 +808,31 @@ extern "C" int32_t etxb_sample(int device, const etxb_sample_args* args, size_t 
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
   cfg.blockDim = dim3(THREADS); cfg.stream = (cudaStream_t)cuda_stream; cfg.attrs = &at; cfg.numAttrs = 1;
-  // blocks of a row: as many as its counters need, and more while the device has room and each block still has 8192 logits
   int C = 1;
-  const long long vectors = ((long long)a.V + 7 + 7) / 8;
-  while ((vectors + C - 1) / C > CHUNK) C *= 2;
   static std::atomic<char> ready[11][64];
   const void* k;
   int which;
-  if (a.dtype == ETXB_F32 || C > MAX_CLUSTER) {
-    static const void* const kernels[3] = {(const void*)sums_kernel<__nv_bfloat16>, (const void*)sums_kernel<__half>, (const void*)sums_kernel<float>};
-    k = kernels[a.dtype]; which = 8 + a.dtype;
-    C = 1;
+  if (a.dtype == ETXB_F32) {
+    k = (const void*)sums_kernel; which = 10;
     while (C < MAX_CLUSTER && (long long)a.rows * 2 * C <= sms && a.V / C > 2048) C *= 2;
     cfg.dynamicSmemBytes = sizeof(Sums);
   } else {
-    static const void* const kernels[2][4] = {
-        {(const void*)counts_kernel<__nv_bfloat16, 1>, (const void*)counts_kernel<__nv_bfloat16, 2>, (const void*)counts_kernel<__nv_bfloat16, 4>, (const void*)counts_kernel<__nv_bfloat16, 8>},
-        {(const void*)counts_kernel<__half, 1>, (const void*)counts_kernel<__half, 2>, (const void*)counts_kernel<__half, 4>, (const void*)counts_kernel<__half, 8>}};
-    while (C < MAX_CLUSTER && (long long)a.rows * 2 * C <= sms && vectors / C > 1024) C *= 2;
-    const int nv = ((int)((vectors + C - 1) / C) + THREADS - 1) / THREADS, size = nv <= 1 ? 0 : nv <= 2 ? 1 : nv <= 4 ? 2 : 3;
-    k = kernels[a.dtype == ETXB_F16][size]; which = 4 * (a.dtype == ETXB_F16) + size;
+    static const void* const kernels[2][5] = {
+        {(const void*)counts_kernel<__nv_bfloat16, 0>, (const void*)counts_kernel<__nv_bfloat16, 1>, (const void*)counts_kernel<__nv_bfloat16, 2>, (const void*)counts_kernel<__nv_bfloat16, 4>,
+         (const void*)counts_kernel<__nv_bfloat16, 8>},
+        {(const void*)counts_kernel<__half, 0>, (const void*)counts_kernel<__half, 1>, (const void*)counts_kernel<__half, 2>, (const void*)counts_kernel<__half, 4>, (const void*)counts_kernel<__half, 8>}};
+    // blocks of a row: as many as its counters need, and more while the device has room and each block still has 8192 logits; where those would not run all at once,
+    // or would be too many, one block has a whole row
+    const long long vectors = ((long long)a.V + 7 + 7) / 8;
+    int size = 0;
+    while ((vectors + C - 1) / C > CHUNK) C *= 2;
+    if (C > MAX_CLUSTER || (C > 1 && (long long)a.rows * C > sms)) C = 1;
+    else {
+      while (C < MAX_CLUSTER && (long long)a.rows * 2 * C <= sms && vectors / C > 1024) C *= 2;
+      const int nv = ((int)((vectors + C - 1) / C) + THREADS - 1) / THREADS;
+      size = nv <= 1 ? 1 : nv <= 2 ? 2 : nv <= 4 ? 3 : 4;
+    }
+    k = kernels[a.dtype == ETXB_F16][size]; which = 5 * (a.dtype == ETXB_F16) + size;
     cfg.dynamicSmemBytes = sizeof(Counts);
   }
   at.val.clusterDim.x = (unsigned)C; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;

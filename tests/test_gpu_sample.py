@@ -124,6 +124,49 @@ def test_masks_empty_rows_infinities_and_ties(V, dtype):
 
 
 @pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("off,V", [(0, 524288), (3, 524240)])
+def test_values_that_occur_more_often_than_16_bits_hold(off, V, dtype):
+    lowest = torch.finfo(dtype).min
+    big = rows(12, 524288, dtype, 15)
+    l = big[:, off:off + V]
+    l[0] = lowest; l[0, 70001:200000] = 3.0
+    l[1] = lowest
+    l[2] = -0.0
+    l[3] = 0.0; l[3, ::2] = -0.0
+    l[4] = 2.5; l[4, 1::2] = -0.0; l[4, 3::4] = 0.0
+    l[5] = NEG; l[5, V - 70000:] = -1.0
+    l[6] = float("nan"); l[6, 123456:123460] = 4.0
+    l[7] = float("inf"); l[7, :300000] = 1.0
+    l[8] = 1.0; l[8, 32767:65535] = 2.0; l[8, 131071:196606] = 0.5
+    l[9, 100:400000] = lowest
+    l[10, 5000:77000] = 11.0
+    u = [0.5, 0.4999, 0.9, 0.2, 0.613, 0.7, 0.31, 0.777, 0.4001, 0.55, 0.123, 0.987]
+    for T, k, p, mp in ((1.0, 0, 1.0, 0.0), (0.8, 100001, 1.0, 0.0), (1.0, 0, 0.8013, 0.0), (0.0, 0, 1.0, 0.0), (3.0, 0, 1.0, 0.5)):
+        check(l, u, T, k, p, mp, exact_margin=False)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_more_rows_than_blocks_at_once(dtype):
+    """So many long rows that a block has a whole one; the same rows a few at a time are shared by several blocks."""
+    B, V = 150, 66003
+    l = rows(B, V, dtype, 16, masked=0.3)
+    l[7] = l[7].abs().neg(); l[9] = torch.finfo(dtype).min; l[11] = NEG
+    u = torch.rand(B, device=DEV, generator=torch.Generator(device=DEV).manual_seed(17))
+    T = torch.tensor([(0.0, 0.7, 1.0, 2.5)[i % 4] for i in range(B)], device=DEV)
+    k = torch.tensor([(0, 50, 30000)[i % 3] for i in range(B)], dtype=torch.int32, device=DEV)
+    p = torch.tensor([(1.0, 0.9)[i % 2] for i in range(B)], device=DEV)
+    m = torch.tensor([(0.0, 0.0, 0.0, 0.0, 0.01)[i % 5] for i in range(B)], device=DEV)
+    r = sample(l, u, T, k, p, m)
+    for b in range(0, B, 3):
+        few = sample(l[b:b + 3], u[b:b + 3].clone(), T[b:b + 3], k[b:b + 3], p[b:b + 3], m[b:b + 3])
+        assert torch.equal(r.tokens[b:b + 3], few.tokens) and torch.equal(r.kept[b:b + 3], few.kept)
+        assert bool(((r.logprobs[b:b + 3] == few.logprobs) | ((r.logprobs[b:b + 3] - few.logprobs).abs() <= 2 ** -18)).all())
+    for b in range(0, B, 10):
+        tok, lp, n, margin = oracle(l[b].float().cpu().numpy(), float(u[b]), float(T[b]), int(k[b]), float(p[b]), float(m[b]))
+        assert margin > 1e-11 and (int(r.tokens[b]), int(r.kept[b])) == (tok, n)
+
+
+@pytest.mark.parametrize("dtype", ALL)
 def test_settings_off_the_range(dtype):
     """Negative and not-a-number settings do what the documentation says: no cut, greedy for the temperature."""
     nan = float("nan")

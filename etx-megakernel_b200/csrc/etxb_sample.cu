@@ -7,15 +7,18 @@
 //   min-p   those with w_r >= min_p
 // so together they keep the first n (at least one).  Drawn is the first token whose inclusive sum exceeds u * W_n.
 //
-// The sums have to be right next to every border, and the order of atomics must not change them.
+// The sums have to be right next to every border, and the order of atomics must not change them.  The bytes alone are 0.05 us for a row of 151936 and 12 us for 256;
+// what bounds it is the way from one step of the definition to the next: blocks of a row that wait for each other, sums over all values, a place looked up in them.
 //
 // Logits of 16 bits (counts_kernel).  A row has at most 65536 different values, and a real one some thousands: the row is counted value by value, exactly, with
 // 16-bit counters in shared memory, and then one exp in 64 bits per value that occurs, and sums over values in their order, give all three cuts and the
 // draw.  Nothing is sorted.  A row belongs to a cluster of C blocks, each of which counts a part of it; values are joined through distributed shared
 // memory, 32 neighbouring ones (a group) at a time, and only groups that occur.
+//   32 rows of 151936 22 us (6 of them counting, at 0.2 clocks a logit; a lookup 1), one row 15, 256 rows 90 (870 GB/s), 8 rows of 4000 14.
 // Logits of 32 bits (sums_kernel).  Bins by the first 11 bits of the value, then the next 11 and the last 10 of one bin: three passes for a border.  A bin has a
 // number of tokens and a sum of weights, which are integers: exp in 64 bits times 2^S with S = 62 - ceil(log2 V), so that a row's sum fits 63 bits, is
 // exact whatever the order, and a weight is off by 2^-(S+1) <= 2^-43 of the largest.
+//   13 rows of 50257 37 us without cuts, 45 with top-k and top-p; 256 rows of 151936 522 and 434: three atomics and an exp in 64 bits a logit.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -107,8 +110,7 @@ struct Counts {
 static_assert(sizeof(Counts) <= 231424, "a block's shared memory");
 
 // NV > 0: a block has NV vectors a thread, which stay in registers.  NV = 0: one block counts a whole row, whatever its length, in pieces of PIECE vectors;
-// before a counter could pass its 16 bits, what stands above 32767 in any of them goes to a list.  (A row of 151936 in 4 blocks that wait for each other, 256
-// rows: 194 us; in one: see the launch.)
+// before a counter could pass its 16 bits, what stands above 32767 in any of them goes to a list.
 template <typename T, int NV>
 __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_args a) {
   using K = Key16<sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u>;
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
         if (K::is(k)) mx = max(mx, k == MINUS_ZERO ? ZERO : k);
       }
   };
-  // No branch for a logit (with one for "-inf" and one for the lowest number 0.46 clocks each, so 0.2; the atomics alone are 0.14).  Masked ones, -inf or the type's lowest
+  // No branch for a logit (with one for "-inf" and one for the lowest number 0.46 clocks each, so 0.2; the atomics alone, into 65536 counters, 0.14).  Masked ones, -inf or the type's lowest
   // number, are most of some rows and would wait for each other: the first are not counted, the others without memory.
   const uint32_t hist = (uint32_t)__cvta_generic_to_shared(s.hist);
   auto count = [&]() {
@@ -524,7 +526,7 @@ struct Sums {
   unsigned long long wm[WARPS], wmm[WARPS];
   uint32_t maxkey, live, kept_min, here;
   unsigned long long mass_min;
-  uint32_t bin, before_count, n;
+  uint32_t bin, before_count, n, found;
   unsigned long long before_mass;
   uint32_t part[2][LIST], n_part[2], list[LIST];                    // the values of one of the first bins: this block's, and the row's
 };
@@ -536,9 +538,10 @@ __device__ __forceinline__ double log_weight(const Row& r, uint32_t key) {
   const double d = (double)value_of(key) - r.max;
   return d == d ? d * r.inv_t : 0.0;          // (inf - inf: the largest itself)
 }
+__device__ __noinline__ double exponential(double x) { return exp(x); }   // (one place in the code: three inlined were slower by a twentieth)
 __device__ __forceinline__ double real_weight(const Row& r, uint32_t key) {
   const double d = (double)value_of(key) - r.max;
-  return d < 0.0 ? (d == -INFINITY ? 0.0 : exp(d * r.inv_t)) : 1.0;     // (beside an infinite logit a finite one has none, at any temperature)
+  return d < 0.0 ? (d == -INFINITY ? 0.0 : exponential(d * r.inv_t)) : 1.0;     // (beside an infinite logit a finite one has none, at any temperature)
 }
 __device__ __forceinline__ unsigned long long weight(const Row& r, uint32_t key) { return __double2ull_rn(real_weight(r, key) * r.scale); }
 
@@ -560,15 +563,20 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
   clear();
   __syncthreads();
   uint32_t mx = 0u, live = 0u;
-  // 8 logits a thread at once: their loads are on the way together
+  // four loads ahead
   auto for_all = [&](auto use) {
-    for (int i = i0 + tid; i < i1; i += 8 * THREADS) {
-      float v[8];
+    auto at = [&](int i) { return i < i1 ? l[i] : -INFINITY; };
+    float x[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = i + j * THREADS < i1 ? l[i + j * THREADS] : -INFINITY;
+    for (int j = 0; j < 4; ++j) x[j] = at(i0 + tid + j * THREADS);
+#pragma unroll 1
+    for (int i = i0 + tid; i < i1; i += 4 * THREADS)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) use(key_of(v[j]));
-    }
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t k = key_of(x[j]);
+        x[j] = at(i + (4 + j) * THREADS);
+        use(k);
+      }
   };
   for_all([&](uint32_t key) { mx = max(mx, key); live += key ? 1u : 0u; });
   mx = __reduce_max_sync(~0u, mx); live = __reduce_add_sync(~0u, live);
@@ -711,39 +719,58 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
         find_bin(1, nb, how, rank, x, cb, mb);
         if (s.bin == ~0u) return false;       // (cannot be: the sums of a bin are the bin's)
         prefix = (prefix << bits) | s.bin; cb = s.before_count; mb = s.before_mass;
+        if (few && level == 1 && s.n == 1u) { // one token: its value needs no more bins
+          for (uint32_t i = tid; i < in_bin; i += THREADS) if (s.list[i] >> 10 == prefix) s.found = s.list[i];
+          __syncthreads();
+          prefix = s.found;
+          break;
+        }
       }
       place_key = prefix; place_before = cb; place_mass = mb; place_count = s.n;
       return true;
     };
     uint32_t n = live;
     unsigned long long Wn = find_bin(0, BINS, BY_RANK, ~0u, 0.0, 0u, 0ull);
-    if (st.k > 0 && (uint32_t)st.k < live) {
-      lookup(BY_RANK, (uint32_t)st.k - 1u, 0.0);
-      n = (uint32_t)st.k;
-      Wn = place_mass + (unsigned long long)(n - place_before) * weight(w, place_key);
-    }
-    if (st.top_p < 1.f) {
-      const double x = (double)st.top_p * (double)Wn;
-      uint32_t np = 1u;
-      unsigned long long Wp = (unsigned long long)w.scale;
-      if (x > 0.0 && lookup(BY_MASS_BEFORE, 0u, x)) {
-        const unsigned long long y = weight(w, place_key);
-        const double q = ceil((x - (double)place_mass) / (double)y);
-        const uint32_t in = (uint32_t)fmin(fmax(q, 1.0), (double)place_count);
-        np = place_before + in; Wp = place_mass + in * y;
+    // top-k, top-p, the draw, and the last token that is kept where rounding next to the last border asks for it
+#pragma unroll 1
+    for (int stage = 0; stage < 4; ++stage) {
+      int how = BY_RANK;
+      uint32_t rank = 0u;
+      double x = 0.0;
+      if (stage == 0) {
+        if (!(st.k > 0 && (uint32_t)st.k < live)) continue;
+        rank = (uint32_t)st.k - 1u;
+      } else if (stage == 1) {
+        if (!(st.top_p < 1.f)) continue;
+        how = BY_MASS_BEFORE; x = (double)st.top_p * (double)Wn;
+        if (!(x > 0.0)) { n = 1u; Wn = (unsigned long long)w.scale; continue; }
+      } else if (stage == 2) {
+        if (st.min_p > 0.f && n_min < n) {
+          n = n_min ? n_min : 1u;
+          Wn = n_min ? mass_min : (unsigned long long)w.scale;
+        }
+        how = BY_MASS_UPTO; x = st.u * (double)Wn;
+      } else {
+        if (place_before + nth < n) break;
+        rank = n - 1u;
       }
-      if (np < n) { n = np; Wn = Wp; }
-    }
-    if (st.min_p > 0.f && n_min < n) {
-      n = n_min ? n_min : 1u;
-      Wn = n_min ? mass_min : (unsigned long long)w.scale;
-    }
-    const double x = st.u * (double)Wn;
-    const bool found = lookup(BY_MASS_UPTO, 0u, x);
-    if (found) nth = (uint32_t)fmin(fmax(floor((x - (double)place_mass) / (double)weight(w, place_key)), 0.0), (double)(place_count - 1u));
-    if (!found || place_before + nth >= n) {                        // rounding next to the last border: the last token that is kept
-      lookup(BY_RANK, n - 1u, 0.0);
-      nth = n - 1u - place_before;
+      const bool found = lookup(how, rank, x);
+      const unsigned long long y = weight(w, place_key);
+      if (stage == 0) {
+        n = (uint32_t)st.k;
+        Wn = place_mass + (unsigned long long)(n - place_before) * y;
+      } else if (stage == 1) {
+        uint32_t np = 1u;
+        unsigned long long Wp = (unsigned long long)w.scale;
+        if (found) {
+          const uint32_t in = (uint32_t)fmin(fmax(ceil((x - (double)place_mass) / (double)y), 1.0), (double)place_count);
+          np = place_before + in; Wp = place_mass + in * y;
+        }
+        if (np < n) { n = np; Wn = Wp; }
+      } else if (stage == 2) {
+        if (found) nth = (uint32_t)fmin(fmax(floor((x - (double)place_mass) / (double)y), 0.0), (double)(place_count - 1u));
+        else { place_before = n; nth = 0u; }                        // (rounding next to the last border)
+      } else nth = n - 1u - place_before;
     }
     at = place_key;
     logp = (float)(log_weight(w, at) - log((double)Wn / w.scale));
@@ -757,7 +784,7 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
   // its nth token, by index: a warp has 32nd parts of the block's part
   const int per = (i1 - i0 + WARPS - 1) / WARPS, w0 = i0 + warp * per, w1 = min(i1, w0 + per);
   uint32_t c = 0u;
-#pragma unroll 8
+#pragma unroll 4
   for (int i = w0 + lane; i < w1; i += 32) c += key_of(l[i]) == at ? 1u : 0u;
   c = __reduce_add_sync(~0u, c);
   if (tid == 0) s.here = 0u;
@@ -821,12 +848,13 @@ extern "C" int32_t etxb_sample(int device, const etxb_sample_args* args, size_t 
         {(const void*)counts_kernel<__nv_bfloat16, 0>, (const void*)counts_kernel<__nv_bfloat16, 1>, (const void*)counts_kernel<__nv_bfloat16, 2>, (const void*)counts_kernel<__nv_bfloat16, 4>,
          (const void*)counts_kernel<__nv_bfloat16, 8>},
         {(const void*)counts_kernel<__half, 0>, (const void*)counts_kernel<__half, 1>, (const void*)counts_kernel<__half, 2>, (const void*)counts_kernel<__half, 4>, (const void*)counts_kernel<__half, 8>}};
-    // blocks of a row: as many as its counters need, and more while the device has room and each block still has 8192 logits; where those would not run all at once,
-    // or would be too many, one block has a whole row
+    // Blocks of a row: as many as its counters need, and more while the device has room and each block still has 8192 logits.  Where more than twice the device's blocks
+    // would come of it, or too many for a cluster, one block has a whole row (rows of 151936, four blocks each / one, us: 64 rows 42.6 / 46.5, the largest of them
+    // 24 / 31; 100 rows 88 / 47; 256 rows 191 / 90).
     const long long vectors = ((long long)a.V + 7 + 7) / 8;
     int size = 0;
     while ((vectors + C - 1) / C > CHUNK) C *= 2;
-    if (C > MAX_CLUSTER || (C > 1 && (long long)a.rows * C > sms)) C = 1;
+    if (C > MAX_CLUSTER || (C > 1 && (long long)a.rows * C > 2 * sms)) C = 1;
     else {
       while (C < MAX_CLUSTER && (long long)a.rows * 2 * C <= sms && vectors / C > 1024) C *= 2;
       const int nv = ((int)((vectors + C - 1) / C) + THREADS - 1) / THREADS;

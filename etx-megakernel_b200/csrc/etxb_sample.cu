@@ -14,7 +14,7 @@
 // 16-bit counters in shared memory, and then one exp in 64 bits per value that occurs, and sums over values in their order, give all three cuts and the
 // draw.  Nothing is sorted.  A row belongs to a cluster of C blocks, each of which counts a part of it; values are joined through distributed shared
 // memory, 32 neighbouring ones (a group) at a time, and only groups that occur.
-//   32 rows of 151936 22 us (6 of them counting, at 0.2 clocks a logit; a lookup 1), one row 15, 256 rows 90 (870 GB/s), 8 rows of 4000 14.
+//   32 rows of 151936 21 us (4 of them counting, at 0.2 clocks a logit; a lookup 1), one row 14, 256 rows 78 (1 TB/s), 8 rows of 4000 14.
 // Logits of 32 bits (sums_kernel).  Bins by the first 11 bits of the value, then the next 11 and the last 10 of one bin: three passes for a border.  A bin has a
 // number of tokens and a sum of weights, which are integers: exp in 64 bits times 2^S with S = 62 - ceil(log2 V), so that a row's sum fits 63 bits, is
 // exact whatever the order, and a weight is off by 2^-(S+1) <= 2^-43 of the largest.
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
   const T* l = (const T*)a.logits + (long long)row * a.row_stride;
   const int shift = (int)((uintptr_t)l & 15) / 2, nvec = (shift + V + 7) / 8;
   const int v0 = (int)((long long)nvec * r / C), v1 = (int)((long long)nvec * (r + 1) / C);
-  auto keys_of = [&](int v, int end) {
+  auto bits_of = [&](int v, int end) {                              // (-inf beside the row)
     uint4 q = make_uint4(K::NOTHING, K::NOTHING, K::NOTHING, K::NOTHING);
     const int e = v * 8 - shift;
     if (v < end && e >= 0 && e + 8 <= V) q = __ldg((const uint4*)(l + e));
@@ -142,6 +142,10 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
       }
       q = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    return q;
+  };
+  auto keys_of = [&](int v, int end) {
+    const uint4 q = bits_of(v, end);
     return make_uint4(K::of_two(q.x), K::of_two(q.y), K::of_two(q.z), K::of_two(q.w));
   };
   uint4 key[N];
@@ -168,9 +172,8 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const uint32_t w = ((const uint32_t*)&key[i])[j >> 1], k = j & 1 ? w >> 16 : w & 0xffffu;
-        asm volatile("{\n .reg .pred p;\n setp.gt.u32 p, %0, 1;\n @p red.shared.add.u32 [%1], %2;\n}" ::
+        asm volatile("{\n .reg .pred p;\n setp.gt.u32 p, %1, 1;\n @p red.shared.add.u32 [%2], %3;\n @!p add.u32 %0, %0, %1;\n}" : "+r"(low) :
                          "r"(k - (K::LOWEST - 1u)), "r"(hist + ((k << 1) & 0x1fffcu)), "r"(k & 1u ? 0x10000u : 1u) : "memory");
-        low += k == K::LOWEST ? 1u : 0u;
       }
     }
   };
@@ -430,6 +433,13 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
   const int kept = s.kept;
   const bool mine = s.mine != 0;
   const uint32_t at_too = at == ZERO ? MINUS_ZERO : at;
+  // Most vectors have none: both halves of four words are looked at together, where a borrow from a lower half that is equal may take the upper one along.
+  auto some = [&](const uint4& q, uint32_t care, uint32_t is) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { const uint32_t x = ((&q.x)[j] & care) ^ is; m |= (x - 0x00010001u) & ~x; }
+    return (m & 0x80008000u) != 0u;
+  };
   auto matches = [&](const uint4& q) {
     uint32_t m = 0u;
 #pragma unroll
@@ -440,9 +450,13 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
     // a warp has a 32nd of the row, in the order of the indices
     uint32_t* cnt = (uint32_t*)s.list;
     const int per = (nvec + WARPS - 1) / WARPS, w0 = min(warp * per, nvec), w1 = min(w0 + per, nvec);
+    const uint32_t care = at == ZERO ? 0x7fff7fffu : ~0u, is = (at & 0x8000u ? at & 0x7fffu : ~at & 0xffffu) * 0x10001u;
     uint32_t c = 0u;
 #pragma unroll 4
-    for (int v = w0; v < w1; v += 32) c += (uint32_t)__popc(matches(keys_of(v + lane, w1)));
+    for (int v = w0; v < w1; v += 32) {
+      const uint4 q = bits_of(v + lane, w1);
+      if (some(q, care, is)) c += (uint32_t)__popc(matches(make_uint4(K::of_two(q.x), K::of_two(q.y), K::of_two(q.z), K::of_two(q.w))));
+    }
     c = __reduce_add_sync(~0u, c);
     if (lane == 0) cnt[warp] = c;
     __syncthreads();
@@ -452,6 +466,7 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
       for (int v = w0; v < w1; v += 32) {
         uint32_t m = matches(keys_of(v + lane, w1));
         const uint32_t n = (uint32_t)__popc(m);
+        if (!__any_sync(~0u, m != 0u)) continue;
         uint32_t upto = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(~0u, upto, o); if (lane >= o) upto += x; }
@@ -468,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
     uint32_t match[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      match[i] = matches(key[i]);
+      match[i] = at == ZERO || some(key[i], ~0u, at * 0x10001u) ? matches(key[i]) : 0u;
       const uint32_t c = __reduce_add_sync(~0u, (uint32_t)__popc(match[i]));
       if (lane == 0) cnt[i * WARPS + warp] = c;
     }
@@ -849,8 +864,8 @@ extern "C" int32_t etxb_sample(int device, const etxb_sample_args* args, size_t 
          (const void*)counts_kernel<__nv_bfloat16, 8>},
         {(const void*)counts_kernel<__half, 0>, (const void*)counts_kernel<__half, 1>, (const void*)counts_kernel<__half, 2>, (const void*)counts_kernel<__half, 4>, (const void*)counts_kernel<__half, 8>}};
     // Blocks of a row: as many as its counters need, and more while the device has room and each block still has 8192 logits.  Where more than twice the device's blocks
-    // would come of it, or too many for a cluster, one block has a whole row (rows of 151936, four blocks each / one, us: 64 rows 42.6 / 46.5, the largest of them
-    // 24 / 31; 100 rows 88 / 47; 256 rows 191 / 90).
+    // would come of it, or too many for a cluster, one block has a whole row (rows of 151936, us: 64 in four blocks each 40, the largest of them 21; 100 in one each 41, 25,
+    // where four each would take three rounds of the 21 that 32 rows take; 256 in one each 78).
     const long long vectors = ((long long)a.V + 7 + 7) / 8;
     int size = 0;
     while ((vectors + C - 1) / C > CHUNK) C *= 2;

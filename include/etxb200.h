@@ -215,7 +215,8 @@ enum { ETXB_BF16 = 0, ETXB_F16 = 1, ETXB_F32 = 2 };
  * them (p not below 1: all), min-p the ones with w_r >= min_p (not above 0: all); at least one is kept.  Drawn is the first token whose inclusive
  * sum exceeds u times the sum of the kept ones.  temperature not above 0: the first of the order.  u is taken as within [0, 1 - 2^-24].  A row without a
  * live token: token -1, log-probability -inf, kept 0.
- * Weights are summed as integers in steps of 2^-43 of the largest or finer: the outcome depends on no order of execution. */
+ * Weights are 64-bit numbers; 16-bit logits are counted value by value and summed in the order of the values, those of 32 bits are summed as integers in steps of
+ * 2^-43 of the largest or finer: the outcome depends on no order of execution. */
 #define ETXB_SAMPLE_MAX_V 524288
 typedef struct etxb_sample_args {
   const void* logits;          /* [rows][V], row_stride elements apart */

@@ -1,7 +1,7 @@
 """Drawing tokens (runtime.sample) against the definition in 64 bits, row by row on the CPU.
 
-Tokens and numbers of kept tokens are whole numbers and have to be equal: the weights of the kernel are off by at most 2^-43 of the largest, and no case
-here has a border within a millionth of its random number or share (checked for each row below).  A log-probability is the fp32 rounding of a sum of two
+Tokens and numbers of kept tokens are whole numbers and have to be equal: the weights of the kernel are off by at most 2^-43 of the largest for
+fp32 and by roundings of 64-bit numbers for 16 bits, and no border lies within 1e-11 of the sum from a random number or a share (checked for each row below).  A log-probability is the fp32 rounding of a sum of two
 64-bit numbers; |value| < 64 gives an error of at most 2^-24 * 64 from the rounding and 1e-9 from the weights."""
 import math
 

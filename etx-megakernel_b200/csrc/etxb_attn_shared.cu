@@ -915,13 +915,15 @@ extern "C" int32_t etxb_attn_shared(int device, const etxb_attn_shared_args* arg
   P.a.group_first = nullptr;
   memset(&P.groups, 0, sizeof P.groups);
   memcpy(P.groups.first, a.group_first, (size_t)(a.groups + 1) * 4);
-  static encode_fn encode = nullptr;
+  static std::atomic<encode_fn> known{nullptr};
+  encode_fn encode = known.load(std::memory_order_relaxed);
   if (!encode) {
     cudaDriverEntryPointQueryResult q;
     void* fn = nullptr;
     ETXB_HOST_CU(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
     if (!fn || q != cudaDriverEntryPointSuccess) return refuse(ETXB_E_CUDA, "the driver does not offer cuTensorMapEncodeTiled");
     encode = (encode_fn)fn;
+    known.store(encode, std::memory_order_relaxed);
   }
   const cuuint64_t dim[3] = {BS, (cuuint64_t)a.NKV * a.HD, (cuuint64_t)a.pages}, str[2] = {BS * 2, (cuuint64_t)a.v_stride * 2};
   const cuuint32_t box[3] = {BS, (cuuint32_t)a.HD, 1}, one[3] = {1, 1, 1};

@@ -279,7 +279,15 @@ static void hold(etxb_pool& p, const std::vector<int32_t>& fresh) {
   p.n_free -= (int32_t)fresh.size();
   if (!fresh.empty() && fresh.front() == p.lowest) p.lowest = fresh.back() + 1;      // (they were the lowest free ones)
 }
-static int32_t carry_out(etxb_pool& p, etxb_pages_args& a, void* stream) { return p.update(p.device, &a, sizeof a, stream); }
+// (The books change once, when the call is made: replayed, it would write pages that are others' by then.)
+static int32_t carry_out(etxb_pool& p, etxb_pages_args& a, void* stream) {
+  if (p.update == etxb_pages_update) {
+    cudaStreamCaptureStatus captured = cudaStreamCaptureStatusNone;
+    ETXB_HOST_CU(cudaStreamIsCapturing((cudaStream_t)stream, &captured));
+    if (captured != cudaStreamCaptureStatusNone) return refuse(ETXB_E_ARG, "calls that change the books are not captured");
+  }
+  return p.update(p.device, &a, sizeof a, stream);
+}
 static int32_t rows_once(const etxb_pool& p, const int32_t* rows, int32_t n) {
   if (n < 0 || (n && !rows)) return refuse(ETXB_E_ARG, "a list is null");
   std::vector<uint8_t> seen(p.length.size(), 0);

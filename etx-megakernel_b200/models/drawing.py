@@ -20,12 +20,12 @@ def run(prog, n: int, first: int, pos: int, rows: int, sampling: Sampling, sync_
     stream = getattr(prog, "_draw_stream", None)
     if stream is None:
         stream = prog._draw_stream = torch.cuda.Stream(dev)
-    stream.wait_stream(torch.cuda.current_stream(dev))
     logits, tin, tout = b["logits"].view(rows, -1), b["token_in"].view(-1, rows), b["token_out"].view(-1, rows)
+    logprobs = torch.empty((n - first, rows), dtype=torch.float32, device=dev)      # (the caller's: of the caller's stream)
+    stream.wait_stream(torch.cuda.current_stream(dev))
     try:
         with torch.cuda.stream(stream):
             u = sampling.numbers(n - first, rows, dev)
-            logprobs = torch.empty((n - first, rows), dtype=torch.float32, device=dev)
             for t in range(n):
                 prog.session.set_step(tok=t, pos=pos + t, write_next=0)
                 prog.session.launch(stream.cuda_stream)

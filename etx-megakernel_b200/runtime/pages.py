@@ -82,6 +82,16 @@ def copy_pages(src, dst, src_ids, dst_ids, stream=None) -> None:
     _check(L.load().etxb_pages_update(index, C.byref(a), _BYTES, stream_handle(index, stream, (*src, *dst))))
 
 
+class _Books:
+    """A pool of the library, given back with the last PagePool that refers to it (a copied object is a second one)."""
+
+    def __init__(self, lib, handle):
+        self.lib, self.handle = lib, handle
+
+    def __del__(self):
+        self.lib.etxb_pool_destroy(self.handle)
+
+
 class PagePool:
     """The pages of a cache and the sequences that hold them.
 
@@ -89,7 +99,7 @@ class PagePool:
     Forked sequences share the full pages of what they have in common; a page that is shared is never written, since only full pages are.  Pages are
     given out lowest first.  Which pages are whose is kept on the host; a call changes the tables and copies pages in one launch on its stream, so the
     steps that read them follow on the same stream (or wait for it).  A call that fails changes nothing: ValueError for what cannot be asked,
-    EtxbError (E_FULL) where pages or rows run out."""
+    EtxbError (E_FULL) where pages or rows run out.  Calls that change tables are not captured into a graph: a replay would change what is others' by then."""
 
     def __init__(self, tensors, max_seqs: int, max_pages: int, tables=None, page_len: int = 16):
         self.tensors = _pool("tensors", tensors)
@@ -105,14 +115,10 @@ class PagePool:
         a.tables, a.table_stride, a.table_rows, a.table_width = tables.data_ptr(), max(tables.stride(0), max_pages), max_seqs, max_pages
         self._lib, self._h = L.load(), C.c_void_p()
         _check(self._lib.etxb_pool_create(self._index, C.byref(a), _BYTES, page_len, self._carrier(), C.byref(self._h)))
+        self._books = _Books(self._lib, self._h)
 
     def _carrier(self):
         return None                                             # (the library's own etxb_pages_update)
-
-    def __del__(self):
-        if getattr(self, "_h", None):
-            self._lib.etxb_pool_destroy(self._h)
-            self._h = None
 
     def _stream(self, stream):
         if stream is None:
@@ -164,7 +170,7 @@ class PagePool:
         _check(self._lib.etxb_pool_extend(self._h, rows, lengths, len(rows), self._stream(stream)))
 
     def fork(self, row: int, n: int, length: int | None = None, stream=None) -> list:
-        """n new sequences that continue `row` from `length` positions on (None: all of it): the full pages are shared, the last, partly filled one is
+        """n new sequences that continue `row` from `length` positions on (None: all of it; positions that are written by then): the full pages are shared, the last, partly filled one is
         copied for each.  Returns their rows."""
         if length is not None and length < 0:
             raise ValueError(f"fork: from {length} positions")

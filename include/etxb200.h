@@ -265,12 +265,12 @@ int32_t etxb_pages_update(int device, const etxb_pages_args* args, size_t bytes,
 /* A pool: which pages are whose.  A sequence is a row of the tables with a length in positions; its pages are given out lowest first.  Forked sequences
  * share the full pages of what they have in common, and the last, partly filled one is copied for each; a shared page is never written, since only full
  * pages are shared.  The books are the host's; what changes on the device (tables, copied pages) goes through one etxb_pages_update on the call's stream.
- * A call that fails changes nothing (ETXB_E_ARG; ETXB_E_FULL: no free pages or rows).  Calls on one pool exclude one another.
+ * A call that fails changes nothing (ETXB_E_ARG; ETXB_E_FULL: no free pages or rows).  Calls on one pool exclude one another; none is captured into a graph.
  *   create   `layout`: t[].dst and its strides, n_tensors, layers, dst_pages, tables, table_stride, table_rows, table_width (the rest is ignored).
  *            update: what carries the changes out, null: etxb_pages_update (a host without the device gives its own)
  *   open     a new sequence with pages for `length` positions
  *   extend   pages up to lengths[i] positions for rows[i] (never fewer than it has; each row once)
- *   fork     n sequences that continue `row` from `length` positions on (-1: all of them); rows: [n], theirs
+ *   fork     n sequences that continue `row` from `length` positions on (-1: all of them), which are written by then; rows: [n], theirs
  *   close    the sequences end: pages that nobody else holds are free (contents and table entries stay as they are)
  *   compact  moves pages until the ones in use are the lowest, the highest into the lowest hole first; moved: how many, may be null
  *   row      *length = -1 for a row without a sequence; pages: [capacity], its first pages; n: how many it has.  Pointers may be null

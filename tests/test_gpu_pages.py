@@ -140,6 +140,22 @@ def test_many_rows_and_captured_calls():
     assert bool((dst[0][:, [8, 0]] == 123).all())
 
 
+def test_books_are_not_captured():
+    k, = pool_tensors(1, 40, [(8,)], 12)
+    pool = PagePool([k], 6, 5)
+    r = pool.open(37)
+    before, g = pool.tables.clone(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        x = k + 1
+        for call in (lambda: pool.open(20), lambda: pool.fork(r, 2), lambda: pool.extend([r], 60)):
+            with pytest.raises(ValueError, match="not captured"):
+                call()
+    g.replay()
+    assert pool.rows() == [r] and pool.length_of(r) == 37 and pool.free_pages == 37 and torch.equal(pool.tables, before) and torch.equal(x, k + 1)
+    assert pool.fork(r, 2) == [1, 2]
+
+
 def test_renumbering_in_several_launches():
     """5000 moves (a launch lists 1975 of them beside the rows): every table entry is renumbered once."""
     k, = pool_tensors(1, 12000, [(8,)], 11)

@@ -223,3 +223,16 @@ def test_host_tensors_are_refused():
         copy_pages([torch.zeros(1, 2, 8)], [torch.zeros(1, 2, 8)], [0], [1])
     with pytest.raises(ValueError, match="CUDA tensor"):
         PagePool([torch.zeros(1, 2, 8)], 1, 1)
+
+
+def test_a_copied_pool_is_the_same_pool(on_host):
+    import copy
+    import gc
+    pool = HostPool([torch.zeros((1, 8, 4), dtype=torch.int64)], 3, 4, page_len=4)
+    r = pool.open(6)
+    other = copy.copy(pool)
+    del pool
+    gc.collect()
+    assert other.rows() == [r] and other.open(4) == 1 and other.free_pages == 5
+    with pytest.raises((TypeError, ValueError)):
+        copy.deepcopy(other)

@@ -6,6 +6,7 @@ from __future__ import annotations
 import ctypes as C
 import struct
 from array import array
+from functools import lru_cache
 from itertools import accumulate
 
 import torch
@@ -16,7 +17,17 @@ from ._call import cuda_tensor, raw_stream, same_device, stream_handle
 MAX_SEQS = 1024
 _BF16, _I32 = (torch.bfloat16,), (torch.int32,)
 _T, _BYTES = torch.Tensor, C.sizeof(L.AttnSharedArgs)
-_pack, _WORK = struct.Struct("11PN6q8ifi").pack, 10                # (the structure's fields in order, quicker than through ctypes; where `work` stands)
+_pack = struct.Struct("11PN6q8ifi").pack                           # (the structure's fields in order, quicker than through ctypes)
+
+
+@lru_cache(maxsize=1024)
+def _work_bytes(index, first, seqs, groups, NH, NKV, HD, pages, width, prefix_width):
+    """What the library asks for; it depends on nothing but these sizes (first: the groups' beginnings, as bytes)."""
+    n = C.c_size_t()
+    rc = L.load().etxb_attn_shared_work(index, _pack(*[0] * 8, C.cast(C.c_char_p(first), C.c_void_p).value, *[0] * 9, seqs, groups, NH, NKV, HD, pages, width, prefix_width, 1.0, 0), _BYTES, C.byref(n))
+    if rc:
+        L.check(rc)
+    return n.value
 _BAD = {1: "a table names a page outside the cache", 2: "a length lies outside its table", 4: "a wait inside the kernel ran past two seconds"}
 
 
@@ -85,19 +96,14 @@ def attn_shared(q, kc, vc, tables, lens, prefix_tables, prefix_lens, groups=None
         raise ValueError(f"attn_shared: at most {MAX_SEQS} sequences and groups")
     first = array("i", (0, *accumulate(sizes)))
     page = HD * NKV * 16
-    a = [q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), tables.data_ptr(), lens.data_ptr(), prefix_tables.data_ptr(), prefix_lens.data_ptr(),
-         first.buffer_info()[0], 0 if status is None else status.data_ptr(), 0, 0,
-         q.stride(0) if seqs > 1 else NH * HD, out.stride(0) if seqs > 1 else NH * HD, kc.stride(0) if pages > 1 else page, vc.stride(0) if pages > 1 else page,
-         tables.stride(0), prefix_tables.stride(0), seqs, n_groups, NH, NKV, HD, pages, t[1], p[1], HD ** -0.5 if scale is None else float(scale), 0]
-    lib, n, work = L.load(), C.c_size_t(), None
-    rc = lib.etxb_attn_shared_work(index, _pack(*a), _BYTES, C.byref(n))
-    if rc:
-        L.check(rc)
-    if n.value:                                                  # of this call alone: torch keeps it from others until the stream has passed
-        work = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        a[_WORK:_WORK + 2] = work.data_ptr(), n.value
+    n = _work_bytes(index, first.tobytes(), seqs, n_groups, NH, NKV, HD, pages, t[1], p[1])
+    work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None      # of this call alone: torch keeps it from others until the stream has passed
+    a = _pack(q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), tables.data_ptr(), lens.data_ptr(), prefix_tables.data_ptr(), prefix_lens.data_ptr(),
+              first.buffer_info()[0], 0 if status is None else status.data_ptr(), work.data_ptr() if n else 0, n,
+              q.stride(0) if seqs > 1 else NH * HD, out.stride(0) if seqs > 1 else NH * HD, kc.stride(0) if pages > 1 else page, vc.stride(0) if pages > 1 else page,
+              tables.stride(0), prefix_tables.stride(0), seqs, n_groups, NH, NKV, HD, pages, t[1], p[1], HD ** -0.5 if scale is None else float(scale), 0)
     handle = raw_stream(index) if stream is None else stream_handle(index, stream, (q, out, kc, vc, tables, lens, prefix_tables, prefix_lens, status, work))
-    rc = lib.etxb_attn_shared(index, _pack(*a), _BYTES, handle)
+    rc = L.load().etxb_attn_shared(index, a, _BYTES, handle)
     if rc:
         L.check(rc)
     return out

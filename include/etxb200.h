@@ -309,7 +309,7 @@ typedef struct etxb_attn_shared_args {
   int32_t reserved;
 } etxb_attn_shared_args;
 int32_t etxb_attn_shared(int device, const etxb_attn_shared_args* args, size_t bytes, void* cuda_stream);
-/* The bytes of `work` a call with these sizes needs (pointers are not looked at). */
+/* The bytes of `work` a call with these sizes needs (of the pointers only group_first is looked at). */
 int32_t etxb_attn_shared_work(int device, const etxb_attn_shared_args* args, size_t bytes, size_t* work_bytes);
 
 #ifdef __cplusplus

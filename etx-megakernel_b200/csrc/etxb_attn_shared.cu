@@ -25,7 +25,7 @@
 // at once, so products, softmax and copies of neighbouring tiles and segments overlap.  Every wait is bounded, and every role waits for every phase of a barrier.
 //
 // Measured (32 q heads of 128): 2 sequences over 131000 shared positions, 8 kv heads, 125 us, 4.3 TB/s (539 MB: 83 us); 64 over 32500 103 us (199 MB: 30 us; products: 21);
-// 32 over 8150, 4 kv heads, 36 us; 4 over 1024 20 us, mostly the host's.  A tile takes 2900 to 3000 clocks: its bytes 2900 from HBM with all SMs at it, its products 1800.  Tried and slower: one set of softmax warps; P in columns of its own (softmax waits for P V);
+// 32 over 8150, 4 kv heads, 36 us; 4 over 1024 18 us, mostly the host's.  A tile takes 2900 to 3000 clocks: its bytes 2900 from HBM with all SMs at it, its products 1800.  Tried and slower: one set of softmax warps; P in columns of its own (softmax waits for P V);
 // the second kernel launched ahead of the first one's end (its blocks wait on the SMs).  Contexts of their own, a short segment each, take 4500 clocks a tile, most of it the way from Q to the first product.
 #include <cuda.h>
 #include <cuda_bf16.h>

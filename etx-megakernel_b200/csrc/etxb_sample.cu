@@ -18,7 +18,7 @@
 // Logits of 32 bits (sums_kernel).  Bins by the first 11 bits of the value, then the next 11 and the last 10 of one bin: three passes for a border.  A bin has a
 // number of tokens and a sum of weights, which are integers: exp in 64 bits times 2^S with S = 62 - ceil(log2 V), so that a row's sum fits 63 bits, is
 // exact whatever the order, and a weight is off by 2^-(S+1) <= 2^-43 of the largest.
-//   13 rows of 50257 37 us without cuts, 45 with top-k and top-p, 10 of them a lookup; 256 rows of 151936 522 and 434, where bins have more than LIST tokens.  Four copies
+//   13 rows of 50257 36 us without cuts, 44 with top-k and top-p, 8 of them a lookup; 256 rows of 151936 528 and 438, where bins have more than LIST tokens.  Four copies
 //   of the first bins, for four lanes each, gave nothing, nor did an exp in 32 bits (1 us): it is the passes and what the blocks wait for between them.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -649,16 +649,18 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
     uint32_t n_min = 0u;
     unsigned long long mass_min = 0ull;
     for (int c = 0; c < C; ++c) { n_min += *cluster.map_shared_rank(&s.kept_min, c); mass_min += *cluster.map_shared_rank(&s.mass_min, c); }
-    // the bin (in descending order) that a lookup falls into, given the tokens and mass before all of them; the mass of all
-    auto find_bin = [&](int level, int nbins, int how, uint32_t rank, double x, uint32_t c0, unsigned long long m0) -> unsigned long long {
-      uint32_t c[2], ci;
-      unsigned long long m[2], mi;
+    // A thread's two bins (in descending order), with the tokens and the mass of those before them.
+    struct Two { uint32_t c[2], before; unsigned long long m[2], mass; };
+    unsigned long long total = 0ull;
+    auto scan = [&](int level, int nbins) {
+      Two b;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int i = nbins - 1 - (2 * tid + k);
-        c[k] = i >= 0 ? s.all_count[level][i] : 0u; m[k] = i >= 0 ? s.all_mass[level][i] : 0ull;
+        b.c[k] = i >= 0 ? s.all_count[level][i] : 0u; b.m[k] = i >= 0 ? s.all_mass[level][i] : 0ull;
       }
-      ci = c[0] + c[1]; mi = m[0] + m[1];
+      uint32_t ci = b.c[0] + b.c[1];
+      unsigned long long mi = b.m[0] + b.m[1];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t y = __shfl_up_sync(~0u, ci, o);
@@ -667,7 +669,6 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
       }
       __syncthreads();
       if (lane == 31) { s.wc[warp] = ci; s.wm[warp] = mi; }
-      if (tid == 0) s.bin = ~0u;
       __syncthreads();
       uint32_t cw = s.wc[lane];
       unsigned long long mw = s.wm[lane];
@@ -677,24 +678,33 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
         const unsigned long long z = __shfl_up_sync(~0u, mw, o);
         if (lane >= o) { cw += y; mw += z; }
       }
-      const unsigned long long total = __shfl_sync(~0u, mw, 31);
+      total = __shfl_sync(~0u, mw, 31);
       const uint32_t cb = __shfl_sync(~0u, cw, (warp + 31) & 31);
       const unsigned long long mb = __shfl_sync(~0u, mw, (warp + 31) & 31);
-      ci = c0 + (warp ? cb : 0u) + ci - c[0] - c[1]; mi = m0 + (warp ? mb : 0ull) + mi - m[0] - m[1];
+      b.before = (warp ? cb : 0u) + ci - b.c[0] - b.c[1]; b.mass = (warp ? mb : 0ull) + mi - b.m[0] - b.m[1];
+      return b;
+    };
+    // the bin that a lookup falls into, given the tokens and mass before all of them: s.bin, or ~0
+    auto pick = [&](const Two& b, int nbins, int how, uint32_t rank, double x, uint32_t c0, unsigned long long m0) {
+      __syncthreads();                        // (the last lookup's bin is read)
+      if (tid == 0) s.bin = ~0u;
+      __syncthreads();
+      uint32_t ci = c0 + b.before;
+      unsigned long long mi = m0 + b.mass;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        if (falls(how, rank, x, ci, c[k], mi, mi + m[k])) { s.bin = (uint32_t)(nbins - 1 - (2 * tid + k)); s.before_count = ci; s.before_mass = mi; s.n = c[k]; }
-        ci += c[k]; mi += m[k];
+        if (falls(how, rank, x, ci, b.c[k], mi, mi + b.m[k])) { s.bin = (uint32_t)(nbins - 1 - (2 * tid + k)); s.before_count = ci; s.before_mass = mi; s.n = b.c[k]; }
+        ci += b.c[k]; mi += b.m[k];
       }
       __syncthreads();
-      return total;
     };
+    const Two first = scan(0, BINS);          // (the same for every lookup)
     uint32_t place_key = 0u, place_before = 0u, place_count = 0u;
     unsigned long long place_mass = 0ull;
     uint32_t held = ~0u;                      // the bin whose tokens s.list has
     int buf = 0;
     auto lookup = [&](int how, uint32_t rank, double x) {
-      find_bin(0, BINS, how, rank, x, 0u, 0ull);
+      pick(first, BINS, how, rank, x, 0u, 0ull);
       if (s.bin == ~0u) return false;
       uint32_t prefix = s.bin, cb = s.before_count;
       unsigned long long mb = s.before_mass;
@@ -732,7 +742,7 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
           for_all(take);
           join(1);
         }
-        find_bin(1, nb, how, rank, x, cb, mb);
+        pick(scan(1, nb), nb, how, rank, x, cb, mb);
         if (s.bin == ~0u) return false;       // (cannot be: the sums of a bin are the bin's)
         prefix = (prefix << bits) | s.bin; cb = s.before_count; mb = s.before_mass;
         if (few && level == 1 && s.n == 1u) { // one token: its value needs no more bins
@@ -746,7 +756,7 @@ __global__ void __launch_bounds__(THREADS) sums_kernel(const etxb_sample_args a)
       return true;
     };
     uint32_t n = live;
-    unsigned long long Wn = find_bin(0, BINS, BY_RANK, ~0u, 0.0, 0u, 0ull);
+    unsigned long long Wn = total;            // (of the first bins: the last scan is theirs)
     // top-k, top-p, the draw, and the last token that is kept where rounding next to the last border asks for it
 #pragma unroll 1
     for (int stage = 0; stage < 4; ++stage) {

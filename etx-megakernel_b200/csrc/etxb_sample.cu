@@ -14,7 +14,7 @@
 // 16-bit counters in shared memory, and then one exp in 64 bits per value that occurs, and sums over values in their order, give all three cuts and the
 // draw.  Nothing is sorted.  A row belongs to a cluster of C blocks, each of which counts a part of it; values are joined through distributed shared
 // memory, 32 neighbouring ones (a group) at a time, and only groups that occur.
-//   32 rows of 151936 21 us (4 of them counting, at 0.2 clocks a logit; a lookup 1), one row 14, 256 rows 78 (1 TB/s), 8 rows of 4000 14.
+//   32 rows of 151936 20 us (4 of them counting, at 0.2 clocks a logit; a lookup 1), one row 14, 256 rows 76 (1 TB/s), 8 rows of 4000 12.5.
 // Logits of 32 bits (sums_kernel).  Bins by the first 11 bits of the value, then the next 11 and the last 10 of one bin: three passes for a border.  A bin has a
 // number of tokens and a sum of weights, which are integers: exp in 64 bits times 2^S with S = 62 - ceil(log2 V), so that a row's sum fits 63 bits, is
 // exact whatever the order, and a weight is off by 2^-(S+1) <= 2^-43 of the largest.
@@ -94,15 +94,13 @@ struct Group {
 };
 struct Counts {
   uint32_t hist[32768];                                             // two counters a word
-  Group group[GROUPS];                                              // of the whole row: each block joins a C-th of them and tells the others
-  double before_mass[GROUPS + 1];                                   // of the groups above (index: from the largest value down)
-  uint32_t before_count[GROUPS + 1];
-  uint16_t list[GROUPS];                                            // of the groups this block joins, the ones that occur
-  uint32_t bits[GROUPS / 32], row_bits[GROUPS / 32];                // the groups that occur in this block's part; those of the row that this block joins
+  Group group[GROUPS];                                              // of the whole row, those that occur, from the largest value down: each block joins a C-th of them
+  double before_mass[GROUPS];                                       // and tells the others; of the groups before each
+  uint32_t before_count[GROUPS];
+  uint16_t list[GROUPS];                                            // which groups they are
+  uint32_t bits[GROUPS / 32], row_bits[GROUPS / 32];                // the groups that occur in this block's part; in the row
   uint32_t part_key[PARTS], part_count[PARTS], n_parts, low;        // (a whole row) counts that 16 bits do not hold
-  uint32_t wc[WARPS], wcm[WARPS];
-  double wm[WARPS], wmm[WARPS];
-  uint32_t maxkey, n_list;
+  uint32_t maxkey;
   uint32_t at, nth, here;                                           // what was drawn: a value, and which of its tokens in this block
   int kept, mine;
   float logp;
@@ -181,9 +179,8 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
   if constexpr (!WHOLE) fetch(v0, v1);
   if (!greedy) {
     for (int i = tid; i < 32768 / 4; i += THREADS) ((uint4*)s.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
-    for (int i = tid; i < (int)(sizeof s.group / 16); i += THREADS) ((uint4*)s.group)[i] = make_uint4(0u, 0u, 0u, 0u);
   }
-  if (tid == 0) { s.maxkey = 0u; s.n_list = 0u; s.n_parts = 0u; s.low = 0u; }
+  if (tid == 0) { s.maxkey = 0u; s.n_parts = 0u; s.low = 0u; }
   __syncthreads();
   if constexpr (!WHOLE) {
     if (greedy) largest(); else count();
@@ -281,24 +278,23 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
   if (greedy) {
     if (tid == 0) { s.at = maxkey; s.nth = 0u; s.kept = 1; s.logp = 0.f; s.mine = r == first_with_max; }
   } else {
-    // this block joins the groups g with g % C = r (the ones that occur lie close together): their list, then a warp a group
+    // the row's groups that occur, in descending order
     if (tid < GROUPS / 32) {
       uint32_t b = 0u;
       from_all(&s.bits[tid], uint32_t(), [&](int, uint32_t x) { b |= x; });
-      s.row_bits[tid] = b & (C == 1 ? ~0u : C == 2 ? 0x55555555u : C == 4 ? 0x11111111u : 0x01010101u) << r;
+      s.row_bits[tid] = b;
     }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < GROUPS / THREADS; ++i) {
-      const uint32_t b = s.row_bits[i * WARPS + warp];
-      uint32_t n = 0u;
-      if (lane == 0 && b) n = atomicAdd(&s.n_list, (uint32_t)__popc(b));
-      n = __shfl_sync(~0u, n, 0) + (uint32_t)__popc(b & ((1u << lane) - 1u));
-      if (b >> lane & 1u) s.list[n] = (uint16_t)(i * THREADS + tid);
-    }
+    static_assert(GROUPS == 2 * THREADS, "two words of 32 groups a warp");
+    const uint32_t bits0 = s.row_bits[warp], bits1 = s.row_bits[WARPS + warp], c0 = (uint32_t)__popc(s.row_bits[lane]), c1 = (uint32_t)__popc(s.row_bits[WARPS + lane]);
+    const uint32_t upper = __reduce_add_sync(~0u, c1), groups = upper + __reduce_add_sync(~0u, c0), above = ~((2u << lane) - 1u);
+    const uint32_t first1 = __reduce_add_sync(~0u, lane > warp ? c1 : 0u), first0 = upper + __reduce_add_sync(~0u, lane > warp ? c0 : 0u);
+    if (bits1 >> lane & 1u) s.list[first1 + (uint32_t)__popc(bits1 & above)] = (uint16_t)(THREADS + tid);
+    if (bits0 >> lane & 1u) s.list[first0 + (uint32_t)__popc(bits0 & above)] = (uint16_t)tid;
     __syncthreads();
-    for (uint32_t i = warp; i < s.n_list; i += WARPS) {
-      const uint32_t g = s.list[i], k = g * 32u + 31u - (uint32_t)lane;                            // lanes from the group's largest value down
+    // each block joins every C-th, a warp a group
+    for (uint32_t i = (uint32_t)(r + C * warp); i < groups; i += (uint32_t)(C * WARPS)) {
+      const uint32_t k = s.list[i] * 32u + 31u - (uint32_t)lane;                                   // lanes from the group's largest value down
       const uint32_t n = tokens_of(k);
       const double w = n ? weight(k) : 0.0;
       const bool in = n && w >= (double)st.min_p;
@@ -307,64 +303,42 @@ __global__ void __launch_bounds__(THREADS, 1) counts_kernel(const etxb_sample_ar
       for (int o = 16; o; o >>= 1) { m += __shfl_xor_sync(~0u, m, o); mm += __shfl_xor_sync(~0u, mm, o); }
       Group x;
       x.mass = m; x.mass_min = mm; x.count = __reduce_add_sync(~0u, n); x.count_min = __reduce_add_sync(~0u, in ? n : 0u);
-      if (lane < C) *cluster.map_shared_rank(&s.group[g], lane) = x;
+      if (lane < C) *cluster.map_shared_rank(&s.group[i], lane) = x;
     }
     cluster.sync();
-    // every block goes over all groups in descending order, two a thread: tokens and mass before each
-    Group x[2];
-    x[0] = s.group[GROUPS - 1 - 2 * tid]; x[1] = s.group[GROUPS - 2 - 2 * tid];
-    uint32_t gb = x[0].count + x[1].count, cm = __reduce_add_sync(~0u, x[0].count_min + x[1].count_min);
-    const uint32_t own_c = gb;
-    double mb = x[0].mass + x[1].mass, mm = x[0].mass_min + x[1].mass_min;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(~0u, gb, o);
-      const double z = __shfl_up_sync(~0u, mb, o);
-      if (lane >= o) { gb += y; mb += z; }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mm += __shfl_xor_sync(~0u, mm, o);
-    if (lane == 31) { s.wc[warp] = gb; s.wm[warp] = mb; s.wcm[warp] = cm; s.wmm[warp] = mm; }
-    gb -= own_c;
-    const double before = __shfl_up_sync(~0u, mb, 1);
-    __syncthreads();
-    {
-      // the warps' sums in order: each lane one of them
-      uint32_t c = s.wc[lane];
-      double m = s.wm[lane];
+    if (warp == 0) {
+      // tokens and mass before each group: a lane has a 32nd of them (a real row has some hundred groups; all warps and two barriers took 1.5 us)
+      const uint32_t per = (groups + 31u) / 32u, i0 = min(lane * per, groups), i1 = min(i0 + per, groups);
+      uint32_t own_c = 0u, total_min = 0u;
+      double own_m = 0.0, total_mm = 0.0;
+      for (uint32_t i = i0; i < i1; ++i) { const Group x = s.group[i]; own_c += x.count; own_m += x.mass; total_min += x.count_min; total_mm += x.mass_min; }
+      uint32_t cb = own_c;
+      double mb = own_m;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(~0u, c, o);
-        const double z = __shfl_up_sync(~0u, m, o);
-        if (lane >= o) { c += y; m += z; }
+        const uint32_t y = __shfl_up_sync(~0u, cb, o);
+        const double z = __shfl_up_sync(~0u, mb, o);
+        if (lane >= o) { cb += y; mb += z; }
       }
-      const uint32_t cw = __shfl_sync(~0u, c, (warp + 31) & 31);
-      const double mw = __shfl_sync(~0u, m, (warp + 31) & 31);
-      gb += warp ? cw : 0u;
-      mb = (lane ? before : 0.0) + (warp ? mw : 0.0);
-      s.before_count[2 * tid] = gb; s.before_mass[2 * tid] = mb;
-      s.before_count[2 * tid + 1] = gb + x[0].count; s.before_mass[2 * tid + 1] = mb + x[0].mass;
-      if (tid == THREADS - 1) { s.before_count[GROUPS] = __shfl_sync(1u << 31, c, 31); s.before_mass[GROUPS] = __shfl_sync(1u << 31, m, 31); }
-    }
-    __syncthreads();
-    if (warp == 0) {
-      uint32_t total_min = __reduce_add_sync(~0u, s.wcm[lane]);
-      double total_mm = s.wmm[lane];
 #pragma unroll
       for (int o = 16; o; o >>= 1) total_mm += __shfl_xor_sync(~0u, total_mm, o);
-      const uint32_t total = s.before_count[GROUPS];
-      const double total_m = s.before_mass[GROUPS];
+      total_min = __reduce_add_sync(~0u, total_min);
+      const uint32_t total = __shfl_sync(~0u, cb, 31);
+      const double total_m = __shfl_sync(~0u, mb, 31), up_m = __shfl_up_sync(~0u, mb, 1);
+      cb -= own_c; mb = lane ? up_m : 0.0;
+      for (uint32_t i = i0; i < i1; ++i) { s.before_count[i] = cb; s.before_mass[i] = mb; cb += s.group[i].count; mb += s.group[i].mass; }
+      __syncwarp();
       // A border: the group it falls into -- the last that begins at or before it, found 32 at a time -- and then the value in it, a lane each.
       uint32_t place_key = 0u, place_before = 0u, place_count = 0u;
       double place_mass = 0.0, place_weight = 1.0;
       auto lookup = [&](int how, uint32_t rank, double y) {
-        auto begins = [&](int i) { return how == BY_RANK ? s.before_count[i] <= rank : how == BY_MASS_BEFORE ? s.before_mass[i] < y : s.before_mass[i] <= y; };
+        auto begins = [&](uint32_t i) { return how == BY_RANK ? s.before_count[i] <= rank : how == BY_MASS_BEFORE ? s.before_mass[i] < y : s.before_mass[i] <= y; };
         // (beginnings do not fall, but by a rounding between two groups that hold next to nothing: the last one that holds is taken)
-        int i = 64 * (31 - __clz(__ballot_sync(~0u, begins(64 * lane)) | 1u));
-        i += 2 * (31 - __clz(__ballot_sync(~0u, begins(i + 2 * lane)) | 1u));
-        if (begins(i + 1)) ++i;
-        while (i > 0 && s.group[GROUPS - 1 - i].count == 0u) --i;     // (groups without tokens begin where the next one does)
-        const uint32_t k = (uint32_t)(GROUPS - 1 - i) * 32u + 31u - (uint32_t)lane, n = tokens_of(k);
+        uint32_t i = per * (31u - (uint32_t)__clz(__ballot_sync(~0u, lane * per < groups && begins(lane * per)) | 1u));
+        const uint32_t low = __ballot_sync(~0u, (uint32_t)lane < per && i + lane < groups && begins(i + lane)) | 1u;
+        const uint32_t high = __ballot_sync(~0u, 32u + lane < per && i + 32u + lane < groups && begins(i + 32u + lane));
+        i += high ? 63u - (uint32_t)__clz(high) : 31u - (uint32_t)__clz(low);
+        const uint32_t k = s.list[i] * 32u + 31u - (uint32_t)lane, n = tokens_of(k);
         const double w = n ? weight(k) : 0.0;
         uint32_t c = n;
         double m = (double)n * w;

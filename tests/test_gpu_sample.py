@@ -145,6 +145,27 @@ def test_values_that_occur_more_often_than_16_bits_hold(off, V, dtype):
         check(l, u, T, k, p, mp, exact_margin=False)
 
 
+@pytest.mark.parametrize("rows_, V", [(3, 65536), (90, 131072)])
+@pytest.mark.parametrize("dtype,T", [(torch.bfloat16, 4e37), (torch.float16, 1.5e4)])
+def test_every_value_occurs(dtype, T, rows_, V):
+    """All 16-bit patterns but the infinite ones, in any order, NaN among them; blocks that share rows, and one for each."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    bits = torch.where(bits == float("inf"), torch.ones_like(bits), bits)
+    g = torch.Generator().manual_seed(31)
+    l = torch.stack([bits.repeat(V // 65536)[torch.randperm(V, generator=g)] for _ in range(3)]).to(DEV)
+    l = l.repeat(rows_ // 3, 1)
+    u = torch.rand(rows_, generator=g).tolist()
+    for k, p, mp in ((0, 1.0, 0.0), (30001, 0.7, 0.0), (0, 0.6, 0.9)):
+        if rows_ == 3:
+            check(l, u, T, k, p, mp)
+            continue
+        r = sample(l, torch.tensor(u, device=DEV), T, k, p, mp)
+        few = sample(l[3:6], torch.tensor(u[3:6], device=DEV), T, k, p, mp)
+        assert torch.equal(r.tokens[3:6], few.tokens) and torch.equal(r.kept[3:6], few.kept) and torch.equal(r.logprobs[3:6], few.logprobs)
+        tok, _, n, margin = oracle(l[0].float().cpu().numpy(), u[0], T, k, p, mp)
+        assert margin > 1e-11 and (int(r.tokens[0]), int(r.kept[0])) == (tok, n)
+
+
 @pytest.mark.parametrize("dtype", ALL)
 def test_more_rows_than_blocks_at_once(dtype):
     """So many long rows that a block has a whole one; the same rows a few at a time are shared by several blocks."""

@@ -47,6 +47,26 @@ def test_a_batch_over_pages_equals_one_over_blocks(weights, B):
     a.close(); b.close()
 
 
+@pytest.mark.parametrize("B,engine", [(3, "tc"), (24, "tc"), (4, "mma")])
+def test_long_contexts_over_scattered_pages(weights, B, engine):
+    """Contexts of several partitions, in pages that lie in any order: as blocks one after the other, and a fork as a sequence that was fed all of it."""
+    prompts = np.random.default_rng(B).integers(0, SMALL.V, (B, 170))
+    kw = dict(device=0, maxlen=256, steps=224, engine=engine)
+    a, b = BT.BatchProgram(SMALL, weights, B, **kw), BT.BatchProgram(SMALL, weights, B, pages=14 * B + 20, **kw)
+    assert [b.cache.open(0) for _ in range(B)] == list(range(B))
+    for t in range(169):                                                # a position at a time: the columns take their pages in turn
+        b.decode(prompts[:, t], t, 1)
+    want, got = a.generate(prompts, 30), b.decode(prompts[:, 169], 169, 30)
+    assert b.cache.pages_of(1)[:3] == [1, 1 + B, 1 + 2 * B]
+    assert np.array_equal(got, want) and np.array_equal(a.read("logits"), b.read("logits"))
+    b.release(range(1, B))
+    used = b.cache.length_of(0)                                         # column 0 goes on as two, the others as they would alone
+    assert used == 199 and b.fork(0, 1) == [1]
+    again = b.decode([5, 5] + [1] * (B - 2), used, 20)
+    assert np.array_equal(again[0], again[1])
+    a.close(); b.close()
+
+
 def test_forked_sequences_equal_sequences_of_their_own(weights):
     """A context of 37 positions adopted once and forked, against adopted for every column: the same logits to the bit at every length, the shared pages
     untouched, though the columns go different ways."""

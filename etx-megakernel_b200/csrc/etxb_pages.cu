@@ -305,6 +305,7 @@ extern "C" int32_t etxb_pool_create(int device, const etxb_pages_args* layout, s
   using namespace etxb_pages;
   if (!out || !layout || bytes != sizeof(etxb_pages_args)) return refuse(ETXB_E_ARG, "needs an etxb_pages_args");
   if (page_len < 1 || layout->dst_pages < 1 || layout->table_rows < 1 || layout->table_width < 1) return refuse(ETXB_E_ARG, "at least one page, row, entry and position");
+  if (layout->tables && layout->table_rows > 1 && layout->table_stride < layout->table_width) return refuse(ETXB_E_ARG, "rows of the tables overlap");
   if (device < 0 || device >= 64) return refuse(ETXB_E_ARG, "device index out of range");
   try {
     etxb_pool* p = new etxb_pool;

@@ -110,9 +110,11 @@ class PagePool:
             tables = torch.zeros((max_seqs, max_pages), dtype=torch.int32, device=dev)
         self.tables = cuda_tensor("tables", tables, (torch.int32,), (max_seqs, max_pages))
         same_device(dev, tables=tables)
+        if max_seqs > 1 and tables.stride(0) < max_pages:
+            raise ValueError(f"tables: rows overlap (stride {tables.stride(0)} below {max_pages})")
         self.page_len, self.n_pages, self._index = page_len, self.tensors[0].shape[1], self.tensors[0].get_device()
         a = _layout(self.tensors, self.tensors)
-        a.tables, a.table_stride, a.table_rows, a.table_width = tables.data_ptr(), max(tables.stride(0), max_pages), max_seqs, max_pages
+        a.tables, a.table_stride, a.table_rows, a.table_width = tables.data_ptr(), tables.stride(0) if max_seqs > 1 else max_pages, max_seqs, max_pages
         self._lib, self._h = L.load(), C.c_void_p()
         _check(self._lib.etxb_pool_create(self._index, C.byref(a), _BYTES, page_len, self._carrier(), C.byref(self._h)))
         self._books = _Books(self._lib, self._h)

@@ -236,3 +236,25 @@ def test_a_copied_pool_is_the_same_pool(on_host):
     assert other.rows() == [r] and other.open(4) == 1 and other.free_pages == 5
     with pytest.raises((TypeError, ValueError)):
         copy.deepcopy(other)
+
+
+@pytest.mark.parametrize("tables", [lambda: torch.zeros((1, 4), dtype=torch.int32).expand(3, 4), lambda: torch.zeros(20, dtype=torch.int32).as_strided((3, 4), (2, 1)),
+                                    lambda: torch.zeros(20, dtype=torch.int32).as_strided((3, 4), (3, 1))])
+def test_tables_whose_rows_overlap_are_refused(on_host, tables):
+    """The library is told where the rows lie: an expanded tensor has memory for one, and the others would be written behind it."""
+    with pytest.raises(ValueError, match="rows overlap"):
+        HostPool([torch.zeros((1, 6, 4))], 3, 4, tables=tables(), page_len=4)
+    one = torch.zeros(4, dtype=torch.int32).as_strided((1, 4), (0, 1))    # a single row has no stride to speak of
+    pool = HostPool([torch.zeros((1, 6, 4))], 1, 4, tables=one, page_len=4)
+    assert pool.open(7) == 0 and one[0, :2].tolist() == [0, 1]
+
+
+def test_the_library_refuses_tables_whose_rows_overlap():
+    import __graft_entry__ as ge
+    ge.build()
+    h, fn = C.c_void_p(), lib.load()
+    for stride in (0, 2, -3):
+        a = lib.PagesArgs(dst_pages=4, tables=1 << 24, table_stride=stride, table_rows=2, table_width=3)
+        assert fn.etxb_pool_create(0, C.byref(a), C.sizeof(a), 16, None, C.byref(h)) == 1 and b"overlap" in fn.etxb_last_error()
+    a.table_rows = 1
+    assert fn.etxb_pool_create(0, C.byref(a), C.sizeof(a), 16, None, C.byref(h)) == 0 and fn.etxb_pool_destroy(h) == 0

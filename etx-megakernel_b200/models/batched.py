@@ -321,6 +321,8 @@ class BatchProgram:
         """Every column takes its token of `tokens` [B] at position `pos`, then n_gen tokens per column; [B][n_gen].  Sequences grow as far as the steps
         reach; all have `pos` positions behind them (columns without a sequence run along)."""
         pool, n = self._paged(), n_gen
+        if pos < 0:
+            raise ValueError(f"decode: at position {pos}")
         if n + 2 > self.buf["token_in"].shape[0] or pos + n > self.maxlen or n_gen < 1:
             raise ValueError("sequence longer than the session was sized for")
         rows = pool.rows()

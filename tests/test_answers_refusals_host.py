@@ -1,0 +1,44 @@
+"""What a batch over pages refuses, on the host: the program's device part is left out (steps are recorded), its pool keeps its books in the library over CPU
+tensors.  A call that is refused runs no step and leaves rows, lengths and tables as they were."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import etx_megakernel_b200  # noqa: E402,F401
+from etx_megakernel_b200.models import batched as BT  # noqa: E402
+from etx_megakernel_b200.models import qwen as Q  # noqa: E402
+from tests.test_pages_host import HostPool, on_host  # noqa: E402,F401
+
+DIMS = Q.Dims(name="small", H=512, NH=8, NKV=2, HD=128, INTER=0, L=3, V=1504, qk_norm=True, moe=True, E=16, TOPK=4, MI=128, norm_topk=True)
+
+
+class Program(BT.BatchProgram):
+    def __init__(self, B=3, pages=20, maxlen=128, steps=64):
+        nblk = -(-maxlen // BT.BS)
+        self.d, self.B, self.pages, self.maxlen, self.steps, self.dev = DIMS, B, pages, maxlen, steps, torch.device("cpu")
+        self.buf = {"token_in": torch.zeros((steps, B), dtype=torch.int32), "block_tables": torch.full((B, nblk), pages, dtype=torch.int32),
+                    "logits": torch.zeros((B, DIMS.V)), "kc": torch.zeros((2, pages + 1, 8)), "vc": torch.zeros((2, pages + 1, 8))}
+        self.cache = HostPool([self.buf["kc"][:, :pages], self.buf["vc"][:, :pages]], B, nblk, tables=self.buf["block_tables"], page_len=BT.BS)
+        self.runs = []
+
+    def _run(self, fed, pos, n_gen, sync_every, sampling):
+        self.runs.append((fed.tolist(), pos, n_gen))
+        return np.zeros((self.B, n_gen), np.int32)
+
+    def state(self):
+        return [(r, self.cache.length_of(r), self.cache.pages_of(r)) for r in self.cache.rows()], self.buf["block_tables"].tolist(), self.runs
+
+
+@pytest.mark.parametrize("rows", [0, 1])
+@pytest.mark.parametrize("pos", [-1, -16, -(2 ** 31)])
+def test_decode_refuses_positions_below_0(on_host, rows, pos):  # noqa: F811
+    """Without a sequence nothing else names the position: tables would be read before their beginning, and the slot found there written."""
+    prog = Program()
+    for _ in range(rows):
+        prog.cache.open(5)
+    before = prog.state()
+    with pytest.raises(ValueError, match="position"):
+        prog.decode([1, 2, 3], pos, 4)
+    assert prog.state() == before
+    assert prog.decode([1, 2, 3], 5, 4).shape == (3, 4) and prog.runs == [([[1, 2, 3]], 5, 4)]

@@ -34,17 +34,30 @@ def same_device(device, **tensors):
             raise ValueError(f"{name} is on {t.device}, the call runs on {device}")
 
 
+def other_stream(index: int, stream):
+    """`stream` (a raw handle or a torch stream) as a torch stream of device `index`, or None where it is the current one (or None)."""
+    if stream is None:
+        return None
+    handle = int(getattr(stream, "cuda_stream", stream))
+    if handle == raw_stream(index):
+        return None
+    device = torch.device("cuda", index)
+    return torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+
+
+def lend(stream, tensors):
+    """The tensors' memory, which belongs to other streams, is kept until `stream` has passed what it was given so far when they are released."""
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+
+
 def stream_handle(index: int, stream, tensors) -> int:
     """The raw handle of the call's stream on device `index`: the current one, or `stream` (a raw handle or a torch stream), which the tensors' memory is
-    then kept for until it has passed the call."""
-    current = raw_stream(index)
-    if stream is None:
-        return current
-    handle = int(getattr(stream, "cuda_stream", stream))
-    if handle != current:
-        device = torch.device("cuda", index)
-        s = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
-        for t in tensors:
-            if t is not None:
-                t.record_stream(s)
-    return handle
+    then kept for until it has passed the call.  (For calls that allocate nothing: memory of the current stream's may still be written there by what was
+    queued before it was released.)"""
+    other = other_stream(index, stream)
+    if other is None:
+        return raw_stream(index)
+    lend(other, tensors)
+    return other.cuda_stream

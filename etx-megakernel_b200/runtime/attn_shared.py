@@ -12,7 +12,7 @@ from itertools import accumulate
 import torch
 
 from . import lib as L
-from ._call import cuda_tensor, raw_stream, same_device, stream_handle
+from ._call import cuda_tensor, lend, other_stream, raw_stream, same_device
 
 MAX_SEQS = 1024
 _BF16, _I32 = (torch.bfloat16,), (torch.int32,)
@@ -68,7 +68,8 @@ def attn_shared(q, kc, vc, tables, lens, prefix_tables, prefix_lens, groups=None
     out          bf16, shaped like q; returned
     status       int32 tensor [1] or None.  A page outside the cache or a length outside its table makes the outputs of the sequences concerned NaN and
                  sets a bit there, which `attn_shared_check` turns into an error
-    stream       a raw handle or torch stream; None is the current one
+    stream       a raw handle or torch stream; None is the current one.  What the call reads and is given to write has to be ready there; what it returns is
+                 memory of that stream, also kept for what the current one still does with it when it is released
 
     Scores, statistics and sums are fp32.  A sequence without any position has the output 0.  Equal inputs give equal outputs."""
     # What usually comes passes here in a few microseconds, which is what small calls take; all else goes through _check, which says what is wrong.
@@ -87,8 +88,6 @@ def attn_shared(q, kc, vc, tables, lens, prefix_tables, prefix_lens, groups=None
         shape, k, t, p, index = q.shape, kc.shape, tables.shape, prefix_tables.shape, q.get_device()
     seqs, pages, NKV, HD, n_groups = shape[0], k[0], k[1], 8 * k[2], p[0]
     NH = shape[1] if len(shape) == 3 else shape[1] // HD
-    if out is None:
-        out = torch.empty_like(q) if plain else torch.empty(shape, dtype=torch.bfloat16, device=q.device)
     sizes = (seqs,) if groups is None else [int(n) for n in groups]
     if len(sizes) != n_groups or min(sizes, default=0) < 0 or sum(sizes) != seqs:
         raise ValueError(f"groups: {n_groups} sizes of {seqs} sequences altogether, got {list(sizes)}")
@@ -97,12 +96,23 @@ def attn_shared(q, kc, vc, tables, lens, prefix_tables, prefix_lens, groups=None
     first = array("i", (0, *accumulate(sizes)))
     page = HD * NKV * 16
     n = _work_bytes(index, first.tobytes(), seqs, n_groups, NH, NKV, HD, pages, t[1], p[1])
-    work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None      # of this call alone: torch keeps it from others until the stream has passed
+    other = None if stream is None else other_stream(index, stream)
+    if other is None:
+        if out is None:
+            out = torch.empty_like(q) if plain else torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+        work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None  # of this call alone: torch keeps it from others until the stream has passed
+        handle = raw_stream(index)
+    else:
+        lend(other, (q, out, kc, vc, tables, lens, prefix_tables, prefix_lens, status))
+        with torch.cuda.stream(other):                            # (memory of the call's stream: the current one's may still be written there)
+            made = torch.empty(shape, dtype=torch.bfloat16, device=q.device) if out is None else None
+            work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        lend(torch.cuda.current_stream(index), (made,))
+        out, handle = made if out is None else out, other.cuda_stream
     a = _pack(q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), tables.data_ptr(), lens.data_ptr(), prefix_tables.data_ptr(), prefix_lens.data_ptr(),
               first.buffer_info()[0], 0 if status is None else status.data_ptr(), work.data_ptr() if n else 0, n,
               q.stride(0) if seqs > 1 else NH * HD, out.stride(0) if seqs > 1 else NH * HD, kc.stride(0) if pages > 1 else page, vc.stride(0) if pages > 1 else page,
               tables.stride(0), prefix_tables.stride(0), seqs, n_groups, NH, NKV, HD, pages, t[1], p[1], HD ** -0.5 if scale is None else float(scale), 0)
-    handle = raw_stream(index) if stream is None else stream_handle(index, stream, (q, out, kc, vc, tables, lens, prefix_tables, prefix_lens, status, work))
     rc = L.load().etxb_attn_shared(index, a, _BYTES, handle)
     if rc:
         L.check(rc)

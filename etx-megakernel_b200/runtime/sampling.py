@@ -11,7 +11,7 @@ from typing import NamedTuple
 import torch
 
 from . import lib as L
-from ._call import cuda_tensor, raw_stream, stream_handle, vector
+from ._call import cuda_tensor, lend, other_stream, raw_stream, vector
 
 _DT = {torch.bfloat16: L.DTYPES["bf16"], torch.float16: L.DTYPES["f16"], torch.float32: L.DTYPES["f32"]}
 MAX_V = 524288
@@ -53,7 +53,9 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=Non
     with itself exceeds u times the sum of the kept ones.  temperature 0: the largest logit.  Equal inputs give equal tokens, whatever else runs.
 
     temperature, top_k, top_p, min_p: numbers, or tensors [rows] (float32; top_k int32).  tokens / next_tokens: int32 tensors [rows] that take the tokens
-    (the second one them once more, 0 where there is none: the next step's input).  stream: a raw handle or torch stream; None is the current one."""
+    (the second one them once more, 0 where there is none: the next step's input).  stream: a raw handle or torch stream; None is the current one.  What
+    the call reads and is given to write has to be ready there; what it returns is memory of that stream, also kept for what the current one still does with it
+    when it is released."""
     if not (isinstance(logits, _T) and logits.is_cuda and logits.dtype in _DT and len(logits.shape) == 2 and (logits.shape[1] == 1 or logits.stride(1) == 1)):
         cuda_tensor("logits", logits, _DT, (None, None))          # (says what is wrong)
     rows, V = logits.shape
@@ -78,13 +80,23 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=Non
     mins, least = setting("min_p", min_p, torch.float32)
     if next_tokens is not None:
         keep.append(vector("next_tokens", next_tokens, torch.int32, rows, index))
-    logprobs = torch.empty_like(u)
-    kept = torch.empty_like(u, dtype=torch.int32)
-    if tokens is None:
-        tokens = torch.empty_like(kept)
+    if tokens is not None:
+        keep.append(vector("tokens", tokens, torch.int32, rows, index))
+    other = None if stream is None else other_stream(index, stream)
+    if other is None:
+        logprobs = torch.empty_like(u)
+        kept = torch.empty_like(u, dtype=torch.int32)
+        if tokens is None:
+            tokens = torch.empty_like(kept)
+        handle = raw_stream(index)
     else:
-        vector("tokens", tokens, torch.int32, rows, index)
-    handle = raw_stream(index) if stream is None else stream_handle(index, stream, (*keep, tokens, logprobs, kept))
+        with torch.cuda.stream(other):                            # (the results are of the call's stream: memory of the current one's may still be written there)
+            logprobs = torch.empty_like(u)
+            kept = torch.empty_like(u, dtype=torch.int32)
+            made = torch.empty_like(kept) if tokens is None else None
+        lend(other, keep)
+        lend(torch.cuda.current_stream(index), (logprobs, kept, made))
+        tokens, handle = made if tokens is None else tokens, other.cuda_stream
     a = _pack(logits.data_ptr(), u.data_ptr(), temperatures, ks, ps, mins, tokens.data_ptr(), 0 if next_tokens is None else next_tokens.data_ptr(), logprobs.data_ptr(),
               kept.data_ptr(), stride, rows, V, _DT[logits.dtype], k, temperature, p, least, 0)
     rc = L.load().etxb_sample(index, a, _BYTES, handle)

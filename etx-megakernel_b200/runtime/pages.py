@@ -107,7 +107,7 @@ class PagePool:
         if max_seqs < 1 or max_pages < 1 or page_len < 1:
             raise ValueError("PagePool: at least one sequence, page and position")
         if tables is None:
-            tables = torch.zeros((max_seqs, max_pages), dtype=torch.int32, device=dev)
+            tables = torch.zeros((max_seqs, max_pages), dtype=torch.int32).to(dev)      # (there when the pool is: its calls may come on any stream)
         self.tables = cuda_tensor("tables", tables, (torch.int32,), (max_seqs, max_pages))
         same_device(dev, tables=tables)
         if max_seqs > 1 and tables.stride(0) < max_pages:

@@ -5,7 +5,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import etx_megakernel_b200  # noqa: E402,F401
-from etx_megakernel_b200.runtime import sample  # noqa: E402
+from etx_megakernel_b200.runtime import PagePool, sample  # noqa: E402
 from tests.test_gpu_attn_shared import Case  # noqa: E402
 
 DEV = "cuda:0"
@@ -79,3 +79,15 @@ def test_captured_on_another_stream():
         g.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want) and all(torch.equal(x, y) for x, y in zip(r, drawn)) and all(bool((j == 7).all()) for j in junk)
+
+
+def test_a_pools_own_tables():
+    """Tables that the pool makes are there when it is, whatever its stream still has to do: a call on another stream does not wait for that."""
+    k, s = torch.zeros((1, 40, 8), device=DEV, dtype=torch.int16), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(LATER)
+    pool = PagePool([k], 4, 6)
+    row = pool.open(90, stream=s)
+    forks = pool.fork(row, 2, stream=s)
+    torch.cuda.synchronize()
+    assert all(pool.tables[r, :6].tolist() == pool.pages_of(r) for r in (row, *forks)) and pool.pages_of(row) == [0, 1, 2, 3, 4, 5]

@@ -7,9 +7,11 @@ from ..runtime import Sampling, sample
 
 
 def check(prog, n: int, rows: int, sampling: Sampling):
-    """Refuses what `run` would refuse at its first draw of n: settings, and random numbers of another shape."""
+    """Refuses what `run` would refuse at its first draw of n: settings, a seed, random numbers of another shape, type or place."""
     if sampling.given is not None:
         sampling.numbers(n, rows, prog.dev)
+    else:
+        sampling.numbers(0, rows, prog.dev)                             # (the seed)
     sample(prog.buf["logits"].view(rows, -1), torch.zeros(rows, device=prog.dev), sampling.temperature, sampling.top_k, sampling.top_p, sampling.min_p)
 
 

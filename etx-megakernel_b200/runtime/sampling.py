@@ -37,10 +37,13 @@ class Sampling:
 
     def numbers(self, steps: int, rows: int, device) -> torch.Tensor:
         """The random numbers of a run: [steps][rows] in [0, 1)."""
-        if self.given is not None:
-            if tuple(self.given.shape) != (steps, rows):
-                raise ValueError(f"given random numbers {tuple(self.given.shape)}, the run takes {(steps, rows)}")
-            return self.given
+        g, device = self.given, torch.device(device)
+        if g is not None:
+            if not isinstance(g, _T) or tuple(g.shape) != (steps, rows):
+                raise ValueError(f"given random numbers {tuple(g.shape) if isinstance(g, _T) else type(g).__name__}, the run takes {(steps, rows)}")
+            if g.dtype is not torch.float32 or g.device.type != device.type or device.index not in (None, g.device.index) or (rows > 1 and g.stride(1) != 1):
+                raise ValueError(f"given random numbers: {g.dtype} on {g.device} with strides {g.stride()}, the run takes adjoining float32 ones on {device}")
+            return g
         return torch.rand((steps, rows), device=device, generator=torch.Generator(device=device).manual_seed(self.seed))
 
 

@@ -7,7 +7,9 @@ torch = pytest.importorskip("torch")
 
 import etx_megakernel_b200  # noqa: E402,F401
 from etx_megakernel_b200.models import batched as BT  # noqa: E402
+from etx_megakernel_b200.models import drawing  # noqa: E402
 from etx_megakernel_b200.models import qwen as Q  # noqa: E402
+from etx_megakernel_b200.runtime import Sampling  # noqa: E402
 from tests.test_pages_host import HostPool, on_host  # noqa: E402,F401
 
 DIMS = Q.Dims(name="small", H=512, NH=8, NKV=2, HD=128, INTER=0, L=3, V=1504, qk_norm=True, moe=True, E=16, TOPK=4, MI=128, norm_topk=True)
@@ -42,3 +44,22 @@ def test_decode_refuses_positions_below_0(on_host, rows, pos):  # noqa: F811
         prog.decode([1, 2, 3], pos, 4)
     assert prog.state() == before
     assert prog.decode([1, 2, 3], 5, 4).shape == (3, 4) and prog.runs == [([[1, 2, 3]], 5, 4)]
+
+
+BAD_NUMBERS = [torch.zeros((4, 3), dtype=torch.float64), torch.zeros((4, 3), device="meta"), torch.zeros((4, 6))[:, ::2], torch.zeros((3, 4)), [[0.5] * 3] * 4]
+
+
+@pytest.mark.parametrize("given", BAD_NUMBERS)
+def test_decode_refuses_random_numbers_before_sequences_grow(on_host, monkeypatch, given):  # noqa: F811
+    monkeypatch.setattr(drawing, "sample", lambda *a, **k: None)        # (settings are looked at on the device)
+    prog = Program()
+    prog.cache.open(5)
+    before = prog.state()
+    with pytest.raises(ValueError, match="random numbers"):
+        prog.decode([1, 2, 3], 5, 4, sampling=Sampling(given=given))
+    assert prog.state() == before
+    with pytest.raises((TypeError, ValueError, RuntimeError)):
+        prog.decode([1, 2, 3], 5, 4, sampling=Sampling(seed="seven"))
+    assert prog.state() == before
+    prog.decode([1, 2, 3], 5, 4, sampling=Sampling(given=torch.zeros((4, 3))))
+    assert prog.cache.length_of(0) == 9

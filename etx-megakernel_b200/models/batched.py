@@ -17,6 +17,7 @@ then final norm (B tasks) -> lm_head (batched) -> argmax (B tasks).  All sequenc
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from dataclasses import replace
 
 import numpy as np
@@ -255,11 +256,17 @@ class BatchProgram:
         if n + 2 > self.buf["token_in"].shape[0] or n > self.maxlen:
             raise ValueError("sequence longer than the session was sized for")
         if self.cache is not None:
+            if P < 1 or n_gen < 0:
+                raise ValueError(f"generate: {n_gen} tokens behind prompts of {P}")
             if self.B * -(-n // BS) > self.pages:
                 raise ValueError(f"{self.B} sequences of {n} positions in {self.pages} pages")
+            if sampling is not None:
+                drawing.check(self, n_gen, self.B, sampling)                 # (before the sequences end)
             self.release(self.cache.rows())
-            for _ in range(self.B):
-                self.cache.open(n)
+            with self._ends_what_fails():
+                for _ in range(self.B):
+                    self.cache.open(n)
+                return self._run(prompts.T, 0, n_gen, sync_every, sampling)
         return self._run(prompts.T, 0, n_gen, sync_every, sampling)
 
     def _run(self, fed, pos: int, n_gen: int, sync_every: int, sampling):
@@ -288,6 +295,17 @@ class BatchProgram:
         if self.cache is None:
             raise ValueError("the program was built without pages")
         return self.cache
+
+    @contextmanager
+    def _ends_what_fails(self):
+        """Around what opens sequences and runs them: when it raises, they hold positions that were not written, and end."""
+        try:
+            yield
+        except BaseException:
+            if self.dev.type == "cuda":
+                torch.cuda.synchronize(self.dev)                             # (steps on their way still write the pages)
+            self.release(self.cache.rows())
+            raise
 
     def release(self, columns) -> None:
         """The columns' sequences end; the columns write to a page of nobody's until new ones begin there."""

@@ -63,3 +63,42 @@ def test_decode_refuses_random_numbers_before_sequences_grow(on_host, monkeypatc
     assert prog.state() == before
     prog.decode([1, 2, 3], 5, 4, sampling=Sampling(given=torch.zeros((4, 3))))
     assert prog.cache.length_of(0) == 9
+
+
+def no_such_setting(*a, **k):
+    raise ValueError("temperature: shape (4,), expected (3,)")
+
+
+@pytest.mark.parametrize("what", ["setting", "numbers", "pages", "long", "no prompt", "less than none", "fails"])
+def test_generate_over_pages_ends_no_sequence_for_nothing(on_host, monkeypatch, what):  # noqa: F811
+    """Refused calls leave the sequences; a run that fails ends the ones it opened, whose positions nobody has written."""
+    prog = Program()
+    monkeypatch.setattr(drawing, "sample", no_such_setting if what == "setting" else lambda *a, **k: None)
+    prog.cache.open(21)
+    prog.cache.open(40)
+    before = prog.state()
+    prompts, n, s = np.ones((3, 7), int), 5, Sampling()
+    if what == "numbers":
+        s = Sampling(given=torch.zeros((4, 3)))
+    elif what == "pages":
+        prompts = np.ones((3, 100), int)
+        prog.buf["token_in"] = torch.zeros((200, 3), dtype=torch.int32)
+        n = 29                                                          # 8 pages a sequence of 20
+    elif what == "long":
+        n = 70
+    elif what == "no prompt":
+        prompts = np.ones((3, 0), int)
+    elif what == "less than none":
+        prompts, n = np.ones((3, 1), int), -1
+    elif what == "fails":
+        def failing(*a):
+            raise RuntimeError("E_TIMEOUT")
+        prog._run = failing
+    with pytest.raises((ValueError, RuntimeError)) as e:
+        prog.generate(prompts, n, sampling=s)
+    if what == "fails":
+        assert "E_TIMEOUT" in str(e.value) and prog.cache.rows() == [] and prog.cache.free_pages == 20 and bool((prog.buf["block_tables"] == 20).all())
+    else:
+        assert isinstance(e.value, ValueError) and prog.state() == before
+    prog.__dict__.pop("_run", None)
+    assert prog.generate(np.ones((3, 7), int), 0).shape == (3, 0) and prog.cache.rows() == [0, 1, 2] and prog.cache.length_of(2) == 6

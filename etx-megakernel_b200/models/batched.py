@@ -327,8 +327,12 @@ class BatchProgram:
             raise ValueError(f"adopt: {length} positions of a cache of {d.L} layers, {d.NKV} kv heads of {d.HD}, {one.maxlen} positions on {one.dev}")
         column = pool.open(length)
         ids = pool.pages_of(column)
-        if ids:
-            copy_pages([one.buf["kc"], one.buf["vc"]], pool.tensors, list(range(len(ids))), ids)
+        try:
+            if ids:
+                copy_pages([one.buf["kc"], one.buf["vc"]], pool.tensors, list(range(len(ids))), ids)
+        except BaseException:                                                # (a cache of another layout, a shard's for one: nothing of it is here)
+            self.release([column])
+            raise
         return column
 
     def fork(self, column: int, n: int) -> list:

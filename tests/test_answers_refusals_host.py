@@ -9,7 +9,7 @@ import etx_megakernel_b200  # noqa: E402,F401
 from etx_megakernel_b200.models import batched as BT  # noqa: E402
 from etx_megakernel_b200.models import drawing  # noqa: E402
 from etx_megakernel_b200.models import qwen as Q  # noqa: E402
-from etx_megakernel_b200.runtime import Sampling  # noqa: E402
+from etx_megakernel_b200.runtime import Sampling, copy_pages  # noqa: E402
 from tests.test_pages_host import HostPool, on_host  # noqa: E402,F401
 
 DIMS = Q.Dims(name="small", H=512, NH=8, NKV=2, HD=128, INTER=0, L=3, V=1504, qk_norm=True, moe=True, E=16, TOPK=4, MI=128, norm_topk=True)
@@ -102,3 +102,29 @@ def test_generate_over_pages_ends_no_sequence_for_nothing(on_host, monkeypatch, 
         assert isinstance(e.value, ValueError) and prog.state() == before
     prog.__dict__.pop("_run", None)
     assert prog.generate(np.ones((3, 7), int), 0).shape == (3, 0) and prog.cache.rows() == [0, 1, 2] and prog.cache.length_of(2) == 6
+
+
+class One:
+    """What adopt and answers take of a one-sequence program."""
+
+    def __init__(self, kc=(2, 9, 8), dims=DIMS, maxlen=128):
+        self.d, self.maxlen, self.dev = dims, maxlen, torch.device("cpu")
+        self.buf = {"kc": torch.zeros(kc), "vc": torch.zeros(kc), "logits": torch.zeros(dims.V)}
+        self.fed = []
+
+    def generate(self, prompt, n_gen):
+        self.fed.append(list(prompt))
+
+
+@pytest.mark.parametrize("what", ["shape", "copy", "negative", "long", "pages"])
+def test_adopt_that_fails_opens_no_sequence(on_host, monkeypatch, what):  # noqa: F811
+    """A cache of another layout (a shard's, say) is refused by the copy, behind the opening of a column."""
+    def failing(*a, **k):
+        raise RuntimeError("E_CUDA")
+    monkeypatch.setattr(BT, "copy_pages", failing if what == "copy" else copy_pages)
+    prog = Program(pages=8)
+    prog.cache.open(21)
+    before = prog.state()[0]
+    with pytest.raises((ValueError, RuntimeError)):
+        prog.adopt(One((2, 9, 4) if what == "shape" else (2, 9, 8)), {"negative": -1, "long": 129, "pages": 100}.get(what, 20))
+    assert prog.state()[0] == before and prog.cache.free_pages == 6 and bool((prog.buf["block_tables"][1:] == 8).all())

@@ -319,12 +319,17 @@ class BatchProgram:
         if idle:
             self.buf["block_tables"][idle] = self.pages
 
+    def _takes(self, one, length: int):
+        d = one.d
+        if (d.L, d.NKV, d.HD) != (self.d.L, self.d.NKV, self.d.HD) or not 0 <= length <= one.maxlen or one.dev != self.dev or \
+                any(one.buf[n].shape[2:] != self.buf[n].shape[2:] for n in ("kc", "vc")):
+            raise ValueError(f"adopt: {length} positions of a cache of {d.L} layers, {d.NKV} kv heads of {d.HD}, {one.maxlen} positions, pages {tuple(one.buf['kc'].shape[2:])} on {one.dev}")
+
     def adopt(self, one, length: int) -> int:
         """A new sequence with the first `length` positions of a one-sequence program's cache (models.decode.DecodeProgram of the same model on the same
         GPU); returns its column."""
-        pool, d = self._paged(), one.d
-        if (d.L, d.NKV, d.HD) != (self.d.L, self.d.NKV, self.d.HD) or not 0 <= length <= one.maxlen or one.dev != self.dev:
-            raise ValueError(f"adopt: {length} positions of a cache of {d.L} layers, {d.NKV} kv heads of {d.HD}, {one.maxlen} positions on {one.dev}")
+        pool = self._paged()
+        self._takes(one, length)
         column = pool.open(length)
         ids = pool.pages_of(column)
         try:
@@ -360,20 +365,34 @@ class BatchProgram:
     def answers(self, one, prompt, n_gen: int, sampling, sync_every: int = 32):
         """B answers to one prompt: `one` (a DecodeProgram of the same weights) reads it, its cache is adopted and forked, and every column draws its own
         tokens.  Returns [B][n_gen]; log-probabilities in self.logprobs, [n_gen][B]."""
-        one.generate(prompt, 1)
+        self._paged()
+        prompt = [int(x) for x in prompt]
         P = len(prompt)
-        self.release(self._paged().rows())
-        self.fork(self.adopt(one, P), self.B - 1)
-        u = sampling.numbers(n_gen, self.B, self.dev)
-        logits = one.buf["logits"].view(1, -1).expand(self.B, -1).contiguous()
-        first = sample(logits, u[0], sampling.temperature, sampling.top_k, sampling.top_p, sampling.min_p)
-        tokens = first.tokens.cpu().numpy()
-        if n_gen == 1:
-            self.logprobs = first.logprobs[None]
-            return tokens[:, None]
-        rest = self.decode(tokens, P, n_gen - 1, sync_every, replace(sampling, given=u[1:]))
-        self.logprobs = torch.cat([first.logprobs[None], self.logprobs])
-        return np.concatenate([tokens[:, None], rest], axis=1)
+        total, full = P + n_gen - 1, P // BS
+        if P < 1 or n_gen < 1:
+            raise ValueError(f"answers: {n_gen} tokens to a prompt of {P}")
+        if total > self.maxlen or (n_gen > 1 and n_gen + 1 > self.buf["token_in"].shape[0]):
+            raise ValueError("sequence longer than the session was sized for")
+        if full + self.B * (-(-total // BS) - full) > self.pages:
+            raise ValueError(f"{self.B} answers of {n_gen} tokens to a prompt of {P} in {self.pages} pages")
+        self._takes(one, P)
+        if one.d.V != self.d.V:
+            raise ValueError(f"answers: a program of {one.d.V} tokens for one of {self.d.V}")
+        drawing.check(self, n_gen, self.B, sampling)                         # (all this before sequences end)
+        one.generate(prompt, 1)
+        self.release(self.cache.rows())
+        with self._ends_what_fails():
+            self.fork(self.adopt(one, P), self.B - 1)
+            u = sampling.numbers(n_gen, self.B, self.dev)
+            logits = one.buf["logits"].view(1, -1).expand(self.B, -1).contiguous()
+            first = sample(logits, u[0], sampling.temperature, sampling.top_k, sampling.top_p, sampling.min_p)
+            tokens = first.tokens.cpu().numpy()
+            if n_gen == 1:
+                self.logprobs = first.logprobs[None]
+                return tokens[:, None]
+            rest = self.decode(tokens, P, n_gen - 1, sync_every, replace(sampling, given=u[1:]))
+            self.logprobs = torch.cat([first.logprobs[None], self.logprobs])
+            return np.concatenate([tokens[:, None], rest], axis=1)
 
     def load_kv(self, layer: int, seq: int, K: np.ndarray, V: np.ndarray):
         """Pre-fill positions 0..ctx-1 of one layer of sequence `seq` from contiguous float32 (bf16-exact) [ctx][NKV][HD] arrays."""

@@ -8,6 +8,8 @@ from ..runtime import Sampling, sample
 
 def check(prog, n: int, rows: int, sampling: Sampling):
     """Refuses what `run` would refuse at its first draw of n: settings, a seed, random numbers of another shape, type or place."""
+    if not isinstance(sampling, Sampling):
+        raise ValueError(f"sampling: a runtime.Sampling, got {type(sampling).__name__}")
     if sampling.given is not None:
         sampling.numbers(n, rows, prog.dev)
     else:

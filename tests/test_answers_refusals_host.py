@@ -128,3 +128,53 @@ def test_adopt_that_fails_opens_no_sequence(on_host, monkeypatch, what):  # noqa
     with pytest.raises((ValueError, RuntimeError)):
         prog.adopt(One((2, 9, 4) if what == "shape" else (2, 9, 8)), {"negative": -1, "long": 129, "pages": 100}.get(what, 20))
     assert prog.state()[0] == before and prog.cache.free_pages == 6 and bool((prog.buf["block_tables"][1:] == 8).all())
+
+
+@pytest.mark.parametrize("what", ["setting", "numbers", "no setting", "none asked", "no prompt", "long", "steps", "pages", "other model", "other layers", "other layout", "fails"])
+def test_answers_end_no_sequence_for_nothing(on_host, monkeypatch, what):  # noqa: F811
+    """Sizes, pages, settings and the other program are looked at before anything ends or runs; what fails behind that ends the sequences it opened."""
+    class First:
+        tokens, logprobs = torch.tensor([3, 4, 5], dtype=torch.int32), torch.zeros(3)
+    monkeypatch.setattr(drawing, "sample", no_such_setting if what == "setting" else lambda *a, **k: First)
+    monkeypatch.setattr(BT, "sample", no_such_setting if what == "setting" else lambda *a, **k: First)
+    monkeypatch.setattr(BT, "copy_pages", lambda *a, **k: None)
+    prog = Program(pages=11)
+    prog.logprobs = torch.zeros((0, 3))
+    prog.cache.open(21)
+    prog.cache.open(40)
+    before = prog.state()
+    one, prompt, n, s = One(), list(range(33)), 31, Sampling()          # 2 pages shared, 2 for each answer's own: 8
+    if what == "numbers":
+        s = Sampling(given=torch.zeros((30, 3)))
+    elif what == "no setting":
+        s = None
+    elif what == "none asked":
+        n = 0
+    elif what == "no prompt":
+        prompt = []
+    elif what == "long":
+        n = 97
+    elif what == "steps":
+        n = 64
+    elif what == "pages":
+        n = 49                                                          # 81 positions: 2 + 3 * 4 pages
+    elif what == "other model":
+        one = One(dims=Q.Dims(**{**DIMS.__dict__, "V": 1600}))
+    elif what == "other layers":
+        one = One(dims=Q.Dims(**{**DIMS.__dict__, "L": 2}))
+    elif what == "other layout":
+        one = One((2, 9, 4))
+    elif what == "fails":
+        def failing(*a):
+            raise RuntimeError("E_TIMEOUT")
+        prog._run = failing
+    with pytest.raises((ValueError, RuntimeError)) as e:
+        prog.answers(one, prompt, n, s)
+    if what == "fails":
+        assert "E_TIMEOUT" in str(e.value) and prog.cache.rows() == [] and prog.cache.free_pages == 11 and bool((prog.buf["block_tables"] == 11).all())
+        return
+    assert isinstance(e.value, ValueError) and prog.state() == before and one.fed == []
+    monkeypatch.setattr(drawing, "sample", lambda *a, **k: First)
+    monkeypatch.setattr(BT, "sample", lambda *a, **k: First)
+    assert prog.answers(One(), list(range(33)), 31, Sampling())[:, 0].tolist() == [3, 4, 5]
+    assert [prog.cache.length_of(r) for r in prog.cache.rows()] == [63, 63, 63] and prog.cache.free_pages == 3 and prog.runs == [([[3, 4, 5]], 33, 30)]

@@ -390,7 +390,7 @@ class BatchProgram:
             if n_gen == 1:
                 self.logprobs = first.logprobs[None]
                 return tokens[:, None]
-            rest = self.decode(tokens, P, n_gen - 1, sync_every, replace(sampling, given=u[1:]))
+            rest = self.decode(np.maximum(tokens, 0), P, n_gen - 1, sync_every, replace(sampling, given=u[1:]))
             self.logprobs = torch.cat([first.logprobs[None], self.logprobs])
             return np.concatenate([tokens[:, None], rest], axis=1)
 

@@ -178,3 +178,16 @@ def test_answers_end_no_sequence_for_nothing(on_host, monkeypatch, what):  # noq
     monkeypatch.setattr(BT, "sample", lambda *a, **k: First)
     assert prog.answers(One(), list(range(33)), 31, Sampling())[:, 0].tolist() == [3, 4, 5]
     assert [prog.cache.length_of(r) for r in prog.cache.rows()] == [63, 63, 63] and prog.cache.free_pages == 3 and prog.runs == [([[3, 4, 5]], 33, 30)]
+
+
+def test_answers_go_on_behind_a_first_token_that_there_is_none(on_host, monkeypatch):  # noqa: F811
+    """A prompt whose logits allow no token: -1, and the step takes 0 for it, as behind every other token."""
+    class First:
+        tokens, logprobs = torch.tensor([-1, 7, -1], dtype=torch.int32), torch.zeros(3)
+    for mod in (drawing, BT):
+        monkeypatch.setattr(mod, "sample", lambda *a, **k: First)
+    monkeypatch.setattr(BT, "copy_pages", lambda *a, **k: None)
+    prog = Program()
+    prog.logprobs = torch.zeros((3, 3))
+    got = prog.answers(One(), [5, 6], 4, Sampling())
+    assert got[:, 0].tolist() == [-1, 7, -1] and prog.runs == [([[0, 7, 0]], 2, 3)]

@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
     }
   } else if (warp == W_COPY) {
     // ---- copies: a lane per page
-    uint32_t use = 0, sl = 0, round = 0, seg = 0;                   // running number of ring slots taken, the next one, how often it was before
+    uint32_t use = 0, sl = 0, round = 0, seg = 0, left_out = ~0u;    // running number of ring slots taken, the next one, how often it was before; a use without a copy
     bool ok = true, have = false;
     int vp = 0, vn = 0, vh = 0;                                     // the tile whose values follow
     auto put = [&](int n_pages, int page, int h, bool values) {
@@ -571,12 +571,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
       t += s.n;
     }
     if (have && ok) {                                               // the use behind the last K is left out
-      ++use;
+      left_out = use++;
       if (++sl == SLOTS) { sl = 0; ++round; }
       put(vn, vp, vh, true);
     }
-    // before the block ends, nothing is on its way into its memory any more (also when it gave up): the last use of every slot
-    const uint32_t left_out = have && use > 0 ? use - 2 : ~0u;
+    // before the block ends, nothing is on its way into its memory any more (also when it gave up, before or behind the use without a copy): the last copy
+    // into every slot.  (Earlier ones have come: a slot is taken again when it was read.)
     for (uint32_t u = use > SLOTS + 2 ? use - SLOTS - 2 : 0; u < use; ++u) {
       if (u == left_out || (u + SLOTS < use && u + SLOTS != left_out)) continue;
       const unsigned long long w0 = now_ns();

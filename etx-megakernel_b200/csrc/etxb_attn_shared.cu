@@ -98,6 +98,15 @@ __device__ __noinline__ bool bar_wait_on(uint32_t bar, uint32_t parity, volatile
   }
 }
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t n, volatile int* stop) { return bar_try(b, n & 1) || bar_wait_on(smem_u32(b), n & 1, stop); }
+// Waits for a phase whatever the others do, for what a block has on its way before it ends (with the same limit).
+__device__ __noinline__ void bar_drain(uint32_t bar, uint32_t parity) {
+  const unsigned long long t0 = now_ns();
+  uint32_t ok = 0;
+  while (!ok) {
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (now_ns() - t0 > WAIT_NS) break;
+  }
+}
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
@@ -290,7 +299,7 @@ __device__ __forceinline__ void segment_at(const Params& P, const Cum& c, int t,
 constexpr int SEGS = 8;                       // segments known ahead
 struct Shared {
   uint64_t full[MAX_SLOTS], empty[MAX_SLOTS];       // ring of key / value tiles: K0 K1 V0 K2 V1 .. (V of tile n: use 2 n + 2)
-  uint64_t s_full[3], p_full[3], pv_done[3], o_full[SETS], o_free, q_full[4], q_free[4], seg_full[SEGS], seg_free[SEGS], pair[SETS][4], m_full[3][4];
+  uint64_t s_full[3], p_full[3], pv_done[3], o_full[SETS], o_free, q_full[4], q_free[4], seg_full[SEGS], seg_free[SEGS], pair[SETS][4], m_full[3][4], drained[2];
   Segment seg[SEGS];
   float part[SETS][2][2][ROWS];               // maxima that the two warps of a row tell each other: by set, turn, half
   float m[3][ROWS];                           // each row's maximum after tile n, at n % 3
@@ -322,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
     for (int i = 0; i < SLOTS; ++i) { bar_init(&sh.full[i], 1); bar_init(&sh.empty[i], 1); }
     for (int i = 0; i < 3; ++i) { bar_init(&sh.s_full[i], 1); bar_init(&sh.p_full[i], SET_WARPS); bar_init(&sh.pv_done[i], 1); }
     for (int i = 0; i < 12; ++i) bar_init(&sh.m_full[i / 4][i % 4], 1);
-    for (int i = 0; i < SETS; ++i) bar_init(&sh.o_full[i], 1);
+    for (int i = 0; i < SETS; ++i) { bar_init(&sh.o_full[i], 1); bar_init(&sh.drained[i], 1); }
     bar_init(&sh.o_free, SET_WARPS);
     for (int i = 0; i < 4; ++i) { bar_init(&sh.q_full[i], 32); bar_init(&sh.q_free[i], 1); bar_init(&sh.pair[0][i], 2); bar_init(&sh.pair[1][i], 2); }
     for (int i = 0; i < SEGS; ++i) { bar_init(&sh.seg_full[i], 1); bar_init(&sh.seg_free[i], SETS * SET_WARPS + 3); }
@@ -579,8 +588,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
     // into every slot.  (Earlier ones have come: a slot is taken again when it was read.)
     for (uint32_t u = use > SLOTS + 2 ? use - SLOTS - 2 : 0; u < use; ++u) {
       if (u == left_out || (u + SLOTS < use && u + SLOTS != left_out)) continue;
-      const unsigned long long w0 = now_ns();
-      while (!bar_try(&sh.full[u % SLOTS], (u / SLOTS) & 1) && now_ns() - w0 < WAIT_NS) {}
+      bar_drain(smem_u32(&sh.full[u % SLOTS]), (u / SLOTS) & 1);
     }
   } else if (warp == W_QK) {
     // ---- S = Q K^T: one thread, and another one for O += P V, so that neither waits behind what the other waits for
@@ -619,6 +627,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
         bar_arrive(&sh.seg_free[seg % SEGS]);
         t += s.n;
       }
+      mma_commit(&sh.drained[0]);                                   // (a block that gives up has products on their way)
+      bar_drain(smem_u32(&sh.drained[0]), 0);
     }
     __syncwarp();
   } else if (warp == W_PV) {
@@ -678,6 +688,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
       if (lane == 0) bar_arrive(&sh.seg_free[seg % SEGS]);
       t += s.n;
     }
+    __syncwarp();
+    if (elect()) {
+      mma_commit(&sh.drained[1]);
+      bar_drain(smem_u32(&sh.drained[1]), 0);
+    }
+    __syncwarp();
   } else if (warp == W_Q) {
     // ---- the segments, and Q: their rows as [HD / 8][rows][8]: 128 rows of a prefix in all of the buffer, a sequence's 16 in one of four places of it
     uint32_t seg = 0, waited = 0;                                   // segments whose rows the products are known to be done with
@@ -935,6 +951,7 @@ extern "C" int32_t etxb_attn_shared(int device, const etxb_attn_shared_args* arg
   const int slot = P.y.tp * a.HD * 2, other = 256 + q_size(a.HD, P.y.qrows) + (a.groups + a.seqs + 1) * 8 + 2048;
   const int slots = (232448 - (int)sizeof(Shared) - 1024 - other) / slot & ~1;
   P.y.slots = slots > MAX_SLOTS ? MAX_SLOTS : slots;                // (four at least: 128 rows of Q and 1024 sequences leave 130 KB)
+  static_assert(232448 - (int)sizeof(Shared) - 1024 - (256 + ROWS * 256 * 2 + (2 * ETXB_SHARED_MAX_SEQS + 1) * 8 + 2048) >= 4 * 64 * 256 * 2, "a ring of four tiles");
   const int smem = other + P.y.slots * slot;
   static std::atomic<char> ready[2][64];
   ETXB_HOST_CU(etxb_host_smem(k, 232448 - (int)sizeof(Shared) - 1024, device, ready[a.HD > 128]));

@@ -47,11 +47,11 @@ struct Layout {
   int G, spt;                 // q heads per kv head; sequences whose rows fill a unit of a prefix
   int tp;                     // positions of a tile
   int workers;
-  int prows;                  // rows of a slot of a prefix
+  int prows;                  // rows of the largest unit of a prefix
   int slots, qrows;           // of the kernel's shared memory: tiles of keys or values in the ring (even), rows of Q kept for a prefix
-  int punits;                 // units of prefixes, counted generously (see prefix_unit); a unit's parts lie in the slots unit + worker
-  long long pslots, oslots;   // slots of prefixes / of own positions
-  float* pO; float* pml; float* oO; float* oml;      // [slot][HD / 4][rows][4], [slot][rows][2] (m in units of log2, l)
+  int punits;                 // units of prefixes, counted generously (see prefix_unit); a unit's parts have the numbers unit + worker
+  long long pslots, oslots;   // numbers of parts of prefixes / of own positions
+  float* pO; float* pml; float* oO; float* oml;      // of a part [HD / 4][rows][4], [rows][2] (m in units of log2, l), from the row on that part_row names
   int32_t* hdr;               // [pslots + oslots]: status bits of a segment
   int32_t* gave_up;           // [workers]: not 0 where one did
   int32_t* of;                // [units][2]: first and last worker that has tiles of a unit
@@ -249,6 +249,11 @@ __device__ __forceinline__ void share_of(int tp, int to, int W, int w, int& t0, 
   else if (w < wp + wo) { t0 = tp + share(to, w - wp, wo); t1 = tp + share(to, w - wp + 1, wo); }
 }
 
+// The first row of worker w's part of a unit whose rows have row0 others of units before them: parts of one unit lie `most` rows apart, the largest unit's number, and a
+// worker's part of the next unit begins at least the unit's own rows behind its part of this one.  (With `most` rows for every part, one large group beside a
+// thousand of one sequence took 567 MB for 43.)
+__device__ __forceinline__ long long part_row(int row0, int most, int w) { return (long long)row0 + (long long)most * w; }
+
 // The first unit of group g's prefix: no more units lie before it than sequences / spt + groups, for each kv head.
 __device__ __forceinline__ int prefix_unit(const Params& P, int g) { return (P.groups.first[g] / P.y.spt + g) * P.a.NKV; }
 
@@ -259,8 +264,8 @@ struct Segment {
   int seq0, rows;             // first sequence and number of rows
   int tile0, ends;            // the unit's last tile is in it
   int len;                    // positions of the unit
-  int unit;                   // of all units, prefixes' first; its parts lie in the slots unit + worker
-  int pad;
+  int unit;                   // of all units, prefixes' first; its parts have the numbers unit + worker
+  int row0;                   // rows of the units before it, prefixes' or own positions'
   const int32_t* table;
 };
 __device__ __forceinline__ void segment_at(const Params& P, const Cum& c, int t, int end, Segment& s) {
@@ -280,6 +285,7 @@ __device__ __forceinline__ void segment_at(const Params& P, const Cum& c, int t,
     s.len = c.len[g];
     s.table = a.prefix_tables + g * a.prefix_stride;
     s.unit = prefix_unit(P, g) + unit;
+    s.row0 = (first * a.NKV + s.h * (P.groups.first[g + 1] - first) + m * P.y.spt) * P.y.G;
   } else {
     const int r = t - tp_all, b = find(c.s, a.seqs, r);
     per = (c.s[b + 1] - c.s[b]) / a.NKV;
@@ -290,6 +296,7 @@ __device__ __forceinline__ void segment_at(const Params& P, const Cum& c, int t,
     s.len = c.len[a.groups + b];
     s.table = a.tables + b * a.table_stride;
     s.unit = P.y.punits + b * a.NKV + s.h;
+    s.row0 = (b * a.NKV + s.h) * P.y.G;
   }
   s.n = min(per - s.tile0, end - t);
   s.ends = s.tile0 + s.n == per;
@@ -493,10 +500,10 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
         ok = __all_sync(~0u, ok);
         fence_after();
         const int mid = (HD / 16 + 1) / 2 * 16, c0 = hf ? mid : 0, c1 = hf ? HD : mid;           // this warp's columns
-        const int stride = s.own ? P.y.G : P.y.prows;
-        const long long slot = (long long)(s.own ? s.unit - P.y.punits : s.unit) + worker;
+        const int stride = s.rows;
+        const long long at = part_row(s.row0, s.own ? P.y.G : P.y.prows, worker);
         const bool writes = ok && row < s.rows;
-        float* O = (s.own ? P.y.oO : P.y.pO) + slot * stride * HD + (size_t)row * 4;
+        float* O = (s.own ? P.y.oO : P.y.pO) + at * HD + (size_t)row * 4;
 #pragma unroll 1
         for (int c = c0; c < c1; c += 32) {
           uint32_t r[32];
@@ -522,7 +529,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const __grid_constant
             const float2 p = sh.l[seg & 1][set ^ (x >> 1)][x & 1][row];
             if (p.y != 0.f) L += p.x == m ? p.y : p.y * ex2((p.x - m) * sl);
           }
-          *((float2*)(s.own ? P.y.oml : P.y.pml) + slot * stride + row) = make_float2(m == -INFINITY ? m : m * sl, L);
+          *((float2*)(s.own ? P.y.oml : P.y.pml) + at + row) = make_float2(m == -INFINITY ? m : m * sl, L);
         }
       }
       n += s.n;
@@ -755,9 +762,15 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
   while (g < hi) { const int mid = (g + hi + 1) >> 1; if (P.first.first[mid] <= b) g = mid; else hi = mid - 1; }
   const int first = P.first.first[g], um = (b - first) / P.spt, mt = (P.first.first[g + 1] - first + P.spt - 1) / P.spt;
   const int pu = (first / P.spt + g) * P.NKV + h * mt + um, ou = b * P.NKV + h;                 // (see prefix_unit)
-  const int prow = (b - first - um * P.spt) * G + j;
+  const int size = P.first.first[g + 1] - first, prow = (b - first - um * P.spt) * G + j, prows = min(P.spt, size - um * P.spt) * G;
   const int pl = __ldg(P.prefix_lens + g), ol = __ldg(P.lens + b);
   int2 po = __ldcg((const int2*)P.of + pu), oo = __ldcg((const int2*)P.of + P.punits + ou);
+  // where worker 0's parts would be (see part_row): the others' offsets fit 32 bits
+  const int pieces = HD / 4, prow0 = (first * P.NKV + h * size + um * P.spt) * G, orow0 = ou * G;
+  const float2* const pml = (const float2*)P.pml + prow0 + prow;
+  const float2* const oml = (const float2*)P.oml + orow0 + j;
+  const float4* const pO = (const float4*)P.pO + (int64_t)prow0 * pieces + prow;
+  const float4* const oO = (const float4*)P.oO + (int64_t)orow0 * pieces + j;
   int lost = 0;
 #pragma unroll
   for (int w = 0; w < MAX_WORKERS; w += 32) if (w + lane < P.workers) lost |= __ldcg(P.gave_up + w + lane);
@@ -765,21 +778,18 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
   if (__any_sync(~0u, lost)) bad |= ETXB_SHARED_GAVE_UP;            // (something is unwritten: nothing is looked at)
   const int n0 = bad || pl <= 0 ? 0 : po.y - po.x + 1, n = n0 + (bad || ol <= 0 ? 0 : oo.y - oo.x + 1);
   // part i: the prefix's from worker po.x on, then the own ones
-  const int64_t ps = (int64_t)pu + po.x, os = (int64_t)ou + oo.x;
-  auto sums = [&](int i) {
-    return __ldcg(i < n0 ? (const float2*)P.pml + (ps + i) * P.prows + prow : (const float2*)P.oml + (os + i - n0) * G + j);
-  };
+  auto sums = [&](int i) { return __ldcg(i < n0 ? pml + (po.x + i) * P.prows : oml + (oo.x + i - n0) * G); };
   float M = -INFINITY, L = 0.f;
   float2 mine = make_float2(-INFINITY, 0.f);
   for (int i = lane; i < n; i += 32) {
     const float2 s = sums(i);
-    bad |= __ldcg(P.hdr + (i < n0 ? ps + i : P.pslots + os + i - n0));
+    bad |= __ldcg(i < n0 ? P.hdr + (pu + po.x + i) : P.hdr + P.pslots + (ou + oo.x + i - n0));
     M = fmaxf(M, s.x);
     if (i < 32) mine = s;
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) { M = fmaxf(M, __shfl_xor_sync(~0u, M, o)); bad |= __shfl_xor_sync(~0u, bad, o); }
-  const int pieces = HD / 4;
+  const int pstep = P.prows * pieces, ostep = G * pieces;
   float4 y[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll 1
   for (int i0 = 0; i0 < n; i0 += 32) {
@@ -797,7 +807,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int i = i0 + min(i1 + k, left - 1);
-          v[k] = __ldcg(i < n0 ? (const float4*)P.pO + ((ps + i) * pieces + piece) * P.prows + prow : (const float4*)P.oO + ((os + i - n0) * pieces + piece) * G + j);
+          v[k] = __ldcg(i < n0 ? pO + ((po.x + i) * pstep + piece * prows) : oO + ((oo.x + i - n0) * ostep + piece * G));
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -875,9 +885,10 @@ static bool lay_out(const etxb_attn_shared_args& a, int workers, unsigned char* 
   y.oslots = (long long)a.seqs * a.NKV + workers;
   size_t at = 0;
   auto take = [&](size_t n) { unsigned char* p = work + at; at += up256(n); return p; };
-  y.pO = (float*)take((size_t)y.pslots * y.prows * a.HD * 4);
+  const size_t prows = (size_t)a.seqs * a.NH + (size_t)y.prows * workers;      // (see part_row)
+  y.pO = (float*)take(prows * a.HD * 4);
   y.oO = (float*)take((size_t)y.oslots * y.G * a.HD * 4);
-  y.pml = (float*)take((size_t)y.pslots * y.prows * 8);
+  y.pml = (float*)take(prows * 8);
   y.oml = (float*)take((size_t)y.oslots * y.G * 8);
   y.hdr = (int32_t*)take((size_t)(y.pslots + y.oslots) * 4);
   y.gave_up = (int32_t*)take((size_t)workers * 4);

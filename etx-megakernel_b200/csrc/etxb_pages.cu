@@ -102,6 +102,27 @@ static cudaError_t run(const Head& h, const std::vector<int32_t>& data, int sms,
   return data.size() <= SMALL ? launch<SMALL>(h, data.data(), data.size(), grid, st) : launch<LARGE>(h, data.data(), data.size(), grid, st);
 }
 
+// Pages of one tensor, layer by layer, from an address on.
+struct Area {
+  uintptr_t at;
+  int64_t layer, page, bytes;
+  int32_t layers, pages;
+  int64_t extent() const { return page * (pages - 1) + bytes; }      // of a layer
+  int64_t size() const { return (layers > 1 ? layer * (layers - 1) : 0) + extent(); }
+};
+// Whether two areas have no byte in common, where that is told by what they span, by their layers lying between each other's (views [layers][2][pages]) or by
+// their pages doing so (views [layers][pages][2]).  Others that are apart by chance count as overlapping.
+static bool apart(const Area& x, const Area& y) {
+  if (x.at + x.size() <= y.at || y.at + y.size() <= x.at) return true;
+  auto between = [&](int64_t step, int64_t first, int64_t second) {  // pieces of `first` and `second` bytes, every `step` bytes in both
+    const int64_t d = (((int64_t)(y.at - x.at)) % step + step) % step;
+    return d >= first && d + second <= step;
+  };
+  const bool one = x.layers == 1, layers = one || x.layer == y.layer;
+  if (!one && layers && between(x.layer, x.extent(), y.extent())) return true;
+  return x.page == y.page && layers && (one || x.layer % x.page == 0) && between(x.page, x.bytes, y.bytes);
+}
+
 // 0 or the text of what is wrong
 static const char* check(const etxb_pages_args& a) {
   if (a.n_tensors < 1 || a.n_tensors > ETXB_PAGES_MAX_TENSORS || a.layers < 1 || a.layers > 65535) return "1 .. 4 tensors of 1 .. 65535 layers";
@@ -128,6 +149,17 @@ static const char* check(const etxb_pages_args& a) {
     if (!one && s0 < d1 && d0 < s1) return "source and destination are one pool or apart";
     if (i == 0) same = one;
     if (one != same) return "source and destination are one pool for every tensor, or for none";
+  }
+  // (all tensors are copied at once, in no order: what one reads or writes no other one writes)
+  for (int i = 0; a.n_copy && i < a.n_tensors; ++i) {
+    const etxb_page_tensor& t = a.t[i];
+    const Area to = {(uintptr_t)t.dst, t.dst_layer, t.dst_page, t.page_bytes, a.layers, a.dst_pages};
+    for (int k = 0; k < a.n_tensors; ++k) {
+      if (k == i) continue;
+      const etxb_page_tensor& o = a.t[k];
+      if (!apart(to, {(uintptr_t)o.src, o.src_layer, o.src_page, o.page_bytes, a.layers, a.src_pages}) ||
+          !apart(to, {(uintptr_t)o.dst, o.dst_layer, o.dst_page, o.page_bytes, a.layers, a.dst_pages})) return "tensors overlap";
+    }
   }
   std::vector<uint8_t> taken(a.n_copy ? (size_t)a.dst_pages : 0, 0);
   for (int i = 0; i < a.n_copy; ++i) {

@@ -69,7 +69,8 @@ def _check(rc):
 
 def copy_pages(src, dst, src_ids, dst_ids, stream=None) -> None:
     """Page dst_ids[i] of the pool `dst` becomes page src_ids[i] of the pool `src`, in every layer and tensor (src and dst: lists of tensors, or one;
-    the same pool, or two with pages of one size).  Within one pool no page may be both read and written; no page is written twice."""
+    the same pool, or two with pages of one size; pages of different tensors do not overlap).  Within one pool no page may be both read and written; no page is
+    written twice."""
     src, dst = _pool("src", src), _pool("dst", dst)
     if len(src) != len(dst) or src[0].shape[0] != dst[0].shape[0] or any(s.shape[2:] != d.shape[2:] or s.dtype != d.dtype for s, d in zip(src, dst)):
         raise ValueError("copy_pages: pools of the same tensors, layers and pages")

@@ -240,13 +240,14 @@ int32_t etxb_sample(int device, const etxb_sample_args* args, size_t bytes, void
 /* Pages of a paged KV cache.  One call copies pages (of all layers and tensors: keys, values) and brings block tables up to date; the lists are host
  * memory, are checked (ETXB_E_ARG) and copied before the call returns, and the device needs none of its own.
  *   copies    page dst_ids[i] := page src_ids[i] of every tensor and layer.  Within one pool no page is both read and written; no page is written twice.
+ *             Pages of different tensors do not overlap (they may lie between each other's: keys and values in one allocation).
  *   set       tables[set_rows[i]][set_cols[i]] := set_pages[i]
  *   share     the first `shared` entries of each of share_rows := those of row share_from
  *   remap     in the first remap_entries[i] entries of row remap_rows[i], a page that is a source of the copies gets the number it was copied to (a call
  *             without set and share) */
 #define ETXB_PAGES_MAX_TENSORS 4
 typedef struct etxb_page_tensor {
-  const void* src; void* dst;                             /* the pools: page p of layer l lies at base + l * layer + p * page (bytes, multiples of 16) */
+  const void* src; void* dst;                             /* the pools: page p of layer l lies at base + l * layer + p * page (bytes, multiples of 16), a layer behind the pages of the last */
   int64_t src_layer, src_page, dst_layer, dst_page;
   int64_t page_bytes;
 } etxb_page_tensor;

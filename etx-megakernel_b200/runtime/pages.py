@@ -17,12 +17,15 @@ _BYTES = C.sizeof(L.PagesArgs)
 
 
 def _pool(name, tensors):
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    try:
+        tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    except TypeError:
+        raise ValueError(f"{name}: tensors, got {type(tensors).__name__}") from None
     if not 1 <= len(tensors) <= 4:
         raise ValueError(f"{name}: 1 to 4 tensors, got {len(tensors)}")
     for i, t in enumerate(tensors):
         cuda_tensor(f"{name}[{i}]", t, (t.dtype,) if isinstance(t, torch.Tensor) else (), inner=False)
-        if t.dim() < 3 or t.shape[:2] != tensors[0].shape[:2] or not t[0, 0].is_contiguous() or t.numel() == 0:
+        if t.dim() < 3 or t.shape[:2] != tensors[0].shape[:2] or t.numel() == 0 or not t[0, 0].is_contiguous():
             raise ValueError(f"{name}[{i}]: shape {tuple(t.shape)}, expected [layers][pages][...] with {tuple(tensors[0].shape[:2])} and pages without gaps")
     same_device(tensors[0].device, **{f"{name}[{i}]": t for i, t in enumerate(tensors)})
     return tensors

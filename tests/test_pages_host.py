@@ -315,3 +315,10 @@ def test_what_counts_as_apart_is_apart(seed):
         assert apart or not says                                        # (never taken for apart; some that are may be refused)
         seen.add((apart, says))
     assert (True, True) in seen and (False, False) in seen
+
+
+@pytest.mark.parametrize("bad", [5, None, torch.zeros((0, 3, 4)), torch.zeros((1, 0, 4)), torch.zeros((1, 3, 0)), [torch.zeros((1, 3, 4)), torch.zeros(0)], [torch.zeros((2, 3))]])
+def test_what_is_no_pool_is_a_value_error(on_host, bad):
+    for f in (lambda: HostPool(bad, 2, 2), lambda: copy_pages(bad, [torch.zeros((1, 3, 4))], [0], [1]), lambda: copy_pages([torch.zeros((1, 3, 4))], bad, [0], [1])):
+        with pytest.raises(ValueError, match="tensors|src|dst"):
+            f()

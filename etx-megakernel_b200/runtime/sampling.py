@@ -19,6 +19,17 @@ _T, _BYTES = torch.Tensor, C.sizeof(L.SampleArgs)
 _pack = struct.Struct("10Pq4i3fi").pack                            # (the structure's fields in order, quicker than through ctypes)
 
 
+def _count(name, v) -> int:
+    """A whole number, as far as a row has tokens (below 1: 0)."""
+    try:
+        n = int(v)
+        if n == v:
+            return max(min(n, MAX_V), 0)
+    except (TypeError, ValueError, OverflowError):
+        pass
+    raise ValueError(f"{name}: a whole number or a tensor, got {v!r}")
+
+
 class Sampled(NamedTuple):
     tokens: torch.Tensor       # int32 [rows]; -1 where no token of a row is allowed
     logprobs: torch.Tensor     # float32 [rows]: of the token among the kept ones
@@ -74,7 +85,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=Non
     def setting(name, v, dtype):
         """The setting as (address of one value per row, value for all)."""
         if not isinstance(v, _T):
-            return 0, max(min(int(v), MAX_V), 0) if dtype is torch.int32 else C.c_float(v).value
+            return 0, _count(name, v) if dtype is torch.int32 else C.c_float(v).value
         keep.append(vector(name, v, dtype, rows, index))
         return v.data_ptr(), 0
     temperatures, temperature = setting("temperature", temperature, torch.float32)

@@ -145,7 +145,8 @@ class DecodeProgram:
             raise ValueError("generate: tokens are drawn behind single launches of a model whose logits lie on one GPU")
         prompt = [int(x) for x in prompt]
         n = len(prompt) + n_gen - 1
-        if n + 2 > self.buf["token_in"].numel() or start_pos + n > self.maxlen:
+        Q.check_prompt(prompt, self.d.V, n, self.maxlen, start_pos)
+        if n + 2 > self.buf["token_in"].numel():
             raise ValueError("sequence longer than the session was sized for")
         tin = torch.zeros_like(self.buf["token_in"])
         tin[:len(prompt)] = torch.tensor(prompt, dtype=torch.int32)
@@ -160,6 +161,7 @@ class DecodeProgram:
 
     def generate_host(self, prompt, n_gen: int, start_pos: int = 0):
         """The same through host buffers: every step's token goes host -> device and its result device -> host."""
+        Q.check_prompt(prompt, self.d.V, len(prompt) + n_gen - 1, self.maxlen, start_pos)
         toks, ms = self.session.decode_host(np.asarray(prompt, np.int32), len(prompt) + n_gen - 1, start_pos)
         return toks[len(prompt) - 1:], ms
 

@@ -411,7 +411,8 @@ class MlaProgram:
         runtime.Sampling whose tokens are drawn on the device (their log-probabilities are left in self.logprobs, [n_gen][1])."""
         prompt = [int(x) for x in prompt]
         n = len(prompt) + n_gen - 1
-        if n + 2 > self.buf["token_in"].numel() or start_pos + n > self.maxlen:
+        Q.check_prompt(prompt, self.d.V, n, self.maxlen, start_pos)
+        if n + 2 > self.buf["token_in"].numel():
             raise ValueError("sequence longer than the session was sized for")
         tin = torch.zeros_like(self.buf["token_in"])
         tin[:len(prompt)] = torch.tensor(prompt, dtype=torch.int32)
@@ -425,6 +426,7 @@ class MlaProgram:
         return self.buf["token_out"][len(prompt) - 1:n].cpu().numpy()
 
     def generate_host(self, prompt, n_gen: int, start_pos: int = 0):
+        Q.check_prompt(prompt, self.d.V, len(prompt) + n_gen - 1, self.maxlen, start_pos)
         toks, ms = self.session.decode_host(np.asarray(prompt, np.int32), len(prompt) + n_gen - 1, start_pos)
         return toks[len(prompt) - 1:], ms
 

@@ -82,6 +82,17 @@ class Dims:
         return (self.NH + 2 * self.NKV) * self.HD
 
 
+def check_prompt(tokens, vocab: int, n: int, maxlen: int, start_pos: int = 0):
+    """Refuses tokens that the embedding does not have and positions start_pos .. start_pos + n - 1 that the cache does not have: the step trusts both."""
+    tokens = np.asarray(tokens, np.int64)
+    if tokens.size and not 0 <= tokens.min() <= tokens.max() < vocab:
+        raise ValueError(f"tokens outside the vocabulary of {vocab}")
+    if start_pos < 0:
+        raise ValueError(f"from position {start_pos}")
+    if start_pos + n > maxlen:
+        raise ValueError("sequence longer than the session was sized for")
+
+
 def load_dims(config=None, layers: int | None = None, name: str | None = None) -> Dims:
     """config: a bundled name ("qwen3-30b-a3b", "qwen3-8b"), a path to a HF config.json, or the dict itself."""
     if config is None:

@@ -36,6 +36,8 @@ def _check(q, kc, vc, tables, lens, prefix_tables, prefix_lens, out, status):
     cuda_tensor("kc", kc, _BF16, (None, None, None, 16, 8), inner=False)
     pages, NKV, hd8 = kc.shape[:3]
     HD = 8 * hd8
+    if not HD or not NKV:
+        raise ValueError(f"kc: {NKV} heads of {HD}")
     cuda_tensor("vc", vc, _BF16, (pages, NKV, HD, 16), inner=False)
     if kc.stride()[1:] != (hd8 * 128, 128, 8, 1) or vc.stride()[1:] != (HD * 16, 16, 1):
         raise ValueError("kc, vc: a page has no gaps")

@@ -237,7 +237,7 @@ class BatchProgram:
                               token_in=b["token_in"], token_out=b["token_out"], token_time=b["token_time"])
 
     def step(self, t: int, pos: int, write_next: bool, wait: bool = True):
-        if self.cache is not None and not (0 <= pos < self.maxlen and 0 <= t < self.buf["token_in"].shape[0]):
+        if self.cache is not None and not (0 <= pos < self.maxlen and 0 <= t < self.buf["token_in"].shape[0] - bool(write_next)):
             raise ValueError(f"step {t} at position {pos}: over pages there are {self.buf['token_in'].shape[0]} steps and {self.maxlen} positions")
         self.session.set_step(tok=t, pos=pos, write_next=int(write_next))
         if wait:

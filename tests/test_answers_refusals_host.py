@@ -193,7 +193,7 @@ def test_answers_go_on_behind_a_first_token_that_there_is_none(on_host, monkeypa
     assert got[:, 0].tolist() == [-1, 7, -1] and prog.runs == [([[0, 7, 0]], 2, 3)]
 
 
-@pytest.mark.parametrize("t,pos", [(0, -1), (0, 128), (3, 10 ** 6), (-1, 5), (64, 5)])
+@pytest.mark.parametrize("t,pos", [(0, -1), (0, 128), (3, 10 ** 6), (-1, 5), (64, 5), (63, 5)])
 def test_steps_over_pages_stay_inside_the_tables(on_host, t, pos):  # noqa: F811
     """A step's position names an entry of each column's table, and the page in it the memory that is written."""
     class Recorded:

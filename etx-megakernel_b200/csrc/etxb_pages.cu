@@ -26,6 +26,7 @@ struct Head {
   int32_t n_tensors, layers;
   int32_t n_copy, n_set, n_share, n_remap;     // data: n_copy (src, dst) pairs -- ascending in src where there is a remap --, n_set (row, column, page)
   int32_t share_from, shared;                  // triples, n_share rows, n_remap (row, entries) pairs
+  int32_t n_move;                              // n_copy, or 0 where the pairs are there for the renumbering alone
 };
 template <int N>
 struct Params {
@@ -64,10 +65,10 @@ __global__ void __launch_bounds__(THREADS) update_kernel(const __grid_constant__
       if (lo < h.n_copy && p.data[2 * lo] == page) row[c] = p.data[2 * lo + 1];
     }
   }
-  const long long units = (long long)h.n_copy * h.layers * h.n_tensors;
+  const long long units = (long long)h.n_move * h.layers * h.n_tensors;
   for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int pair = (int)(u % h.n_copy);
-    const long long lt = u / h.n_copy;
+    const int pair = (int)(u % h.n_move);
+    const long long lt = u / h.n_move;
     const etxb_page_tensor& t = h.t[lt % h.n_tensors];
     const long long layer = lt / h.n_tensors;
     const uint4* s = (const uint4*)((const char*)t.src + layer * t.src_layer + p.data[2 * pair] * t.src_page);
@@ -95,7 +96,7 @@ static cudaError_t launch(const Head& h, const int32_t* data, size_t n, int grid
 constexpr int SMALL = 192, LARGE = 7900;
 
 static cudaError_t run(const Head& h, const std::vector<int32_t>& data, int sms, cudaStream_t st) {
-  const long long units = (long long)h.n_copy * h.layers * h.n_tensors;
+  const long long units = (long long)h.n_move * h.layers * h.n_tensors;
   const long long entries = std::max<long long>(h.n_set, (long long)h.n_share * h.shared);
   const long long blocks = std::max(std::max(units, (entries + THREADS - 1) / THREADS), (long long)h.n_remap);
   const int grid = (int)std::max<long long>(1, std::min<long long>(blocks, (long long)sms * 8));
@@ -227,7 +228,8 @@ static cudaError_t run_all(const etxb_pages_args& a, int sms, cudaStream_t st) {
     for (int i = 0; i < h.n_share; ++i, ++r) data.push_back(a.share_rows[r]);
     const size_t fixed = data.size();
     int m = 0;
-    do {                                       // (once, but for a renumbering of many rows: the copies go with its first part)
+    do {                                       // (once, but for a renumbering of many rows: the pages move with its first part)
+      h.n_move = m == 0 ? h.n_copy : 0;
       data.resize(fixed);
       h.n_remap = std::min(a.n_remap - m, (int)((LARGE - fixed) / 2));
       for (int i = 0; i < h.n_remap; ++i, ++m) { data.push_back(a.remap_rows[m]); data.push_back(a.remap_entries[m]); }

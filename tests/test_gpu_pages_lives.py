@@ -76,3 +76,17 @@ def test_only_what_has_no_room_is_refused(seed):
         for _ in range(ROWS):
             pool.open(WIDTH * P)
     assert e.value.status == "E_FULL" and len(pool.rows()) == N // WIDTH and pool.free_pages == N % WIDTH
+
+
+def test_renumbering_more_rows_than_a_launch_lists():
+    """2600 rows of which 2500 go on, in lists of 1975 and the rest: pages move once, every entry is renumbered once."""
+    n = 2600
+    k = torch.randint(-30000, 30000, (2, 3 * n, 8), device=DEV, dtype=torch.int16)
+    pool = PagePool([k], n, 3)
+    rows = [pool.open(40) for _ in range(n)]
+    held = {r: k[:, pool.pages_of(r)].clone() for r in rows[100:]}
+    pool.close(rows[:100])
+    assert pool.compact() == 300 and pool.free_pages == 300
+    tab = pool.tables.cpu()
+    assert all(tab[r].tolist() == pool.pages_of(r) for r in rows[100:]) and max(max(pool.pages_of(r)) for r in rows[100:]) == 3 * n - 301
+    assert all(torch.equal(k[:, pool.pages_of(r)], c) for r, c in held.items())

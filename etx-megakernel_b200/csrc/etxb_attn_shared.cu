@@ -25,7 +25,7 @@
 // at once, so products, softmax and copies of neighbouring tiles and segments overlap.  Every wait is bounded, and every role waits for every phase of a barrier.
 //
 // Measured (32 q heads of 128): 2 sequences over 131000 shared positions, 8 kv heads, 125 us, 4.3 TB/s (539 MB: 83 us); 64 over 32500 103 us (199 MB: 30 us; products: 21);
-// 32 over 8150, 4 kv heads, 36 us; 4 over 1024 18 us, mostly the host's.  A tile takes 2900 to 3000 clocks: its bytes 2900 from HBM with all SMs at it, its products 1800.  Tried and slower: one set of softmax warps; P in columns of its own (softmax waits for P V);
+// 32 over 8150, 4 kv heads, 35 us; 4 over 1024 19 us, mostly the host's.  Of 256 elements, 4 kv heads: 16 sequences over 32500 67 us (148 MB: 23 us), in tiles of 64 positions.  A tile takes 2900 to 3000 clocks: its bytes 2900 from HBM with all SMs at it, its products 1800.  Tried and slower: one set of softmax warps; P in columns of its own (softmax waits for P V);
 // the second kernel launched ahead of the first one's end (its blocks wait on the SMs).  Contexts of their own, a short segment each, take 4500 clocks a tile, most of it the way from Q to the first product.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -234,7 +234,8 @@ __device__ __forceinline__ int share(int total, int w, int workers) {
 }
 
 // Tiles [t0, t1) of a worker.  Tiles of prefixes and of sequences' own positions have workers of their own, as many as their time asks for: a tile of own
-// positions, in short units, takes OWN_COST / PREFIX_COST times as long as one of a prefix (64 sequences over 32500 positions, 500 of their own, in a graph: 2 : 3 98 us, 1 : 1 113, 1 : 2 104).  No worker among those that share is without a tile.
+// positions, in short units, takes OWN_COST / PREFIX_COST times as long as one of a prefix (64 sequences over 32500 positions, 500 of their own, 8 kv heads of 128, in a graph: 2 : 3 98 us, 1 : 1 113, 1 : 2 104;
+// other shapes take the same, which was not measured for them).  No worker among those that share is without a tile.
 constexpr int PREFIX_COST = 2, OWN_COST = 3;
 __device__ __forceinline__ void share_of(int tp, int to, int W, int w, int& t0, int& t1) {
   int wp = tp, wo = to;                                             // fewer tiles than workers: one each

@@ -18,7 +18,8 @@
 // Logits of 32 bits (sums_kernel).  Bins by the first 11 bits of the value, then the next 11 and the last 10 of one bin: three passes for a border.  A bin has a
 // number of tokens and a sum of weights, which are integers: exp in 64 bits times 2^S with S = 62 - ceil(log2 V), so that a row's sum fits 63 bits, is
 // exact whatever the order, and a weight is off by 2^-(S+1) <= 2^-43 of the largest.
-//   13 rows of 50257 36 us without cuts, 44 with top-k and top-p, 8 of them a lookup; 256 rows of 151936 528 and 438, where bins have more than LIST tokens.  Four copies
+//   13 rows of 50257 36 us without cuts, 44 with top-k and top-p, 8 of them a lookup; 256 rows of 151936 467 and 473 (their bytes: 24), 64 rows 135: one block
+//   a row (two for 64) keeps nothing of it on the chip and reads it again for every pass, and bins have more than LIST tokens.  Four copies
 //   of the first bins, for four lanes each, gave nothing, nor did an exp in 32 bits (1 us): it is the passes and what the blocks wait for between them.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

@@ -1,6 +1,7 @@
 """Decode attention for sequences that share prefixes (etxb_attn_shared): keys and values of a prefix are read once for all its sequences.
 
-Beside the tiles of the step (ops/attn.py), which read every sequence's whole context; no counterpart in the reference."""
+A call of its own, beside the tiles of the step (ops/attn.py), which the programs use and which read every sequence's whole context.  No counterpart in the
+reference."""
 from __future__ import annotations
 
 import ctypes as C

@@ -64,7 +64,9 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=Non
     A row's allowed tokens (neither -inf nor NaN) stand in the order "larger logit first, equal ones by index" with the weights
     exp((logit - largest) / temperature).  top_k keeps the first so many (0: all); top_p of those the ones with less than its share of their sum before
     them (1: all); min_p the ones of at least that share of the largest weight (0: all); one is always kept.  The token is the first whose sum up to and
-    with itself exceeds u times the sum of the kept ones.  temperature 0: the largest logit.  Equal inputs give equal tokens, whatever else runs.
+    with itself exceeds u times the sum of the kept ones.  temperature 0: the largest logit.  Equal inputs give equal tokens, whatever else runs.  Weights of 16-bit logits
+    are 64-bit numbers; those of fp32 logits are whole steps of 2^-43 of the largest or finer, so that tokens of about a step and less may be counted, or left out, next to a
+    border (a top_p within 2^-24 of 1 over a long, even tail).
 
     temperature, top_k, top_p, min_p: numbers, or tensors [rows] (float32; top_k int32).  tokens / next_tokens: int32 tensors [rows] that take the tokens
     (the second one them once more, 0 where there is none: the next step's input).  stream: a raw handle or torch stream; None is the current one.  What

@@ -255,6 +255,8 @@ class BatchProgram:
             raise ValueError(f"{prompts.shape[0]} prompts for a batch of {self.B}")
         P = prompts.shape[1]
         n = P + n_gen - 1
+        if sampling is not None:
+            drawing.check_sizes(P, n_gen)
         Q.check_prompt(prompts, self.d.V, n, self.maxlen)
         if n + 2 > self.buf["token_in"].shape[0]:
             raise ValueError("sequence longer than the session was sized for")

@@ -145,6 +145,8 @@ class DecodeProgram:
             raise ValueError("generate: tokens are drawn behind single launches of a model whose logits lie on one GPU")
         prompt = [int(x) for x in prompt]
         n = len(prompt) + n_gen - 1
+        if sampling is not None:
+            drawing.check_sizes(len(prompt), n_gen)
         Q.check_prompt(prompt, self.d.V, n, self.maxlen, start_pos)
         if n + 2 > self.buf["token_in"].numel():
             raise ValueError("sequence longer than the session was sized for")

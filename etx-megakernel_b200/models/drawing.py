@@ -6,6 +6,11 @@ import torch
 from ..runtime import Sampling, sample
 
 
+def check_sizes(prompt: int, n_gen: int):
+    if prompt < 1 or n_gen < 0:
+        raise ValueError(f"{n_gen} tokens drawn behind a prompt of {prompt}")
+
+
 def check(prog, n: int, rows: int, sampling: Sampling):
     """Refuses what `run` would refuse at its first draw of n: settings, a seed, random numbers of another shape, type or place."""
     if not isinstance(sampling, Sampling):

@@ -411,6 +411,8 @@ class MlaProgram:
         runtime.Sampling whose tokens are drawn on the device (their log-probabilities are left in self.logprobs, [n_gen][1])."""
         prompt = [int(x) for x in prompt]
         n = len(prompt) + n_gen - 1
+        if sampling is not None:
+            drawing.check_sizes(len(prompt), n_gen)
         Q.check_prompt(prompt, self.d.V, n, self.maxlen, start_pos)
         if n + 2 > self.buf["token_in"].numel():
             raise ValueError("sequence longer than the session was sized for")

@@ -10,6 +10,7 @@ from etx_megakernel_b200.models import batched as BT  # noqa: E402
 from etx_megakernel_b200.models import decode as D  # noqa: E402
 from etx_megakernel_b200.models import dsv2 as M  # noqa: E402
 from etx_megakernel_b200.models import qwen as Q  # noqa: E402
+from etx_megakernel_b200.runtime import Sampling  # noqa: E402
 
 DIMS = Q.Dims(name="small", H=512, NH=8, NKV=2, HD=128, INTER=0, L=3, V=1504, qk_norm=True, moe=True, E=16, TOPK=4, MI=128, norm_topk=True)
 
@@ -44,3 +45,12 @@ def test_positions_outside_the_cache(kind, prompt, n, start):
     for f in (p.generate, p.generate_host):
         with pytest.raises(ValueError, match="session was sized for|position"):
             f(prompt, n, start_pos=start)
+
+
+@pytest.mark.parametrize("kind", [D.DecodeProgram, M.MlaProgram, BT.BatchProgram])
+def test_tokens_are_drawn_behind_a_prompt(kind):
+    """Without a token of a prompt there are no logits to draw from."""
+    p = program(kind)
+    for prompt, n in (([], 4), ([3], -1)):
+        with pytest.raises(ValueError, match="behind a prompt"):
+            p.generate([prompt] if kind is BT.BatchProgram else prompt, n, sampling=Sampling())

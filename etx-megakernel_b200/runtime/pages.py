@@ -170,7 +170,8 @@ class PagePool:
     def extend(self, rows, length, stream=None) -> None:
         """Pages up to `length` positions (a number, or one per row) for each of `rows`; a length is never reduced."""
         rows = _ints("rows", rows)
-        lengths = _ints("length", [length] * len(rows) if isinstance(length, int) else length)
+        length = length.tolist() if hasattr(length, "tolist") else length
+        lengths = _ints("length", length if isinstance(length, (list, tuple, range)) else [length] * len(rows))
         if len(lengths) != len(rows):
             raise ValueError("extend: each row with one length")
         _check(self._lib.etxb_pool_extend(self._h, rows, lengths, len(rows), self._stream(stream)))

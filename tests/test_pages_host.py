@@ -322,3 +322,15 @@ def test_what_is_no_pool_is_a_value_error(on_host, bad):
     for f in (lambda: HostPool(bad, 2, 2), lambda: copy_pages(bad, [torch.zeros((1, 3, 4))], [0], [1]), lambda: copy_pages([torch.zeros((1, 3, 4))], bad, [0], [1])):
         with pytest.raises(ValueError, match="tensors|src|dst"):
             f()
+
+
+@pytest.mark.parametrize("number", [np.int64, np.int32, torch.tensor, int])
+def test_a_length_for_all_rows_is_any_whole_number(on_host, number):
+    pool = HostPool([torch.zeros((1, 12, 4))], 3, 4, page_len=4)
+    rows = [pool.open(3) for _ in range(3)]
+    pool.extend(rows, number(9))
+    assert [pool.length_of(r) for r in rows] == [9, 9, 9]
+    pool.extend(np.array(rows), np.array([10, 11, 12]))
+    assert [pool.length_of(r) for r in rows] == [10, 11, 12]
+    with pytest.raises(ValueError, match="one length"):
+        pool.extend(rows, [13])
